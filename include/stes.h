@@ -455,6 +455,36 @@ int stes_gru_noalloc_prepare(void);
 int stes_mingru_scan_fwd(const uint16_t* pre, const float* h0, uint16_t* h, int B, int T, int H, void* stream);
 int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h, const float* dh, int64_t ld_dh, uint16_t* dpre,
                          int B, int T, int H, void* stream);
+/* Gated linear recurrence over sequences of any length (the minGRU cell, reference model/min_gru.py:76-92, for whole videos, frame
+ * streams and ragged batches; stes_mingru_scan_* is its form for short clips with a fixed initial state).  Per sequence b and
+ * channel c, in scan order s = 0 .. len-1 (reverse == 0: frame t = s; reverse != 0: t = len-1-s):
+ *   z = sigmoid(pre[t][c]),  a = 1 - z = sigmoid(-pre[t][c]),  x_s = a x_{s-1} + z pre[t][H+c],  x_{-1} = h0,  h[t][c] = x_s
+ * and h_last = x_{len-1} (h0 where len = 0).  lengths (int32 [B], values clamped to [0, T]; NULL: T each): rows t >= len of h
+ * (and, in backward, of dpre) are written as zeros, whatever pre and dh hold there.
+ * pre, h, dh, dpre: bf16 (f32 == 0) or fp32 (f32 == 1); ld_*: elements between frames, bs_*: between sequences; the last dimension is
+ * contiguous.  States, h0, h_last and their gradients are fp32, and the recurrence runs in fp32.  h0: row b at h0 + b * bs_h0
+ * (bs_h0 = 0: one state for the whole batch; NULL: zeros).  h_last may be h0's own memory when bs_h0 >= H (a stream's state in
+ * place, bs_hl = bs_h0); nothing else may overlap.
+ * states [B][ceil(T / STES_SCAN_BLOCK)][H] (fp32, optional): the state in front of every STES_SCAN_BLOCK-th step; what
+ * stes_gated_scan_bwd recomputes x from (it reads neither h nor h0).
+ * Backward: l_s = dh_s + a_{s+1} l_{s+1} (+ dh_last at s = len-1), d gate = l_s (cand_s - x_{s-1}) z a, d cand = l_s z,
+ * dh0 [B][H] = a_0 l_0 (dh_last where len = 0).  dh or dh_last may be NULL (zeros); dh0 may be NULL; dh0_sum [H] (optional, needs dh0):
+ * the sum of dh0 over the batch in a fixed order, for an initial state that the batch shares.
+ * T = 0 is a call (h_last = h0).  ws: stes_gated_scan_ws_bytes(B, T, H) bytes, contents irrelevant; calls that may overlap need one each.
+ * Results do not depend on scheduling beyond the association of the time axis: see stes_scan.hip. */
+#define STES_SCAN_BLOCK 128
+typedef struct {
+    const void* pre; int64_t ld_pre, bs_pre;
+    const float* h0; int64_t bs_h0; const int32_t* lengths;
+    void* h; int64_t ld_h, bs_h; float* h_last; int64_t bs_hl; float* states;
+    const void* dh; int64_t ld_dh, bs_dh; const float* dh_last; int64_t bs_dhl;
+    void* dpre; int64_t ld_dpre, bs_dpre; float* dh0; float* dh0_sum;
+    void* ws; int64_t ws_bytes;
+    int32_t B, T, H, f32, reverse;
+} stes_gated_scan_args;
+int64_t stes_gated_scan_ws_bytes(int B, int T, int H);
+int stes_gated_scan_fwd(const stes_gated_scan_args* a, void* stream);
+int stes_gated_scan_bwd(const stes_gated_scan_args* a, void* stream);
 /* nn.Dropout of GRUPrediction (model/modules.py:32): out = x*mask, mask in {0, 1/(1-p)} from a counter hash. */
 int stes_dropout(const uint16_t* x, uint16_t* out, uint16_t* mask, int64_t n, float p, uint32_t seed, void* stream);
 /* Weighted-mean cross entropy + masked L1 on sigmoid(loc) (train_e2e_spatial.py:566-593) and their
@@ -464,6 +494,35 @@ int stes_dropout(const uint16_t* x, uint16_t* out, uint16_t* mask, int64_t n, fl
 int stes_loss(const float* logits, int64_t ldl, const float* loc, int64_t ldloc, const int64_t* label, const float* xy,
               int M, int C, float fg_weight, float grad_scale, const float* ext_denoms, float* out_loss,
               uint16_t* dlogits, uint16_t* dloc, void* stream);
+/* Distillation from a teacher's top logits, beside stes_loss (no counterpart in the reference).  Per row m of logits [M][V]
+ * (bf16 or fp32), with idx / val [M][k] the teacher's top classes and their logits (k <= STES_DISTILL_MAX_K; idx int64 or int32, val fp32
+ * or bf16) and tau = temperature:
+ *   p = softmax(val[m] / tau) over the entries with idx >= 0,  P_v = sum of p over the entries with idx = v,
+ *   q = softmax(logits[m] / tau) over all V classes,  KL_m = sum_v P_v (log P_v - log q_v)  (entries with P_v = 0 count nothing)
+ *   loss = tau^2 / denom * sum_m weight[m] KL_m,   dlogits[m][v] = grad_scale * upstream * weight[m] tau / denom * (q_v - P_v)
+ * weight NULL: ones; upstream (device, one float) NULL: one.  Rows whose weight is 0 or that list no entry (all idx < 0, or every val
+ * -inf) add nothing to the loss and have a gradient of zero whatever their logits hold.  An idx >= V makes its row's KL and gradient
+ * NaN.  Softmax statistics and sums are fp32.
+ * stes_distill: loss [1] and, when dlogits is given, the gradient in the same pass over the logits; stats [M][2] (optional):
+ * the row's maximum and 1 / sum exp((logits - max) / tau), from which stes_distill_bwd computes the gradient later.
+ * dlogits: fp32 (d_f32) or bf16, written, or added to when accumulate != 0; it must not overlap logits.  Columns from V up are
+ * not touched.  ws: stes_distill_ws_floats(M, V) floats.  M = 0 is a call (loss 0).  Sums are taken in a fixed order. */
+#define STES_DISTILL_MAX_K 64
+typedef struct {
+    const void* logits; int64_t ld; int32_t f32;
+    const void* idx; int64_t ld_idx; int32_t idx_i64;
+    const void* val; int64_t ld_val; int32_t val_f32;
+    const float* weight;
+    int32_t M, V, k;
+    float temperature; double denom;
+    float grad_scale; const float* upstream;
+    float* loss; float* stats;
+    void* dlogits; int64_t ld_d; int32_t d_f32; int32_t accumulate;
+    float* ws; int64_t ws_floats;
+} stes_distill_args;
+int64_t stes_distill_ws_floats(int M, int V);
+int stes_distill(const stes_distill_args* a, void* stream);
+int stes_distill_bwd(const stes_distill_args* a, void* stream);
 /* torch.optim.AdamW update over a flat fp32 range (model/common.py:40, step() :61-75). */
 int stes_adamw(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1, float beta2, float eps,
                float weight_decay, int step, float grad_mul, void* stream);

@@ -98,7 +98,34 @@ GruArgs = _struct("GruArgs", [
     ("dgi", _P), ("dgh", _P), ("dhstate", _P),
     ("B", _I32), ("T", _I32), ("H", _I32), ("ws_floats", _I64)])
 
+GatedScanArgs = _struct("GatedScanArgs", [
+    ("pre", _P), ("ld_pre", _I64), ("bs_pre", _I64),
+    ("h0", _P), ("bs_h0", _I64), ("lengths", _P),
+    ("h", _P), ("ld_h", _I64), ("bs_h", _I64), ("h_last", _P), ("bs_hl", _I64), ("states", _P),
+    ("dh", _P), ("ld_dh", _I64), ("bs_dh", _I64), ("dh_last", _P), ("bs_dhl", _I64),
+    ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
+    ("ws", _P), ("ws_bytes", _I64),
+    ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
+SCAN_BLOCK = 128            # STES_SCAN_BLOCK in include/stes.h
+
+DistillArgs = _struct("DistillArgs", [
+    ("logits", _P), ("ld", _I64), ("f32", _I32),
+    ("idx", _P), ("ld_idx", _I64), ("idx_i64", _I32),
+    ("val", _P), ("ld_val", _I64), ("val_f32", _I32),
+    ("weight", _P),
+    ("M", _I32), ("V", _I32), ("k", _I32),
+    ("temperature", _F32), ("denom", _F64),
+    ("grad_scale", _F32), ("upstream", _P),
+    ("loss", _P), ("stats", _P),
+    ("dlogits", _P), ("ld_d", _I64), ("d_f32", _I32), ("accumulate", _I32),
+    ("ws", _P), ("ws_floats", _I64)])
+DISTILL_MAX_K = 64          # STES_DISTILL_MAX_K
+
 _SIGS = {
+    "stes_gated_scan_fwd": [_P, _P],
+    "stes_gated_scan_bwd": [_P, _P],
+    "stes_distill": [_P, _P],
+    "stes_distill_bwd": [_P, _P],
     "stes_gemm": [_P, _P],
     "stes_wgrad": [_P, _P],
     "stes_gemm_small2": [_P, _P],
@@ -153,7 +180,7 @@ _SIGS = {
     "stes_cast_bf16_multi": [_P, _I32, _I32, _P],
 }
 EXPORTS = ["stes_version", "stes_last_error", "stes_gsm_bwd_conv_ws_floats", "stes_gru_ws_floats", "stes_wgrad_ws_floats",
-           "stes_augment_ws_floats", "stes_gru_set_spin_limit", "stes_gru_noalloc_prepare", "stes_set_deterministic"] + list(_SIGS)
+           "stes_augment_ws_floats", "stes_gated_scan_ws_bytes", "stes_distill_ws_floats", "stes_gru_set_spin_limit", "stes_gru_noalloc_prepare", "stes_set_deterministic"] + list(_SIGS)
 
 
 def lib():
@@ -173,6 +200,10 @@ def lib():
         L.stes_wgrad_ws_floats.restype = C.c_int64
         L.stes_augment_ws_floats.argtypes = [C.c_int, C.c_int, C.c_int]
         L.stes_augment_ws_floats.restype = C.c_int64
+        L.stes_gated_scan_ws_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+        L.stes_gated_scan_ws_bytes.restype = C.c_int64
+        L.stes_distill_ws_floats.argtypes = [C.c_int, C.c_int]
+        L.stes_distill_ws_floats.restype = C.c_int64
         L.stes_gru_set_spin_limit.argtypes = [C.c_int]
         L.stes_gru_set_spin_limit.restype = C.c_int
         L.stes_gru_noalloc_prepare.argtypes = []
@@ -221,6 +252,20 @@ def check(rc: int, what: str):
 
 def stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+def guard_leaves(node):
+    """For the outputs' `grad_fn` of autograd functions that may be captured into a graph.  The node that accumulates a leaf's gradient
+    keeps the stream on which it was made for as long as some autograd graph holds it; a backward pass that is captured while an
+    eager graph of the same leaf lives would pull that stream into the capture, which ends the process.  Eager calls mark
+    their leaves' nodes, captured ones refuse marked nodes."""
+    for n, _ in node.next_functions:
+        if n is not None and not n.next_functions:
+            mark = n.metadata
+            if not torch.cuda.is_current_stream_capturing():
+                mark["stes_eager"] = True
+            elif "stes_eager" in mark:
+                raise StesError("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first")
 
 
 def ptr(t):
