@@ -1,10 +1,25 @@
 // Gated linear recurrence over sequences (stes_gated_scan_fwd / _bwd in include/stes.h).
 //
-// x_s = a_s x_{s-1} + z_s c_s with z = sigmoid(g), a = sigmoid(-g): an affine map of the state per step and channel, so runs of
-// steps compose, (A, B) after (A', B') = (A A', A B' + B), and channels are independent.
+// x_s = a_s x_{s-1} + z_s c_s with z = sigmoid(g), a = sigmoid(-g): an affine map of the state per step and channel.  Maps compose,
+// (A, B) after (A', B') = (A A', A B' + B), so the time axis is cut: a thread takes L steps of V channels, a workgroup a block of
+// STES_SCAN_BLOCK steps of a tile of channels, and the blocks of a sequence are joined while they run.  The backward pass is the
+// same recurrence the other way round, k_{s-1} = a_s (dh_s + k_s), on states recomputed from the one in front of the block: it reads
+// pre and dh and writes dpre, and stores no state but one per block.
+//
+// Joining the blocks of a sequence (T > STES_SCAN_BLOCK): workgroups draw tickets, all channels of a block of time before the
+// next block, and a workgroup waits for lower tickets only, whose workgroups have started before it and wait for lower ones
+// still: every wait ends.  Each block publishes its map (A, B) as soon as it has it and its final state when it knows the one in
+// front; a later block walks back over published maps to the nearest published state.  Both are single 64-bit words that are
+// valid when they are not zero (A >= 0 carries its sign bit set, a state a one beside it), so relaxed atomics of agent
+// scope carry them and no fence or cache write-back is needed.  Words are cleared by a kernel in front of every call.
 #include "stes_common.h"
 
 namespace {
+
+template <typename T, int V> struct Vec;
+template <> struct Vec<bf16, 8> { typedef bf16x8 type; };
+template <> struct Vec<float, 4> { typedef f32x4 type; };
+template <typename T> struct Vec<T, 1> { typedef T type __attribute__((ext_vector_type(1))); };
 
 // z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open)
 __device__ __forceinline__ void gate_pair(float x, float& z, float& a) {
@@ -20,72 +35,426 @@ __device__ __forceinline__ int seq_len(const stes_gated_scan_args& p, int b) {
     return n < 0 ? 0 : (n > p.T ? p.T : n);
 }
 
-// One thread per (sequence, channel), step by step.
-template <typename T>
-__global__ __launch_bounds__(64) void scan_fwd_serial_kernel(const stes_gated_scan_args p) {
-    const int c = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-    if (c >= p.H) return;
-    const int n = seq_len(p, b), nb = (p.T + STES_SCAN_BLOCK - 1) / STES_SCAN_BLOCK;
-    const T* pre = (const T*)p.pre + (long)b * p.bs_pre + c;
-    T* h = (T*)p.h + (long)b * p.bs_h + c;
-    float x = p.h0 ? p.h0[(long)b * p.bs_h0 + c] : 0.f;
-    for (int s = 0; s < p.T; ++s) {
-        if (p.states && s % STES_SCAN_BLOCK == 0) p.states[((long)b * nb + s / STES_SCAN_BLOCK) * p.H + c] = x;
-        if (s < n) {
-            const int t = p.reverse ? n - 1 - s : s;
-            float z, a;
-            gate_pair((float)pre[t * p.ld_pre], z, a);
-            x = a * x + z * (float)pre[t * p.ld_pre + p.H];
-            h[t * p.ld_h] = (T)x;
-        } else {
-            h[s * p.ld_h] = (T)0.f;
-        }
-    }
-    if (p.h_last) p.h_last[(long)b * p.bs_hl + c] = x;
+// What another lane of this wave wrote to LDS is read next (a wave's LDS accesses are executed in order; this keeps the compiler's).
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void scan_bwd_serial_kernel(const stes_gated_scan_args p) {
-    __shared__ float xs[STES_SCAN_BLOCK][64];
-    const int c = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-    if (c >= p.H) return;
-    const int n = seq_len(p, b), nb = (p.T + STES_SCAN_BLOCK - 1) / STES_SCAN_BLOCK;
-    const T* pre = (const T*)p.pre + (long)b * p.bs_pre + c;
-    const T* dh = p.dh ? (const T*)p.dh + (long)b * p.bs_dh + c : nullptr;
-    T* dpre = (T*)p.dpre + (long)b * p.bs_dpre + c;
-    float carry = p.dh_last ? p.dh_last[(long)b * p.bs_dhl + c] : 0.f;
-    for (int s = n; s < p.T; ++s) { dpre[s * p.ld_dpre] = (T)0.f; dpre[s * p.ld_dpre + p.H] = (T)0.f; }
-    for (int blk = nb - 1; blk >= 0; --blk) {
-        const int s0 = blk * STES_SCAN_BLOCK, s1 = min(n, s0 + STES_SCAN_BLOCK);
-        float x = p.states[((long)b * nb + blk) * p.H + c];
-        for (int s = s0; s < s1; ++s) {
-            const int t = p.reverse ? n - 1 - s : s;
-            float z, a;
-            gate_pair((float)pre[t * p.ld_pre], z, a);
-            xs[s - s0][threadIdx.x] = x;
-            x = a * x + z * (float)pre[t * p.ld_pre + p.H];
+// ---------------------------------------------------------------- joining blocks
+struct Link { uint64_t* map; uint64_t* state; };     // [block][chain * CT + channel]
+
+__device__ __forceinline__ void publish(uint64_t* w, uint64_t v) { __hip_atomic_store(w, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t peek(const uint64_t* w) { return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t map_word(float A, float B) { return ((uint64_t)__float_as_uint(B) << 32) | (__float_as_uint(A) | 0x80000000u); }
+__device__ __forceinline__ uint64_t state_word(float x) { return ((uint64_t)__float_as_uint(x) << 32) | 1u; }
+
+constexpr int LOOK = 8;                  // blocks looked at in one round trip to memory
+constexpr int MAX_ROUNDS = 1 << 22;      // (an exit for a broken workspace: the state becomes NaN)
+
+// The state in front of block `blk` of a channel (blk >= 1): `at` is the channel's word in block 0's row, `row` the words of a row.
+__device__ __forceinline__ float look_back(const Link& l, long at, long row, int blk) {
+    float A = 1.f, B = 0.f;
+    int t = blk - 1;
+    for (int round = 0; round < MAX_ROUNDS; ++round) {
+        uint64_t st[LOOK], mp[LOOK];
+#pragma unroll
+        for (int k = 0; k < LOOK; ++k) {
+            const int q = t - k < 0 ? 0 : t - k;
+            st[k] = peek(l.state + q * row + at);
+            mp[k] = peek(l.map + q * row + at);
         }
-        for (int s = s1 - 1; s >= s0; --s) {
-            const int t = p.reverse ? n - 1 - s : s;
-            float z, a;
-            gate_pair((float)pre[t * p.ld_pre], z, a);
-            const float l = carry + (dh ? (float)dh[t * p.ld_dh] : 0.f);
-            dpre[t * p.ld_dpre] = (T)(l * ((float)pre[t * p.ld_pre + p.H] - xs[s - s0][threadIdx.x]) * z * a);
-            dpre[t * p.ld_dpre + p.H] = (T)(l * z);
-            carry = a * l;
+        int used = 0;
+        bool found = false, open = true;
+        float x = 0.f;
+#pragma unroll
+        for (int k = 0; k < LOOK; ++k) {
+            if (open && t - k >= 0) {
+                if (st[k]) { x = __uint_as_float((uint32_t)(st[k] >> 32)); found = true; open = false; }
+                else if (mp[k]) {
+                    B = A * __uint_as_float((uint32_t)(mp[k] >> 32)) + B;
+                    A = A * __uint_as_float((uint32_t)mp[k] & 0x7fffffffu);
+                    ++used;
+                } else open = false;
+            }
+        }
+        if (found) return A * x + B;
+        t -= used;
+        if (t < 0) t = 0;                // (block 0 publishes a state: it is found there)
+        if (!used) __builtin_amdgcn_s_sleep(1);
+    }
+    return __builtin_nanf("");
+}
+
+__global__ __launch_bounds__(256) void scan_clear_kernel(u32x4* __restrict__ w, long n) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) w[i] = (u32x4){0u, 0u, 0u, 0u};
+}
+
+// ---------------------------------------------------------------- tiles
+// A workgroup of NT threads: LPR lanes side by side take LPR * V channels of a frame (256 bytes of bf16 or fp32 a row), NT / LPR
+// segments of L steps one after the other in time.
+template <typename T_, int V_, int LPR_, int L_>
+struct Tile {
+    typedef T_ T;
+    static constexpr int V = V_, LPR = LPR_, L = L_, CT = LPR * V, NS = STES_SCAN_BLOCK / L, NT = NS * LPR, NW = NT / 64, SW = 64 / LPR, CPL = CT / 64;
+};
+
+struct Place { int b, c0, n, blk; long chain; };
+
+template <class G, bool JOIN>
+__device__ __forceinline__ Place place(const stes_gated_scan_args& p, int tiles, long chains, unsigned* ticket, unsigned* shared_ticket) {
+    long id = blockIdx.x;
+    Place r;
+    r.blk = 0;
+    if (JOIN) {
+        if (threadIdx.x == 0) *shared_ticket = atomicAdd(ticket, 1u);
+        __syncthreads();
+        id = *shared_ticket;
+        r.blk = (int)(id / chains);
+    }
+    r.chain = id - r.blk * chains;
+    r.b = (int)(r.chain / tiles);
+    r.c0 = (int)(r.chain - (long)r.b * tiles) * G::CT;
+    r.n = seq_len(p, r.b);
+    return r;
+}
+
+template <class G, bool JOIN>
+__global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_args p, int tiles, long chains, int blocks, unsigned* ticket, Link link) {
+    typedef typename G::T T;
+    typedef typename Vec<T, G::V>::type VT;
+    constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
+    __shared__ float sA[G::NS][CT], sB[G::NS][CT];       // maps of the segments, then of what precedes them in their wave
+    __shared__ float tA[NW][CT], tB[NW][CT];             // maps of the waves; tB then: the state in front of each
+    __shared__ unsigned drawn;
+    const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
+    const int tid = threadIdx.x, cl = tid % G::LPR, seg = tid / G::LPR, lane = tid & 63, wave = tid >> 6;
+    const int c = at.c0 + cl * V, n = at.n, s0 = at.blk * STES_SCAN_BLOCK + seg * L;
+    const bool on = c < p.H;
+    const long H = p.H, step = p.reverse ? -p.ld_pre : p.ld_pre;
+    const T* row = (const T*)p.pre + at.b * p.bs_pre + c + (p.reverse ? (long)(n - 1 - s0) : (long)s0) * p.ld_pre;
+    VT g[L], cand[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+        if (on && s0 + j < n) {
+            g[j] = *reinterpret_cast<const VT*>(row + j * step);
+            cand[j] = *reinterpret_cast<const VT*>(row + j * step + H);
+        }
+    float a[L][V], u[L][V], A[V], B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        const bool live = on && s0 + j < n;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float z, k;
+            gate_pair((float)g[j][v], z, k);
+            a[j][v] = live ? k : 1.f;
+            u[j][v] = live ? z * (float)cand[j][v] : 0.f;
+            A[v] *= a[j][v];
+            B[v] = a[j][v] * B[v] + u[j][v];
         }
     }
-    if (p.dh0) p.dh0[(long)b * p.H + c] = carry;
+#pragma unroll
+    for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v]; sB[seg][cl * V + v] = B[v]; }
+    wave_lds_fence();
+#pragma unroll
+    for (int q = 0; q < G::CPL; ++q) {
+        const int ch = q * 64 + lane;
+        float fa = 1.f, fb = 0.f;
+#pragma unroll
+        for (int i = 0; i < SW; ++i) {
+            const float ia = sA[wave * SW + i][ch], ib = sB[wave * SW + i][ch];
+            sA[wave * SW + i][ch] = fa;
+            sB[wave * SW + i][ch] = fb;
+            fb = ia * fb + ib;
+            fa = ia * fa;
+        }
+        tA[wave][ch] = fa;
+        tB[wave][ch] = fb;
+    }
+    __syncthreads();
+    if (tid < CT) {
+        const int ch = at.c0 + tid;
+        const bool live = ch < p.H;
+        float x = 0.f, fa[NW], fb[NW], mA = 1.f, mB = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][tid]; fb[w] = tB[w][tid]; mB = fa[w] * mB + fb[w]; mA = fa[w] * mA; }
+        const long word = at.chain * CT + tid, words = chains * CT;
+        if (live) {
+            if (at.blk == 0) x = p.h0 ? p.h0[at.b * p.bs_h0 + ch] : 0.f;
+            else if (JOIN) {
+                if (at.blk + 1 < blocks) publish(link.map + at.blk * words + word, map_word(mA, mB));
+                x = look_back(link, word, words, at.blk);
+            }
+            const float end = mA * x + mB;
+            if (JOIN && at.blk + 1 < blocks) publish(link.state + at.blk * words + word, state_word(end));
+            if (p.states) p.states[((long)at.b * blocks + at.blk) * H + ch] = x;
+            if (at.blk + 1 == blocks && p.h_last) p.h_last[at.b * p.bs_hl + ch] = end;
+        }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { tB[w][tid] = x; x = fa[w] * x + fb[w]; }
+    }
+    __syncthreads();
+    if (!on) return;
+    float x[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = sA[seg][cl * V + v] * tB[wave][cl * V + v] + sB[seg][cl * V + v];
+    T* out = (T*)p.h + at.b * p.bs_h + c;
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        const int s = s0 + j;
+        VT o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            x[v] = a[j][v] * x[v] + u[j][v];
+            o[v] = (T)(s < n ? x[v] : 0.f);
+        }
+        if (s < p.T) *reinterpret_cast<VT*>(out + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h) = o;
+    }
+}
+
+// blocks are drawn from the end of the sequence: block `at.blk` of the joining order is block blocks - 1 - at.blk of time
+template <class G, bool JOIN>
+__global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_args p, int tiles, long chains, int blocks, unsigned* ticket, Link link) {
+    typedef typename G::T T;
+    typedef typename Vec<T, G::V>::type VT;
+    constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
+    __shared__ float sA[G::NS][CT], sB[G::NS][CT], sR[G::NS][CT], sS[G::NS][CT];
+    __shared__ float tA[NW][CT], tB[NW][CT], tR[NW][CT];
+    __shared__ unsigned drawn;
+    const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
+    const int blk = blocks - 1 - at.blk;
+    const int tid = threadIdx.x, cl = tid % G::LPR, seg = tid / G::LPR, lane = tid & 63, wave = tid >> 6;
+    const int c = at.c0 + cl * V, n = at.n, s0 = blk * STES_SCAN_BLOCK + seg * L;
+    const bool on = c < p.H;
+    const long H = p.H, t0 = p.reverse ? (long)(n - 1 - s0) : (long)s0, sign = p.reverse ? -1 : 1;
+    const T* row = (const T*)p.pre + at.b * p.bs_pre + c + t0 * p.ld_pre;
+    const T* drow = p.dh ? (const T*)p.dh + at.b * p.bs_dh + c + t0 * p.ld_dh : nullptr;
+    VT g[L], cand[L], d[L];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        const bool live = on && s0 + j < n;
+#pragma unroll
+        for (int v = 0; v < V; ++v) d[j][v] = (T)0.f;
+        if (live) {
+            g[j] = *reinterpret_cast<const VT*>(row + sign * j * p.ld_pre);
+            cand[j] = *reinterpret_cast<const VT*>(row + sign * j * p.ld_pre + H);
+            if (drow) d[j] = *reinterpret_cast<const VT*>(drow + sign * j * p.ld_dh);
+        }
+    }
+    // the segment's maps, forwards (A, B) and backwards (A, R)
+    float A[V], B[V], R[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; R[v] = 0.f; }
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        const bool live = on && s0 + j < n;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float z, k;
+            gate_pair((float)g[j][v], z, k);
+            k = live ? k : 1.f;
+            const float u = live ? z * (float)cand[j][v] : 0.f;
+            B[v] = k * B[v] + u;
+            A[v] *= k;
+            R[v] += A[v] * (float)d[j][v];               // d_j reaches the segment's front through a_0 .. a_j
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v]; sB[seg][cl * V + v] = B[v]; sR[seg][cl * V + v] = R[v]; }
+    wave_lds_fence();
+#pragma unroll
+    for (int q = 0; q < G::CPL; ++q) {
+        const int ch = q * 64 + lane;
+        float ia[SW], ib[SW], ir[SW], fa = 1.f, fb = 0.f, ra = 1.f, rr = 0.f;
+#pragma unroll
+        for (int i = 0; i < SW; ++i) { ia[i] = sA[wave * SW + i][ch]; ib[i] = sB[wave * SW + i][ch]; ir[i] = sR[wave * SW + i][ch]; }
+#pragma unroll
+        for (int i = 0; i < SW; ++i) {
+            sA[wave * SW + i][ch] = fa;
+            sB[wave * SW + i][ch] = fb;
+            fb = ia[i] * fb + ib[i];
+            fa = ia[i] * fa;
+        }
+#pragma unroll
+        for (int i = SW - 1; i >= 0; --i) {
+            sS[wave * SW + i][ch] = ra;
+            sR[wave * SW + i][ch] = rr;
+            rr = ia[i] * rr + ir[i];
+            ra = ia[i] * ra;
+        }
+        tA[wave][ch] = fa;
+        tB[wave][ch] = fb;
+        tR[wave][ch] = rr;
+    }
+    __syncthreads();
+    if (tid < CT) {
+        const int ch = at.c0 + tid;
+        float fa[NW], fb[NW], fr[NW], mA = 1.f, mR = 0.f, x = 0.f, k = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][tid]; fb[w] = tB[w][tid]; fr[w] = tR[w][tid]; }
+#pragma unroll
+        for (int w = NW - 1; w >= 0; --w) { mR = fa[w] * mR + fr[w]; mA = fa[w] * mA; }
+        const long word = at.chain * CT + tid, words = chains * CT;
+        if (ch < p.H) {
+            x = p.states[((long)at.b * blocks + blk) * H + ch];
+            if (at.blk == 0) k = p.dh_last ? p.dh_last[at.b * p.bs_dhl + ch] : 0.f;
+            else if (JOIN) {
+                if (blk) publish(link.map + at.blk * words + word, map_word(mA, mR));
+                k = look_back(link, word, words, at.blk);
+            }
+            const float front = mA * k + mR;
+            if (JOIN && blk) publish(link.state + at.blk * words + word, state_word(front));
+            if (!blk && p.dh0) p.dh0[at.b * H + ch] = front;
+        }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { tB[w][tid] = x; x = fa[w] * x + fb[w]; }
+#pragma unroll
+        for (int w = NW - 1; w >= 0; --w) { tR[w][tid] = k; k = fa[w] * k + fr[w]; }
+    }
+    __syncthreads();
+    if (!on) return;
+    float x[L][V], k[V];                                     // the state in front of each step; what comes from the steps behind
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int q = cl * V + v;
+        x[0][v] = sA[seg][q] * tB[wave][q] + sB[seg][q];
+        k[v] = sS[seg][q] * tR[wave][q] + sR[seg][q];
+    }
+#pragma unroll
+    for (int j = 0; j + 1 < L; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float z, w;
+            gate_pair((float)g[j][v], z, w);
+            x[j + 1][v] = s0 + j < n ? w * x[j][v] + z * (float)cand[j][v] : 0.f;
+        }
+    T* out = (T*)p.dpre + at.b * p.bs_dpre + c;
+#pragma unroll
+    for (int j = L - 1; j >= 0; --j) {
+        const int s = s0 + j;
+        if (s >= p.T) continue;
+        VT og, oc;
+        if (s < n) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float z, w;
+                gate_pair((float)g[j][v], z, w);
+                const float lam = (float)d[j][v] + k[v];
+                oc[v] = (T)(lam * z);
+                og[v] = (T)(lam * ((float)cand[j][v] - x[j][v]) * z * w);
+                k[v] = w * lam;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) og[v] = oc[v] = (T)0.f;
+        }
+        T* o = out + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_dpre;
+        *reinterpret_cast<VT*>(o) = og;
+        *reinterpret_cast<VT*>(o + H) = oc;
+    }
+}
+
+// ---------------------------------------------------------------- few steps
+// T <= SHORT: a thread walks all steps of V channels; nothing is shared (frames of streams, one at a time).
+constexpr int SHORT = 8;
+
+template <typename T, int V, bool BWD>
+__global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_args p, long groups) {
+    typedef typename Vec<T, V>::type VT;
+    const long id = (long)blockIdx.x * 64 + threadIdx.x, per = (p.H + V - 1) / V;
+    if (id >= groups) return;
+    const int b = (int)(id / per), c = (int)(id - b * per) * V, n = seq_len(p, b);
+    const long H = p.H;
+    const T* pre = (const T*)p.pre + b * p.bs_pre + c;
+    const T* dh = BWD && p.dh ? (const T*)p.dh + b * p.bs_dh + c : nullptr;
+    VT g[SHORT], cand[SHORT], d[BWD ? SHORT : 1];
+#pragma unroll
+    for (int s = 0; s < SHORT; ++s)
+        if (s < n) {
+            const long t = p.reverse ? n - 1 - s : s;
+            g[s] = *reinterpret_cast<const VT*>(pre + t * p.ld_pre);
+            cand[s] = *reinterpret_cast<const VT*>(pre + t * p.ld_pre + H);
+            if (BWD && dh) d[s] = *reinterpret_cast<const VT*>(dh + t * p.ld_dh);
+        }
+    float x[V], before[BWD ? SHORT : 1][V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (BWD) x[v] = p.T ? p.states[b * H + c + v] : 0.f;
+        else {
+            x[v] = p.h0 ? p.h0[b * p.bs_h0 + c + v] : 0.f;
+            if (p.states && p.T) p.states[b * H + c + v] = x[v];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < SHORT; ++s) {
+        if (s >= p.T) break;
+        VT o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (BWD) before[s][v] = x[v];
+            if (s < n) {
+                float z, a;
+                gate_pair((float)g[s][v], z, a);
+                x[v] = a * x[v] + z * (float)cand[s][v];
+            }
+            o[v] = (T)(s < n ? x[v] : 0.f);
+        }
+        if (!BWD) *reinterpret_cast<VT*>((T*)p.h + b * p.bs_h + c + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h) = o;
+    }
+    if (!BWD) {
+        if (p.h_last)
+#pragma unroll
+            for (int v = 0; v < V; ++v) p.h_last[b * p.bs_hl + c + v] = x[v];
+        return;
+    }
+    float k[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) k[v] = p.dh_last ? p.dh_last[b * p.bs_dhl + c + v] : 0.f;
+#pragma unroll
+    for (int s = SHORT - 1; s >= 0; --s) {
+        if (s >= p.T) continue;
+        VT og, oc;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            og[v] = oc[v] = (T)0.f;
+            if (s < n) {
+                float z, a;
+                gate_pair((float)g[s][v], z, a);
+                const float lam = (dh ? (float)d[BWD ? s : 0][v] : 0.f) + k[v];
+                oc[v] = (T)(lam * z);
+                og[v] = (T)(lam * ((float)cand[s][v] - before[BWD ? s : 0][v]) * z * a);
+                k[v] = a * lam;
+            }
+        }
+        T* o = (T*)p.dpre + b * p.bs_dpre + c + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_dpre;
+        *reinterpret_cast<VT*>(o) = og;
+        *reinterpret_cast<VT*>(o + H) = oc;
+    }
+    if (p.dh0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.dh0[b * H + c + v] = k[v];
 }
 
 // The gradient of an initial state that the batch shares: the rows added up in order.
-__global__ __launch_bounds__(256) void scan_dh0_sum_kernel(const float* __restrict__ dh0, float* __restrict__ out, int B, int H) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(64) void scan_dh0_sum_kernel(const float* __restrict__ dh0, float* __restrict__ out, int B, int H) {
+    const int c = blockIdx.x * 64 + threadIdx.x;
     if (c >= H) return;
     float s = 0.f;
+#pragma unroll 8
     for (int b = 0; b < B; ++b) s += dh0[(long)b * H + c];
     out[c] = s;
 }
+
+// ---------------------------------------------------------------- host
+constexpr int MIN_CT = 64;                   // the narrowest tile: workspaces are sized for its number of tiles, rounded up
+
+int blocks_of(int T) { return (T + STES_SCAN_BLOCK - 1) / STES_SCAN_BLOCK; }
+// words of one kind in the workspace: tiles of 64 or 128 channels alike fit into rows of H rounded up to 128
+long words_of(int B, int T, int H) { return (long)blocks_of(T) * B * ((H + 127) / 128 * 128); }
 
 // rows of `width` elements that a call writes: frames within sequences or the reverse, apart from one another
 bool apart(int64_t ld, int T, int64_t bs, int B, int64_t width) {
@@ -98,9 +467,10 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
     STES_CHECK(a, STES_ERR_ARG, "stes_gated_scan: null pointer");
     STES_CHECK(a->B >= 0 && a->T >= 0 && a->H >= 0, STES_ERR_ARG, "stes_gated_scan: negative size");
     STES_CHECK(a->f32 == 0 || a->f32 == 1, STES_ERR_ARG, "stes_gated_scan: f32 is 0 (bf16) or 1 (fp32)");
+    STES_CHECK(!a->dh0_sum || a->dh0 || !a->B, STES_ERR_ARG, "stes_gated_scan_bwd: dh0_sum needs dh0");
     if (!a->B || !a->H) return STES_OK;
-    STES_CHECK(a->B <= 65535, STES_ERR_UNSUPPORTED, "stes_gated_scan: more than 65535 sequences");
-    STES_CHECK(a->H <= (1 << 24) && (long)a->B * ((a->H + 63) / 64) < (1L << 30), STES_ERR_UNSUPPORTED, "stes_gated_scan: too many channels");
+    STES_CHECK(a->H <= (1 << 24) && (long)a->B * ((a->H + MIN_CT - 1) / MIN_CT) * (blocks_of(a->T) + 1) < (1L << 31), STES_ERR_UNSUPPORTED,
+               "stes_gated_scan: more tiles than a launch holds");
     if (a->T) {
         STES_CHECK(a->pre && a->ld_pre >= 2L * a->H && a->bs_pre >= 0, STES_ERR_ARG, "stes_gated_scan: pre is [B][T][2H]");
         if (!bwd) STES_CHECK(a->h && apart(a->ld_h, a->T, a->bs_h, a->B, a->H), STES_ERR_ARG, "stes_gated_scan_fwd: h is [B][T][H], rows apart");
@@ -110,29 +480,69 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
             STES_CHECK(!a->dh || (a->ld_dh >= a->H && a->bs_dh >= 0), STES_ERR_ARG, "stes_gated_scan_bwd: dh is [B][T][H]");
         }
         const int64_t need = stes_gated_scan_ws_bytes(a->B, a->T, a->H);
-        STES_CHECK(need == 0 || (a->ws && a->ws_bytes >= need), STES_ERR_ARG, "stes_gated_scan: workspace too small");
+        STES_CHECK(need == 0 || (a->ws && a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0), STES_ERR_ARG, "stes_gated_scan: workspace too small or not aligned to 16 bytes");
     }
     STES_CHECK(!a->h0 || a->bs_h0 == 0 || a->bs_h0 >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h0 overlap");
     STES_CHECK(!a->h_last || a->bs_hl >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h_last overlap");
     STES_CHECK(!(a->h_last && a->h_last == a->h0) || a->bs_h0 == a->bs_hl, STES_ERR_ARG, "stes_gated_scan: a state in place keeps its row stride");
-    STES_CHECK(!a->dh0_sum || a->dh0 || !a->B, STES_ERR_ARG, "stes_gated_scan_bwd: dh0_sum needs dh0");
+    STES_CHECK(!bwd || !a->dh_last || a->bs_dhl == 0 || a->bs_dhl >= a->H, STES_ERR_ARG, "stes_gated_scan_bwd: rows of dh_last overlap");
     return STES_OK;
+}
+
+// rows that a lane reads or writes 16 bytes of at a time
+bool wide_rows(const void* p, int64_t ld, int64_t bs, int bytes) { return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && bs * bytes % 16 == 0; }
+
+template <class G, bool BWD>
+void launch_tiles(const stes_gated_scan_args& a, hipStream_t s) {
+    const int tiles = (a.H + G::CT - 1) / G::CT, blocks = blocks_of(a.T);
+    const long chains = (long)a.B * tiles;
+    unsigned* ticket = (unsigned*)a.ws;
+    uint64_t* words = (uint64_t*)((char*)a.ws + 256);
+    const Link link{words, words + words_of(a.B, a.T, a.H)};
+    if (blocks > 1) {
+        const long n = stes_gated_scan_ws_bytes(a.B, a.T, a.H) / 16;
+        hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (u32x4*)a.ws, n);
+        if (BWD) hipLaunchKernelGGL((scan_bwd_kernel<G, true>), dim3((unsigned)(chains * blocks)), dim3(G::NT), 0, s, a, tiles, chains, blocks, ticket, link);
+        else hipLaunchKernelGGL((scan_fwd_kernel<G, true>), dim3((unsigned)(chains * blocks)), dim3(G::NT), 0, s, a, tiles, chains, blocks, ticket, link);
+    } else {
+        if (BWD) hipLaunchKernelGGL((scan_bwd_kernel<G, false>), dim3((unsigned)chains), dim3(G::NT), 0, s, a, tiles, chains, 1, ticket, link);
+        else hipLaunchKernelGGL((scan_fwd_kernel<G, false>), dim3((unsigned)chains), dim3(G::NT), 0, s, a, tiles, chains, 1, ticket, link);
+    }
+}
+
+template <typename T, int V, bool BWD>
+void launch_short(const stes_gated_scan_args& a, hipStream_t s) {
+    const long groups = (long)a.B * ((a.H + V - 1) / V);
+    hipLaunchKernelGGL((scan_short_kernel<T, V, BWD>), dim3((unsigned)((groups + 63) / 64)), dim3(64), 0, s, a, groups);
+}
+
+template <bool BWD>
+void scan_launch(const stes_gated_scan_args& a, hipStream_t s) {
+    const int bytes = a.f32 ? 4 : 2;
+    bool wide = a.H * bytes % 16 == 0 && (!a.T || wide_rows(a.pre, a.ld_pre, a.bs_pre, bytes));
+    if (BWD) wide = wide && wide_rows(a.dpre, a.ld_dpre, a.bs_dpre, bytes) && (!a.dh || wide_rows(a.dh, a.ld_dh, a.bs_dh, bytes));
+    else wide = wide && wide_rows(a.h, a.ld_h, a.bs_h, bytes);
+    if (a.T <= SHORT) {
+        if (a.f32) { if (wide) launch_short<float, 4, BWD>(a, s); else launch_short<float, 1, BWD>(a, s); }
+        else { if (wide) launch_short<bf16, 8, BWD>(a, s); else launch_short<bf16, 1, BWD>(a, s); }
+        return;
+    }
+    if (a.f32) { if (wide) launch_tiles<Tile<float, 4, 16, 8>, BWD>(a, s); else launch_tiles<Tile<float, 1, 64, 32>, BWD>(a, s); }
+    else { if (wide) launch_tiles<Tile<bf16, 8, 16, 8>, BWD>(a, s); else launch_tiles<Tile<bf16, 1, 64, 32>, BWD>(a, s); }
 }
 
 }  // namespace
 
 extern "C" int64_t stes_gated_scan_ws_bytes(int B, int T, int H) {
-    (void)B; (void)T; (void)H;
-    return 0;
+    if (B <= 0 || H <= 0 || T <= STES_SCAN_BLOCK) return 0;
+    return 256 + 16 * words_of(B, T, H);
 }
 
 extern "C" int stes_gated_scan_fwd(const stes_gated_scan_args* a, void* stream) {
     const int rc = scan_check(a, false);
     if (rc) return rc;
     if (!a->B || !a->H) return STES_OK;
-    const dim3 grid((a->H + 63) / 64, a->B);
-    if (a->f32) hipLaunchKernelGGL(scan_fwd_serial_kernel<float>, grid, dim3(64), 0, (hipStream_t)stream, *a);
-    else hipLaunchKernelGGL(scan_fwd_serial_kernel<bf16>, grid, dim3(64), 0, (hipStream_t)stream, *a);
+    scan_launch<false>(*a, (hipStream_t)stream);
     STES_LAUNCH_CHECK();
     return STES_OK;
 }
@@ -142,13 +552,11 @@ extern "C" int stes_gated_scan_bwd(const stes_gated_scan_args* a, void* stream) 
     if (rc) return rc;
     if (!a->H) return STES_OK;
     if (a->B) {
-        const dim3 grid((a->H + 63) / 64, a->B);
-        if (a->f32) hipLaunchKernelGGL(scan_bwd_serial_kernel<float>, grid, dim3(64), 0, (hipStream_t)stream, *a);
-        else hipLaunchKernelGGL(scan_bwd_serial_kernel<bf16>, grid, dim3(64), 0, (hipStream_t)stream, *a);
+        scan_launch<true>(*a, (hipStream_t)stream);
         STES_LAUNCH_CHECK();
     }
     if (a->dh0_sum) {                                       // (zeros for an empty batch)
-        hipLaunchKernelGGL(scan_dh0_sum_kernel, dim3((a->H + 255) / 256), dim3(256), 0, (hipStream_t)stream, a->dh0, a->dh0_sum, a->B, a->H);
+        hipLaunchKernelGGL(scan_dh0_sum_kernel, dim3((a->H + 63) / 64), dim3(64), 0, (hipStream_t)stream, a->dh0, a->dh0_sum, a->B, a->H);
         STES_LAUNCH_CHECK();
     }
     return STES_OK;
