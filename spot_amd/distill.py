@@ -9,6 +9,8 @@ student's class distribution from the teacher's distribution over its k best cla
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 
 import torch
 
@@ -17,15 +19,15 @@ from . import lib
 _ELEMENT = {torch.bfloat16: 0, torch.float32: 1}
 
 
-def _need(ok, text):
-    if not ok:
-        raise lib.StesError("topk_distill: " + text)
+def _refuse(text):
+    raise lib.StesError("topk_distill: " + text)
 
 
 def _flat(t, n):
     """[..., n] -> [M, n] without a copy where the strides allow one row stride, else a contiguous copy."""
-    t = t.reshape(-1, n) if t.dim() != 2 else t
-    if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n):
+    if t.dim() != 2:
+        t = t.reshape(-1, n)
+    if not t.is_contiguous() and ((n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n)):
         t = t.contiguous()
     return t
 
@@ -34,26 +36,23 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _args(logits, idx, val, weight, temperature, denom):
-    """-> (argument block, the tensors it points at); logits is [M, V], rows contiguous."""
+@functools.lru_cache(maxsize=256)
+def _ws_floats(M, V):
+    return lib.lib().stes_distill_ws_floats(M, V)
+
+
+def _call(entry, logits, idx, val, weight, temperature, denom, grad_scale=1.0, upstream=None, loss=None, stats=None, d=None, accumulate=False):
+    """One call of the library; every tensor [M, ...] with contiguous rows."""
     M, V = logits.shape
-    a = lib.DistillArgs()
-    k = idx.shape[1]
-    a.M, a.V, a.k = M, V, k
-    a.logits, a.ld, a.f32 = logits.data_ptr(), _ld(logits), _ELEMENT[logits.dtype]
-    a.idx, a.ld_idx, a.idx_i64 = idx.data_ptr(), _ld(idx), int(idx.dtype == torch.int64)
-    a.val, a.ld_val, a.val_f32 = val.data_ptr(), _ld(val), _ELEMENT[val.dtype]
-    if weight is not None:
-        a.weight = weight.data_ptr()
-    a.temperature, a.denom, a.grad_scale = temperature, denom, 1.0
-    return a
-
-
-def _workspace(a, dev):
-    n = lib.lib().stes_distill_ws_floats(a.M, a.V)
-    ws = torch.empty(n, dtype=torch.float32, device=dev)
-    a.ws, a.ws_floats = ws.data_ptr(), n
-    return ws
+    ws = None if loss is None else torch.empty(_ws_floats(M, V), dtype=torch.float32, device=logits.device)   # (of this call's own)
+    a = lib.DistillArgs(
+        logits.data_ptr(), _ld(logits), _ELEMENT[logits.dtype], idx.data_ptr(), _ld(idx), idx.dtype == torch.int64,
+        val.data_ptr(), _ld(val), _ELEMENT[val.dtype], None if weight is None else weight.data_ptr(), M, V, idx.shape[1],
+        temperature, denom, grad_scale, None if upstream is None else upstream.data_ptr(),
+        None if loss is None else loss.data_ptr(), None if stats is None else stats.data_ptr(),
+        None if d is None else d.data_ptr(), 0 if d is None else _ld(d), 0 if d is None else _ELEMENT[d.dtype], accumulate,
+        None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    lib.call(entry, C.byref(a))
 
 
 class _Distill(torch.autograd.Function):
@@ -62,10 +61,7 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, logits, idx, val, weight, temperature, denom):
         loss = torch.empty((), dtype=torch.float32, device=logits.device)
         stats = torch.empty(logits.shape[0], 2, dtype=torch.float32, device=logits.device)
-        a = _args(logits, idx, val, weight, temperature, denom)
-        _ws = _workspace(a, logits.device)
-        a.loss, a.stats = loss.data_ptr(), stats.data_ptr()
-        lib.call("stes_distill", C.byref(a))
+        _call("stes_distill", logits, idx, val, weight, temperature, denom, loss=loss, stats=stats)
         ctx.save_for_backward(logits, idx, val, weight, stats)
         ctx.scale = (temperature, denom)
         return loss
@@ -76,35 +72,37 @@ class _Distill(torch.autograd.Function):
         logits, idx, val, weight, stats = ctx.saved_tensors
         d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if logits.shape[0]:
-            with torch.cuda.device(logits.device):
-                up = up.to(torch.float32)
-                a = _args(logits, idx, val, weight, *ctx.scale)
-                a.stats, a.upstream = stats.data_ptr(), up.data_ptr()
-                a.dlogits, a.ld_d, a.d_f32 = d.data_ptr(), _ld(d), _ELEMENT[d.dtype]
-                lib.call("stes_distill_bwd", C.byref(a))
+            with lib.on_device(logits.device):
+                _call("stes_distill_bwd", logits, idx, val, weight, *ctx.scale, upstream=up, stats=stats, d=d)
         return d, None, None, None, None, None
 
 
 def _check(logits, idx, val, weight, temperature, denom):
-    _need(isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _ELEMENT and logits.dim() >= 1,
-          "logits must be a bfloat16 or float32 tensor [..., classes] on the GPU")
-    dev, V, lead = logits.device, logits.shape[-1], tuple(logits.shape[:-1])
-    _need(V >= 1, "no classes")
-    _need(idx.device == dev and idx.dtype in (torch.int64, torch.int32) and idx.dim() == logits.dim() and tuple(idx.shape[:-1]) == lead,
-          f"idx must be int64 or int32 {list(lead)} + [k] on {dev}, got {idx.dtype} {list(idx.shape)} on {idx.device}")
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in _ELEMENT or logits.dim() < 1:
+        _refuse("logits must be a bfloat16 or float32 tensor [..., classes] on the GPU")
+    dev, V, lead = logits.device, logits.shape[-1], logits.shape[:-1]
+    if V < 1:
+        _refuse("no classes")
+    if idx.device != dev or idx.dtype not in (torch.int64, torch.int32) or idx.dim() != logits.dim() or idx.shape[:-1] != lead:
+        _refuse(f"idx must be int64 or int32 {list(lead)} + [k] on {dev}, got {idx.dtype} {list(idx.shape)} on {idx.device}")
     k = idx.shape[-1]
-    _need(1 <= k <= lib.DISTILL_MAX_K, f"1 to {lib.DISTILL_MAX_K} teacher classes a row, got {k}")
-    _need(val.device == dev and val.dtype in _ELEMENT and val.shape == idx.shape, f"val must be float32 or bfloat16 {list(idx.shape)} on {dev}")
-    _need(not (torch.is_grad_enabled() and val.requires_grad), "the teacher's logits are constants: detach val")
-    if weight is not None:
-        _need(weight.device == dev and weight.dtype == torch.float32 and tuple(weight.shape) == lead, f"weight must be float32 {list(lead)} on {dev}")
-        _need(not (torch.is_grad_enabled() and weight.requires_grad), "weights are constants: detach weight")
-        weight = weight.reshape(-1).contiguous()
+    if not 1 <= k <= lib.DISTILL_MAX_K:
+        _refuse(f"1 to {lib.DISTILL_MAX_K} teacher classes a row, got {k}")
+    if val.device != dev or val.dtype not in _ELEMENT or val.shape != idx.shape:
+        _refuse(f"val must be float32 or bfloat16 {list(idx.shape)} on {dev}")
+    if weight is not None and (weight.device != dev or weight.dtype != torch.float32 or weight.shape != lead):
+        _refuse(f"weight must be float32 {list(lead)} on {dev}")
+    if torch.is_grad_enabled() and (val.requires_grad or (weight is not None and weight.requires_grad)):
+        _refuse("the teacher's logits and the weights are constants: detach them")
     temperature = float(temperature)
-    _need(0.0 < temperature < float("inf"), f"the temperature is positive, got {temperature}")
+    if not 0.0 < temperature < math.inf:
+        _refuse(f"the temperature is positive, got {temperature}")
     s = _flat(logits, V)
     denom = float(max(1, s.shape[0]) if denom is None else denom)
-    _need(0.0 < denom < float("inf"), f"the denominator is positive, got {denom}")
+    if not 0.0 < denom < math.inf:
+        _refuse(f"the denominator is positive, got {denom}")
+    if weight is not None:
+        weight = weight.reshape(-1).contiguous()
     return s, _flat(idx, k), _flat(val, k), weight, temperature, denom
 
 
@@ -119,16 +117,13 @@ def topk_distill_loss(logits, idx, val, temperature=1.0, weight=None, denom=None
     denom   a number; None: the number of rows
     -> a float32 scalar.  A class listed twice has the sum of its probabilities; an index beyond V makes the result NaN."""
     s, idx, val, weight, temperature, denom = _check(logits, idx, val, weight, temperature, denom)
-    with torch.cuda.device(s.device):
-        if torch.is_grad_enabled() and s.requires_grad:
+    with lib.on_device(s.device):
+        if s.requires_grad and torch.is_grad_enabled():
             loss = _Distill.apply(s, idx, val, weight, temperature, denom)
             lib.guard_leaves(loss.grad_fn)
             return loss
         loss = torch.empty((), dtype=torch.float32, device=s.device)
-        a = _args(s, idx, val, weight, temperature, denom)
-        _ws = _workspace(a, s.device)
-        a.loss = loss.data_ptr()
-        lib.call("stes_distill", C.byref(a))
+        _call("stes_distill", s, idx, val, weight, temperature, denom, loss=loss)
     return loss
 
 
@@ -138,19 +133,17 @@ def topk_distill_grad(logits, idx, val, temperature=1.0, weight=None, denom=None
     out         where the gradient goes: bfloat16 or float32 [..., V] (any row stride), None: a new tensor of the logits' type
     accumulate  add to `out` instead of writing it
     -> (loss, gradient)"""
-    s, idx, val, weight, temperature, denom = _check(logits.detach(), idx, val, weight, temperature, denom)
-    _need(not accumulate or out is not None, "accumulate adds to out")
+    s, idx, val, weight, temperature, denom = _check(logits, idx, val, weight, temperature, denom)
     if out is None:
+        if accumulate:
+            _refuse("accumulate adds to out")
         out = torch.empty(logits.shape, dtype=logits.dtype, device=s.device)
-    else:
-        _need(out.device == s.device and out.dtype in _ELEMENT and out.shape == logits.shape, f"out must be float32 or bfloat16 {list(logits.shape)} on {s.device}")
+    elif out.device != s.device or out.dtype not in _ELEMENT or out.shape != logits.shape:
+        _refuse(f"out must be float32 or bfloat16 {list(logits.shape)} on {s.device}")
     d = out if out.dim() == 2 else out.view(-1, out.shape[-1])
-    _need((d.shape[1] <= 1 or d.stride(1) == 1) and (d.shape[0] <= 1 or d.stride(0) >= d.shape[1]), "rows of out must be contiguous and not overlap")
-    with torch.cuda.device(s.device):
+    if not d.is_contiguous() and ((d.shape[1] > 1 and d.stride(1) != 1) or (d.shape[0] > 1 and d.stride(0) < d.shape[1])):
+        _refuse("rows of out must be contiguous and not overlap")
+    with lib.on_device(s.device):
         loss = torch.empty((), dtype=torch.float32, device=s.device)
-        a = _args(s, idx, val, weight, temperature, denom)
-        _ws = _workspace(a, s.device)
-        a.grad_scale, a.loss = float(grad_scale), loss.data_ptr()
-        a.dlogits, a.ld_d, a.d_f32, a.accumulate = d.data_ptr(), _ld(d), _ELEMENT[d.dtype], int(accumulate)
-        lib.call("stes_distill", C.byref(a))
+        _call("stes_distill", s, idx, val, weight, temperature, denom, float(grad_scale), loss=loss, d=d, accumulate=bool(accumulate))
     return loss, out

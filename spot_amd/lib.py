@@ -5,6 +5,7 @@ raises, it never falls back to another implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -251,7 +252,16 @@ def check(rc: int, what: str):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device, as the hipStream_t the library takes."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())       # (torch.cuda.current_stream() builds an object first: 2.6 us more)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """Makes `dev` the current device for a call on its tensors (nothing where it is: the usual case)."""
+    return _HERE_ALREADY if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def guard_leaves(node):

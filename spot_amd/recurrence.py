@@ -8,6 +8,7 @@ videos, frame streams and ragged batches, differentiable (stes_gated_scan_fwd / 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -16,25 +17,34 @@ from . import lib
 _ELEMENT = {torch.bfloat16: 0, torch.float32: 1}
 
 
-def _need(ok, text):
-    if not ok:
-        raise lib.StesError("gated_scan: " + text)
+def _refuse(text):
+    raise lib.StesError("gated_scan: " + text)
 
 
-def _rows(t, B, H, name):
-    """Stride between the rows of a [B, H] fp32 tensor whose rows are contiguous."""
-    _need(t.dtype == torch.float32 and tuple(t.shape) == (B, H), f"{name} must be float32 [{B}, {H}], got {t.dtype} {list(t.shape)}")
-    _need(H <= 1 or t.stride(1) == 1, f"rows of {name} must be contiguous")
-    _need(B <= 1 or t.stride(0) >= H, f"rows of {name} must not overlap")
+@functools.lru_cache(maxsize=256)
+def _ws_bytes(B, T, H):
+    return lib.lib().stes_gated_scan_ws_bytes(B, T, H)
+
+
+def _workspace(B, T, H, dev):
+    """A workspace of this call's own (None where none is needed): calls on two streams and two graphs never share one."""
+    n = _ws_bytes(B, T, H)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _row_stride(t, B, H, name):
+    """Stride between the rows of a float32 [B, H] tensor whose rows are contiguous and apart."""
+    if t.dtype != torch.float32 or t.shape != (B, H):
+        _refuse(f"{name} must be float32 [{B}, {H}], got {t.dtype} {list(t.shape)}")
+    if (H > 1 and t.stride(1) != 1) or (B > 1 and t.stride(0) < H):
+        _refuse(f"rows of {name} must be contiguous and not overlap")
     return t.stride(0) if B > 1 else max(H, 1)
 
 
-def _frames(t, width, name):
-    """(frame stride, sequence stride) of a [B, T, width] tensor whose last dimension is contiguous."""
-    B, T = t.shape[0], t.shape[1]
-    _need(width <= 1 or t.stride(2) == 1, f"the last dimension of {name} must be contiguous")
-    ld = t.stride(1) if T > 1 else width
-    return ld, t.stride(0) if B > 1 else 0
+def _strides(t, T, width):
+    """(frame stride, sequence stride) of a [B, T, width] tensor; the frame stride of a single frame is immaterial."""
+    bs, ld, _ = t.stride()
+    return (ld if T > 1 else width), bs
 
 
 def _apart(t, width):
@@ -45,47 +55,27 @@ def _apart(t, width):
     return outer[1] == 1 or outer[0] >= inner[0] * (inner[1] - 1) + width
 
 
-def _tidy(t, width):
-    """`t` itself where the kernels take its strides, else a contiguous copy (an expanded or transposed gradient)."""
-    if (width <= 1 or t.stride(2) == 1) and (t.shape[1] <= 1 or t.stride(1) >= width) and (t.shape[0] <= 1 or t.stride(0) >= 0):
-        return t
-    return t.contiguous()
-
-
-def _args(pre, h0, lengths, reverse):
-    B, T, W = pre.shape
-    H = W // 2
-    a = lib.GatedScanArgs()
-    a.B, a.T, a.H, a.f32, a.reverse = B, T, H, _ELEMENT[pre.dtype], int(reverse)
-    a.pre = pre.data_ptr()
-    a.ld_pre, a.bs_pre = _frames(pre, W, "pre")
-    if h0 is not None:
-        a.h0 = h0.data_ptr()
-        a.bs_h0 = 0 if h0.dim() == 1 else _rows(h0, B, H, "h0")
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    need = lib.lib().stes_gated_scan_ws_bytes(B, T, H)
-    ws = None
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=pre.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), need
-    return a, ws
-
-
 def _forward(pre, h0, lengths, reverse, out, state_out, keep_states):
     B, T, W = pre.shape
-    H = W // 2
-    h = torch.empty(B, T, H, dtype=pre.dtype, device=pre.device) if out is None else out
-    last = torch.empty(B, H, dtype=torch.float32, device=pre.device) if state_out is None else state_out
-    states = None
-    if keep_states:
-        states = torch.empty(B, -(-T // lib.SCAN_BLOCK), H, dtype=torch.float32, device=pre.device)
+    H, dev = W // 2, pre.device
+    h = pre.new_empty(B, T, H) if out is None else out
+    if state_out is None:
+        last, bs_hl = torch.empty(B, H, dtype=torch.float32, device=dev), max(H, 1)
+    else:
+        last, bs_hl = state_out, _row_stride(state_out, B, H, "state_out")
+    states = torch.empty(B, -(-T // lib.SCAN_BLOCK), H, dtype=torch.float32, device=dev) if keep_states else None
     if B and H:
-        a, _ws = _args(pre, h0, lengths, reverse)
-        a.h = h.data_ptr()
-        a.ld_h, a.bs_h = _frames(h, H, "out")
-        a.h_last, a.bs_hl = last.data_ptr(), _rows(last, B, H, "state_out")
-        a.states = lib.ptr(states)
+        ws = _workspace(B, T, H, dev)
+        ld, bs = _strides(pre, T, W)
+        ld_h, bs_h = _strides(h, T, H)
+        a = lib.GatedScanArgs(
+            pre.data_ptr(), ld, bs,
+            None if h0 is None else h0.data_ptr(), 0 if h0 is None or h0.dim() == 1 else _row_stride(h0, B, H, "h0"),
+            None if lengths is None else lengths.data_ptr(),
+            h.data_ptr(), ld_h, bs_h, last.data_ptr(), bs_hl, None if states is None else states.data_ptr(),
+            None, 0, 0, None, 0, None, 0, 0, None, None,
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            B, T, H, _ELEMENT[pre.dtype], reverse)
         lib.call("stes_gated_scan_fwd", C.byref(a))
     return h, last, states
 
@@ -105,27 +95,34 @@ class _GatedScan(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
         pre, lengths, states = ctx.saved_tensors
-        B, T, W = pre.shape
-        H = W // 2
-        dev = pre.device
-        dpre = torch.empty(B, T, W, dtype=pre.dtype, device=dev)
-        dh0 = torch.empty(B, H, dtype=torch.float32, device=dev) if ctx.h0_dim else None
-        total = torch.empty(H, dtype=torch.float32, device=dev) if ctx.h0_dim == 1 else None
-        if H and (B or total is not None):
-            with torch.cuda.device(dev):
-                a, _ws = _args(pre, None, lengths, ctx.reverse)
-                a.states = states.data_ptr()
-                if dh is not None:
-                    dh = _tidy(dh, H)
-                    a.dh = dh.data_ptr()
-                    a.ld_dh, a.bs_dh = _frames(dh, H, "dh")
-                if dlast is not None:
-                    dlast = dlast.contiguous()
-                    a.dh_last, a.bs_dhl = dlast.data_ptr(), H
-                a.dpre, a.ld_dpre, a.bs_dpre = dpre.data_ptr(), W, T * W
-                a.dh0, a.dh0_sum = lib.ptr(dh0), lib.ptr(total)
-                lib.call("stes_gated_scan_bwd", C.byref(a))
-        return dpre, (total if ctx.h0_dim == 1 else dh0), None, None
+        with lib.on_device(pre.device):
+            return _backward(pre, lengths, states, ctx.reverse, ctx.h0_dim, dh, dlast)
+
+
+def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast):
+    B, T, W = pre.shape
+    H, dev = W // 2, pre.device
+    dpre = torch.empty(B, T, W, dtype=pre.dtype, device=dev)
+    dh0 = torch.empty(B, H, dtype=torch.float32, device=dev) if h0_dim else None
+    total = torch.empty(H, dtype=torch.float32, device=dev) if h0_dim == 1 else None
+    if H and (B or total is not None):
+        ws = _workspace(B, T, H, dev)
+        ld, bs = _strides(pre, T, W)
+        ld_dh = bs_dh = 0
+        if dh is not None:
+            if not dh.is_contiguous() and ((H > 1 and dh.stride(2) != 1) or (T > 1 and dh.stride(1) < H)):
+                dh = dh.contiguous()                        # a gradient that was expanded or transposed
+            ld_dh, bs_dh = _strides(dh, T, H)
+        if dlast is not None:
+            dlast = dlast.contiguous()
+        a = lib.GatedScanArgs(
+            pre.data_ptr(), ld, bs, None, 0, None if lengths is None else lengths.data_ptr(), None, 0, 0, None, 0, states.data_ptr(),
+            None if dh is None else dh.data_ptr(), ld_dh, bs_dh, None if dlast is None else dlast.data_ptr(), H,
+            dpre.data_ptr(), W, T * W, None if dh0 is None else dh0.data_ptr(), None if total is None else total.data_ptr(),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            B, T, H, _ELEMENT[pre.dtype], reverse)
+        lib.call("stes_gated_scan_bwd", C.byref(a))
+    return dpre, (total if h0_dim == 1 else dh0), None, None
 
 
 def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=None):
@@ -140,40 +137,45 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
     -> h [B, T, H] in pre's type and the states after the last step, float32 [B, H] (h0 where a sequence is empty)
 
     Differentiable (once) in pre and h0, from h and from the final states.  T = 0 and T = 1 are calls like any other."""
-    _need(isinstance(pre, torch.Tensor) and pre.is_cuda and pre.dim() == 3 and pre.dtype in _ELEMENT,
-          "pre must be a bfloat16 or float32 tensor [B, T, 2H] on the GPU")
+    if not isinstance(pre, torch.Tensor) or not pre.is_cuda or pre.dim() != 3 or pre.dtype not in _ELEMENT:
+        _refuse("pre must be a bfloat16 or float32 tensor [B, T, 2H] on the GPU")
     B, T, W = pre.shape
-    _need(W % 2 == 0, f"the last dimension of pre holds gates and candidates and is even, got {W}")
     H, dev = W // 2, pre.device
-    _need(W <= 1 or pre.stride(2) == 1, "the last dimension of pre must be contiguous")
-    _need(T <= 1 or pre.stride(1) >= W, "frames of pre must not overlap")
+    if W % 2:
+        _refuse(f"the last dimension of pre holds gates and candidates and is even, got {W}")
+    if (W > 1 and pre.stride(2) != 1) or (T > 1 and pre.stride(1) < W):
+        _refuse("frames of pre must be contiguous and not overlap")
     if h0 is not None:
-        _need(h0.device == dev and h0.dtype == torch.float32 and tuple(h0.shape) in ((B, H), (H,)),
-              f"h0 must be float32 [{B}, {H}] or [{H}] on {dev}, got {h0.dtype} {list(h0.shape)} on {h0.device}")
-        if h0.dim() == 1:
-            _need(H <= 1 or h0.stride(0) == 1, "h0 must be contiguous")
-        elif (H > 1 and h0.stride(1) != 1) or (B > 1 and h0.stride(0) < H):
-            _need(state_out is None or state_out.data_ptr() != h0.data_ptr(), "a state in place needs contiguous rows that do not overlap")
+        if h0.device != dev or h0.dtype != torch.float32 or h0.shape not in ((B, H), (H,)):
+            _refuse(f"h0 must be float32 [{B}, {H}] or [{H}] on {dev}, got {h0.dtype} {list(h0.shape)} on {h0.device}")
+        if not h0.is_contiguous() and ((H > 1 and h0.stride(-1) != 1) or (h0.dim() == 2 and B > 1 and h0.stride(0) < H)):
+            if state_out is not None and state_out.data_ptr() == h0.data_ptr():
+                _refuse("a state in place needs contiguous rows that do not overlap")
             h0 = h0.contiguous()
-    if lengths is not None:
-        _need(lengths.device == dev and lengths.dtype == torch.int32 and tuple(lengths.shape) == (B,) and lengths.is_contiguous(),
-              f"lengths must be contiguous int32 [{B}] on {dev}, got {lengths.dtype} {list(lengths.shape)} on {lengths.device}")
+    if lengths is not None and (lengths.device != dev or lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous()):
+        _refuse(f"lengths must be contiguous int32 [{B}] on {dev}, got {lengths.dtype} {list(lengths.shape)} on {lengths.device}")
     wants_grad = torch.is_grad_enabled() and (pre.requires_grad or (h0 is not None and h0.requires_grad))
     if out is not None:
-        _need(out.device == dev and out.dtype == pre.dtype and tuple(out.shape) == (B, T, H), f"out must be {pre.dtype} [{B}, {T}, {H}] on {dev}")
-        _need((H <= 1 or out.stride(2) == 1) and _apart(out, H), "frames of out must be contiguous and not overlap")
-        _need(not out.numel() or out.data_ptr() != pre.data_ptr(), "out must not be pre's memory")
+        if wants_grad:
+            _refuse("out and state_out are for calls without gradients")
+        if out.device != dev or out.dtype != pre.dtype or out.shape != (B, T, H):
+            _refuse(f"out must be {pre.dtype} [{B}, {T}, {H}] on {dev}")
+        if (H > 1 and out.stride(2) != 1) or not _apart(out, H):
+            _refuse("frames of out must be contiguous and not overlap")
+        if out.numel() and out.data_ptr() == pre.data_ptr():
+            _refuse("out must not be pre's memory")
     if state_out is not None:
-        _need(state_out.device == dev, f"state_out must be on {dev}")
-        _rows(state_out, B, H, "state_out")
-        _need(h0 is None or state_out.data_ptr() != h0.data_ptr() or (h0.dim() == 2 and (B <= 1 or h0.stride(0) == state_out.stride(0))),
-              "a state in place is h0 itself, one row per sequence")
-    if wants_grad:
-        _need(out is None and state_out is None, "out and state_out are for calls without gradients")
-    with torch.cuda.device(dev):
+        if wants_grad:
+            _refuse("out and state_out are for calls without gradients")
+        if state_out.device != dev:
+            _refuse(f"state_out must be on {dev}")
+        stride = _row_stride(state_out, B, H, "state_out")
+        if h0 is not None and state_out.data_ptr() == h0.data_ptr() and B > 1 and (h0.dim() == 1 or h0.stride(0) != stride):
+            _refuse("a state in place is h0 itself, one row per sequence")
+    with lib.on_device(dev):
         if wants_grad:
             h, last = _GatedScan.apply(pre, h0, lengths, bool(reverse))
             lib.guard_leaves(h.grad_fn)
-            return h, last
-        h, last, _ = _forward(pre, h0, lengths, reverse, out, state_out, False)
+        else:
+            h, last, _ = _forward(pre, h0, lengths, bool(reverse), out, state_out, False)
     return h, last
