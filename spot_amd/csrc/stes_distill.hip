@@ -1,116 +1,353 @@
 // Distillation from a teacher's top logits (stes_distill / stes_distill_bwd in include/stes.h): the temperature-scaled KL divergence
 // of the student's softmax over all V classes from the teacher's softmax over its k best, and its gradient.
+//
+// Everything is bound by the logits' trip through memory, so they are read once: a team of threads holds a row (or a lane group a
+// short row) in registers as it was loaded, takes the maximum, the sum of exp, and writes q straight from the registers; the listed
+// classes, k of V, are written over by the lanes that hold them.  Rows too long for a workgroup's registers are read twice (the
+// second time mostly from the cache).
 #include "stes_common.h"
 
 namespace {
 
-struct Entry { int at; float p; };          // one listed class of a row: its index (-1: none) and its probability, duplicates merged
+template <typename T, int V> struct Vec;
+template <> struct Vec<bf16, 8> { typedef bf16x8 type; };
+template <> struct Vec<float, 4> { typedef f32x4 type; };
+template <typename T> struct Vec<T, 1> { typedef T type __attribute__((ext_vector_type(1))); };
 
-// The teacher's distribution of a row, one entry per lane of a wave (k <= 64).  -> bad: an index beyond V.  An index that is
-// listed again keeps its whole probability at its first place; the later places hold at < 0.
-__device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, long m, int lane, bool& some, bool& bad) {
-    Entry e{-1, 0.f};
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// reductions over the G lanes of an aligned lane group
+template <int G> __device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+template <int G> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+template <int G> __device__ __forceinline__ bool group_any(bool b, int lane) {
+    const uint64_t m = __ballot(b);
+    if (G == 64) return m != 0;
+    return ((m >> (lane & ~(G - 1))) & ((1ull << (G & 63)) - 1)) != 0;
+}
+
+struct Entry {
+    int at;                  // a listed class of the row; < 0: none in this lane
+    float p;                 // its probability
+    bool some, bad;          // of the row: it lists a class of some probability; it lists an index beyond V or a value that is no number
+};
+
+// a lane's value, from place j of the lane's group
+template <int G> __device__ __forceinline__ int from(int v, int j, int lane) {
+    return G == 64 ? __builtin_amdgcn_readlane(v, j) : __shfl(v, (lane & ~(G - 1)) + j, 64);
+}
+template <int G> __device__ __forceinline__ float from(float v, int j, int lane) { return __int_as_float(from<G>(__float_as_int(v), j, lane)); }
+
+// The teacher's distribution of row m, an entry per lane of a group of G >= k lanes (`l`: the lane's place in it).  A class that is
+// listed more than once has its whole probability at its first place; the later places hold none.  With entries == false only
+// what the row is worth (some, bad) is found out.
+template <int G>
+__device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, long m, bool row, int l, int lane, float ct, bool entries) {
+    Entry e;
+    e.at = -1;
     float v = -INFINITY;
-    if (lane < p.k) {
-        const long o = m * p.ld_idx + lane;
-        const long i = p.idx_i64 ? ((const int64_t*)p.idx)[o] : (long)((const int32_t*)p.idx)[o];
-        e.at = i < 0 ? -1 : (i >= p.V ? p.V : (int)i);
-        const long ov = m * p.ld_val + lane;
-        if (i >= 0) v = p.val_f32 ? ((const float*)p.val)[ov] : (float)((const bf16*)p.val)[ov];
+    if (row && l < p.k) {
+        const long o = m * p.ld_idx + l, i = p.idx_i64 ? ((const int64_t*)p.idx)[o] : (long)((const int32_t*)p.idx)[o];
+        const long ov = m * p.ld_val + l;
+        const float u = p.val_f32 ? ((const float*)p.val)[ov] : (float)((const bf16*)p.val)[ov];
+        if (i >= 0) { e.at = i >= p.V ? p.V : (int)i; v = u; }
     }
-    bad = __any(e.at >= p.V);
-    float mx = v;
-    bool nan = v != v;
-    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    bad = bad || __any(nan) || mx == INFINITY;
-    some = mx > -INFINITY || bad;
-    e.p = v > -INFINITY ? __expf((v - mx) / p.temperature) : 0.f;
-    e.p /= wave_sum(e.p);
+    const float mx = group_max<G>(v);                       // (fmaxf passes over NaN: those are caught below)
+    e.bad = group_any<G>(e.at >= p.V || v != v || v == INFINITY, lane);
+    e.some = mx > -INFINITY || e.bad;
+    e.p = 0.f;
+    if (!entries) return e;
+    float w = v > -INFINITY ? exp2_((v - mx) * ct) : 0.f;
+    w *= 1.f / group_sum<G>(w);
+    // merge duplicates
     float whole = 0.f;
-    bool first = true;
+    int first = G;
     for (int j = 0; j < p.k; ++j) {
-        const int aj = __shfl(e.at, j, 64);
-        const float pj = __shfl(e.p, j, 64);
-        if (aj == e.at) { whole += pj; first = first && j >= lane; }
+        const int aj = from<G>(e.at, j, lane);
+        const float pj = from<G>(w, j, lane);
+        if (aj == e.at) { whole += pj; first = first < j ? first : j; }
     }
     e.p = whole;
-    if (!first) e.at = -1;
+    if (first != l || !(whole > 0.f) || e.at >= p.V) e.at = -1;
     return e;
 }
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v = fmaxf(v, red[w]);
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) v += red[w];
-    return v;
+// the factor of a row's gradient
+__device__ __forceinline__ float row_factor(const stes_distill_args& p, float w, bool bad) {
+    const float f = (float)((double)p.temperature / p.denom) * p.grad_scale * w * (p.upstream ? p.upstream[0] : 1.f);
+    return bad ? __builtin_nanf("") : f;
 }
 
-template <typename TS, typename TG>
-__global__ __launch_bounds__(256) void distill_row_kernel(const stes_distill_args p, int have_stats, int want_loss) {
-    __shared__ float red[4];
-    const long m = blockIdx.x;
-    const TS* s = (const TS*)p.logits + m * p.ld;
-    TG* d = p.dlogits ? (TG*)p.dlogits + m * p.ld_d : nullptr;
-    const float w = p.weight ? p.weight[m] : 1.f, it = 1.f / p.temperature;
-    const int lane = threadIdx.x & 63;
-    bool some, bad;
-    const Entry e = teacher_row(p, m, lane, some, bad);
-    if (!some || w == 0.f) {
-        if (want_loss && threadIdx.x == 0) p.ws[m] = 0.f;
-        if (p.stats && !have_stats && threadIdx.x == 0) { p.stats[2 * m] = 0.f; p.stats[2 * m + 1] = 0.f; }
-        if (d && !p.accumulate) for (int v = threadIdx.x; v < p.V; v += 256) d[v] = (TG)0.f;
-        return;
+// A lane's part of KL = sum P (log P - log q), for the class that it holds: s is the class's logit
+__device__ __forceinline__ float kl_part(const Entry& e, float s, float mx, float sum, float it) {
+    return e.at >= 0 ? e.p * (logf(e.p) - ((s - mx) * it - logf(sum))) : 0.f;
+}
+
+// A workgroup's part of the loss; the only one of a launch is the loss.
+__device__ __forceinline__ void leave(const stes_distill_args& p, float* part, float sum, double factor) {
+    if (gridDim.x == 1) *p.loss = (float)(sum * factor);
+    else part[blockIdx.x] = sum;
+}
+
+enum { LOSS = 1, GRAD = 2, STATS_IN = 4 };           // what a launch does
+
+// ---------------------------------------------------------------- short rows
+// V <= 8 G and k <= G: a group of G lanes per row, at most 8 classes a lane, neighbouring lanes neighbouring classes.  256 / G rows a
+// workgroup and round; a workgroup's rows follow from its index alone, and so does the order of its sum.
+template <typename TS, typename TG, int G, int MODE>
+__global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_args p, int rounds, float* __restrict__ part, double factor) {
+    constexpr int E = 8, RPB = 256 / G;
+    __shared__ double red[4];
+    const int lane = threadIdx.x & 63, l = threadIdx.x % G;
+    const float it = 1.f / p.temperature, ct = it * LOG2E;
+    double total = 0.0;
+    for (int r = 0; r < rounds; ++r) {
+        const long m = ((long)blockIdx.x * rounds + r) * RPB + threadIdx.x / G;
+        const bool row = m < p.M;
+        const TS* s = (const TS*)p.logits + m * p.ld;
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = row && e * G + l < p.V ? (float)s[e * G + l] : -INFINITY;
+        const float w = row ? (p.weight ? p.weight[m] : 1.f) : 0.f;
+        const Entry t = teacher_row<G>(p, m, row, l, lane, ct, true);
+        const bool counts = t.some && w != 0.f;
+        float mx, sum;
+        if (MODE & STATS_IN) { mx = row ? p.stats[2 * m] : 0.f; sum = row ? p.stats[2 * m + 1] : 1.f; }
+        else {
+            mx = x[0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) mx = fmaxf(mx, x[e]);
+            mx = group_max<G>(mx);
+        }
+        float q[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[e] = e * G + l < p.V ? exp2_((x[e] - mx) * ct) : 0.f;
+        if (!(MODE & STATS_IN)) {
+            sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum += q[e];
+            sum = group_sum<G>(sum);
+            if (p.stats && row && l == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = sum; }
+        }
+        float pv[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) pv[e] = 0.f;
+        for (int j = 0; j < p.k; ++j) {                      // hand every entry to the lane whose registers hold its class
+            const int aj = from<G>(t.at, j, lane);
+            const float pj = from<G>(t.p, j, lane);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (aj == e * G + l) pv[e] = pj;
+        }
+        if (MODE & LOSS) {
+            float kl = 0.f;
+            const float ls = logf(sum);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (pv[e] > 0.f) kl += pv[e] * (logf(pv[e]) - ((x[e] - mx) * it - ls));
+            kl = group_sum<G>(kl);
+            if (t.bad) kl = __builtin_nanf("");
+            if (counts && l == 0) total += (double)(w * kl);
+        }
+        if ((MODE & GRAD) && row) {
+            const float f = row_factor(p, w, t.bad), inv = 1.f / sum;
+            TG* d = (TG*)p.dlogits + m * p.ld_d;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int v = e * G + l;
+                if (v < p.V) {
+                    const float g = counts ? f * (q[e] * inv - pv[e]) : 0.f;
+                    if (!p.accumulate) d[v] = (TG)g;
+                    else if (counts) d[v] = (TG)((float)d[v] + g);
+                }
+            }
+        }
     }
-    float mx, inv;
-    if (have_stats) { mx = p.stats[2 * m]; inv = p.stats[2 * m + 1]; }
-    else {
-        mx = -INFINITY;
-        for (int v = threadIdx.x; v < p.V; v += 256) mx = fmaxf(mx, (float)s[v]);
-        mx = block_max(mx, red);
-        float sum = 0.f;
-        for (int v = threadIdx.x; v < p.V; v += 256) sum += __expf(((float)s[v] - mx) * it);
-        sum = block_sum(sum, red);
-        inv = 1.f / sum;
-        if (p.stats && threadIdx.x == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = inv; }
+    if (MODE & LOSS) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+        if (lane == 0) red[threadIdx.x >> 6] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) leave(p, part, (float)(red[0] + red[1] + red[2] + red[3]), factor);
     }
-    const float sv = e.at >= 0 && e.at < p.V ? (float)s[e.at] : 0.f;
-    if (want_loss && threadIdx.x < 64) {
-        float kl = e.at >= 0 && e.p > 0.f ? e.p * (logf(e.p) - ((sv - mx) * it + logf(inv))) : 0.f;
-        kl = wave_sum(kl);
-        if (bad) kl = NAN;
-        if (threadIdx.x == 0) p.ws[m] = w * kl;
+}
+
+// ---------------------------------------------------------------- rows in registers
+// A team of TEAM threads holds a row: N vectors of 16 bytes a thread (W elements each), a few elements in front of the first 16-byte
+// boundary and behind the last one as single elements.  TEAM = 64: a wave per row, four rows a workgroup, no barrier.
+// STREAM: rows of any length, read again instead of held.
+template <int TEAM> struct Team {
+    static constexpr int WAVES = TEAM / 64;
+    static __device__ __forceinline__ float max_(float v, float* red) {
+        v = group_max<64>(v);
+        if (WAVES == 1) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v = fmaxf(v, red[w]);
+        return v;
     }
-    if (!d) return;
-    float f = (float)((double)p.temperature / p.denom) * p.grad_scale * w * (p.upstream ? p.upstream[0] : 1.f);
-    if (bad) f = NAN;
-    // the listed classes are written last, by the lanes that hold them: read what they add to first
-    const bool mine = threadIdx.x < 64 && e.at >= 0 && e.at < p.V && e.p > 0.f;
-    const float old = mine && p.accumulate ? (float)d[e.at] : 0.f;
-    __syncthreads();
-    for (int v = threadIdx.x; v < p.V; v += 256) {
-        const float g = f * (__expf(((float)s[v] - mx) * it) * inv);
-        d[v] = (TG)(p.accumulate ? (float)d[v] + g : g);
+    static __device__ __forceinline__ float sum_(float v, float* red) {
+        v = group_sum<64>(v);
+        if (WAVES == 1) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += red[w];
+        return v;
     }
-    __syncthreads();
-    if (mine) d[e.at] = (TG)(old + f * (__expf((sv - mx) * it) * inv - e.p));
+    static __device__ __forceinline__ void sync() {
+        if (WAVES > 1) __syncthreads();
+        else { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+    }
+};
+
+template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(const stes_distill_args p, float* __restrict__ part, double factor) {
+    typedef typename Vec<TS, W>::type VS;
+    typedef typename Vec<TG, W>::type VG;
+    typedef Team<TEAM> Tm;
+    __shared__ float red[TEAM / 64 > 4 ? TEAM / 64 : 4];
+    constexpr int RPB = TEAM == 64 ? 4 : 1;
+    const int lane = threadIdx.x & 63, i0 = threadIdx.x % TEAM;
+    const long m = (long)blockIdx.x * RPB + threadIdx.x / TEAM;
+    const bool row = m < p.M;
+    float out = 0.f;
+    if (row) {
+        const TS* s = (const TS*)p.logits + m * p.ld;
+        const float it = 1.f / p.temperature, ct = it * LOG2E;
+        const float w = p.weight ? p.weight[m] : 1.f;
+        const int V = p.V;
+        // [0, head) single, then nv vectors, then [tail, V) single
+        const int head = W == 1 ? 0 : min(V, (int)((16 - ((uintptr_t)s & 15)) & 15) / (int)sizeof(TS));
+        const int nv = (V - head) / W, tail = head + nv * W, rest = V - tail;
+        const VS* sv = reinterpret_cast<const VS*>(s + head);
+        const int single = i0 < head ? i0 : (i0 - head < rest ? tail + i0 - head : -1);        // (head + rest < 2 W <= TEAM)
+        VS x[STREAM ? 1 : N];
+        float x1 = -INFINITY;
+        if (W > 1 && single >= 0) x1 = (float)s[single];
+        if (!STREAM) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i * TEAM + i0 < nv) x[i] = sv[i * TEAM + i0];
+        }
+        const Entry t = teacher_row<64>(p, m, true, lane, lane, ct, threadIdx.x % TEAM < 64);
+        const float st = t.at >= 0 ? (float)s[t.at] : 0.f;
+        const bool counts = t.some && w != 0.f;
+        float mx = 0.f, sum = 1.f;
+        if (MODE & STATS_IN) { mx = p.stats[2 * m]; sum = p.stats[2 * m + 1]; }
+        else if (counts) {
+            mx = x1;
+            if (STREAM) {
+                // running maximum and sum: a thread's sum is scaled when its maximum rises
+                float acc = 0.f;
+                for (int i = i0; i < nv; i += TEAM) {
+                    const VS y = sv[i];
+                    float top = (float)y[0];
+#pragma unroll
+                    for (int e = 1; e < W; ++e) top = fmaxf(top, (float)y[e]);
+                    if (top > mx) { acc *= mx > -INFINITY ? exp2_((mx - top) * ct) : 0.f; mx = top; }
+                    float add = 0.f;
+                    if (mx > -INFINITY) {
+#pragma unroll
+                        for (int e = 0; e < W; ++e) add += exp2_(((float)y[e] - mx) * ct);
+                    } else {                                 // -inf and NaN alone so far
+#pragma unroll
+                        for (int e = 0; e < W; ++e) add += (float)y[e] == -INFINITY ? 0.f : __builtin_nanf("");
+                    }
+                    acc += add;
+                }
+                if (x1 > -INFINITY || x1 != x1) acc += exp2_((x1 - mx) * ct);
+                const float own = mx;
+                mx = Tm::max_(mx, red);
+                sum = Tm::sum_(own > -INFINITY || acc != 0.f ? acc * exp2_((own - mx) * ct) : 0.f, red);
+                if (mx == -INFINITY) sum = __builtin_nanf("");
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i * TEAM + i0 < nv)
+#pragma unroll
+                        for (int e = 0; e < W; ++e) mx = fmaxf(mx, (float)x[i][e]);
+                mx = Tm::max_(mx, red);
+                sum = W > 1 && single >= 0 ? exp2_((x1 - mx) * ct) : 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (i * TEAM + i0 < nv) {
+                        float add = 0.f;
+#pragma unroll
+                        for (int e = 0; e < W; ++e) add += exp2_(((float)x[i][e] - mx) * ct);
+                        sum += add;
+                    }
+                sum = Tm::sum_(sum, red);
+            }
+        }
+        if (!(MODE & STATS_IN) && p.stats && i0 == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = sum; }
+        if ((MODE & LOSS) && threadIdx.x % TEAM < 64) {
+            float kl = group_sum<64>(kl_part(t, st, mx, sum, it));
+            if (t.bad) kl = __builtin_nanf("");
+            out = counts ? w * kl : 0.f;
+        }
+        if (MODE & GRAD) {
+            TG* d = (TG*)p.dlogits + m * p.ld_d;
+            if (!counts) {
+                if (!p.accumulate) for (int v = i0; v < V; v += TEAM) d[v] = (TG)0.f;
+            } else {
+                const float f = row_factor(p, w, t.bad), fq = f / sum;
+                const bool mine = threadIdx.x % TEAM < 64 && t.at >= 0;
+                const float old = mine && p.accumulate ? (float)d[t.at] : 0.f;
+                if (p.accumulate) Tm::sync();                // (the listed classes are read before anyone adds to them)
+                VG* dv = reinterpret_cast<VG*>(d + head);
+                auto put = [&](int i, const VS& y) {
+                    VG o;
+                    if (p.accumulate) o = dv[i];
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const float g = fq * exp2_(((float)y[e] - mx) * ct);
+                        o[e] = (TG)(p.accumulate ? (float)o[e] + g : g);
+                    }
+                    dv[i] = o;
+                };
+                if (STREAM) for (int i = i0; i < nv; i += TEAM) put(i, sv[i]);
+                else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (i * TEAM + i0 < nv) put(i * TEAM + i0, x[i]);
+                }
+                if (W > 1 && single >= 0) {
+                    const float g = fq * exp2_((x1 - mx) * ct);
+                    d[single] = (TG)(p.accumulate ? (float)d[single] + g : g);
+                }
+                Tm::sync();                                  // the listed classes are written last
+                if (mine) d[t.at] = (TG)(old + (fq * exp2_((st - mx) * ct) - f * t.p));
+            }
+        }
+    }
+    if (MODE & LOSS) {
+        if (TEAM == 64) {
+            if (lane == 0) red[threadIdx.x >> 6] = out;
+            __syncthreads();
+            if (threadIdx.x == 0) leave(p, part, (red[0] + red[1]) + (red[2] + red[3]), factor);
+        } else if (threadIdx.x == 0) leave(p, part, out, factor);
+    }
 }
 
 // loss = factor * (part[0] + part[1] + ...), in a fixed order
 __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ part, int n, double factor, float* __restrict__ loss) {
     __shared__ double red[16];
     double s = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -122,6 +359,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     }
 }
 
+// ---------------------------------------------------------------- host
 int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->M >= 0 && a->V >= 1 && a->k >= 1, STES_ERR_ARG, "stes_distill: M >= 0, V >= 1 and k >= 1");
@@ -130,6 +368,7 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a->denom > 0.0, STES_ERR_ARG, "stes_distill: the denominator is positive");
     STES_CHECK(bwd || a->loss, STES_ERR_ARG, "stes_distill: loss is needed");
     if (!a->M) return STES_OK;
+    STES_CHECK(a->V < 0x7fff0000, STES_ERR_UNSUPPORTED, "stes_distill: too many classes");
     STES_CHECK(a->logits && a->idx && a->val, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->ld >= a->V && a->ld_idx >= a->k && a->ld_val >= a->k, STES_ERR_ARG, "stes_distill: rows overlap");
     STES_CHECK(!a->dlogits || a->ld_d >= a->V, STES_ERR_ARG, "stes_distill: rows of dlogits overlap");
@@ -139,10 +378,69 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     return STES_OK;
 }
 
+double loss_factor(const stes_distill_args& a) { return (double)a.temperature * a.temperature / a.denom; }
+
+template <typename TS, typename TG, int G, int MODE>
+int launch_short(const stes_distill_args& a, hipStream_t s) {
+    constexpr int RPB = 256 / G;
+    const long teams = ((long)a.M + RPB - 1) / RPB;
+    const int rounds = (int)((teams + 2047) / 2048), blocks = (int)((teams + rounds - 1) / rounds);
+    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a));
+    return blocks;
+}
+
+template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
+int launch_row(const stes_distill_args& a, hipStream_t s) {
+    constexpr int RPB = TEAM == 64 ? 4 : 1;
+    const int blocks = (int)(((long)a.M + RPB - 1) / RPB);
+    hipLaunchKernelGGL((distill_row_kernel<TS, TG, W, TEAM, N, STREAM, MODE>), dim3(blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, s, a, a.ws, loss_factor(a));
+    return blocks;
+}
+
+// -> how many partial sums the launch leaves
+template <typename TS, typename TG, int W, int MODE>
+int launch_rows(const stes_distill_args& a, hipStream_t s) {
+    if constexpr (W == 1) {
+        return launch_row<TS, TG, 1, 256, 1, true, MODE>(a, s);
+    } else {
+        if constexpr ((MODE & STATS_IN) != 0) {              // nothing is reduced: read, write
+            if (a.V <= 64 * 8 * W) return launch_row<TS, TG, W, 64, 1, true, MODE>(a, s);
+            return launch_row<TS, TG, W, 256, 1, true, MODE>(a, s);
+        } else {
+            const int vecs = (a.V + W - 1) / W;
+            if (vecs <= 64 * 8) return launch_row<TS, TG, W, 64, 8, false, MODE>(a, s);
+            if (vecs <= 256 * 8) return launch_row<TS, TG, W, 256, 8, false, MODE>(a, s);
+            if (vecs <= 512 * 8) return launch_row<TS, TG, W, 512, 8, false, MODE>(a, s);
+            if (vecs <= 1024 * 8) return launch_row<TS, TG, W, 1024, 8, false, MODE>(a, s);
+            return launch_row<TS, TG, W, 1024, 1, true, MODE>(a, s);
+        }
+    }
+}
+
+template <typename TS, typename TG, int MODE>
+int launch_mode(const stes_distill_args& a, hipStream_t s) {
+    if (a.V <= 8 * 64) {
+        const int g = a.k > (a.V + 7) / 8 ? a.k : (a.V + 7) / 8;
+        if (g <= 4) return launch_short<TS, TG, 4, MODE>(a, s);
+        if (g <= 8) return launch_short<TS, TG, 8, MODE>(a, s);
+        if (g <= 16) return launch_short<TS, TG, 16, MODE>(a, s);
+        if (g <= 32) return launch_short<TS, TG, 32, MODE>(a, s);
+        return launch_short<TS, TG, 64, MODE>(a, s);
+    }
+    if constexpr (sizeof(TS) == sizeof(TG)) {
+        // 16-byte accesses need the rows of logits and of dlogits at the same offset from a 16-byte boundary
+        constexpr int W = 16 / sizeof(TS);
+        const bool same = !(MODE & GRAD) || ((((uintptr_t)a.logits ^ (uintptr_t)a.dlogits) & 15) == 0 && (a.M == 1 || ((a.ld - a.ld_d) * (int)sizeof(TS) & 15) == 0));
+        if (same && (uintptr_t)a.logits % sizeof(TS) == 0) return launch_rows<TS, TG, W, MODE>(a, s);
+    }
+    return launch_rows<TS, TG, 1, MODE>(a, s);
+}
+
 template <typename TS>
-void distill_launch(const stes_distill_args& a, bool bwd, hipStream_t s) {
-    if (a.d_f32) hipLaunchKernelGGL((distill_row_kernel<TS, float>), dim3(a.M), dim3(256), 0, s, a, (int)bwd, (int)!bwd);
-    else hipLaunchKernelGGL((distill_row_kernel<TS, bf16>), dim3(a.M), dim3(256), 0, s, a, (int)bwd, (int)!bwd);
+int launch(const stes_distill_args& a, bool bwd, hipStream_t s) {
+    if (bwd) return a.d_f32 ? launch_mode<TS, float, GRAD | STATS_IN>(a, s) : launch_mode<TS, bf16, GRAD | STATS_IN>(a, s);
+    if (!a.dlogits) return launch_mode<TS, TS, LOSS>(a, s);
+    return a.d_f32 ? launch_mode<TS, float, LOSS | GRAD>(a, s) : launch_mode<TS, bf16, LOSS | GRAD>(a, s);
 }
 
 }  // namespace
@@ -155,13 +453,15 @@ extern "C" int64_t stes_distill_ws_floats(int M, int V) {
 extern "C" int stes_distill(const stes_distill_args* a, void* stream) {
     const int rc = distill_check(a, false);
     if (rc) return rc;
+    int parts = 0;
     if (a->M) {
-        if (a->f32) distill_launch<float>(*a, false, (hipStream_t)stream);
-        else distill_launch<bf16>(*a, false, (hipStream_t)stream);
+        parts = a->f32 ? launch<float>(*a, false, (hipStream_t)stream) : launch<bf16>(*a, false, (hipStream_t)stream);
         STES_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a->ws, a->M, (double)a->temperature * a->temperature / a->denom, a->loss);
-    STES_LAUNCH_CHECK();
+    if (parts != 1) {                                        // (no rows: a sum of nothing)
+        hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a->ws, parts, loss_factor(*a), a->loss);
+        STES_LAUNCH_CHECK();
+    }
     return STES_OK;
 }
 
@@ -169,8 +469,8 @@ extern "C" int stes_distill_bwd(const stes_distill_args* a, void* stream) {
     const int rc = distill_check(a, true);
     if (rc) return rc;
     if (!a->M) return STES_OK;
-    if (a->f32) distill_launch<float>(*a, true, (hipStream_t)stream);
-    else distill_launch<bf16>(*a, true, (hipStream_t)stream);
+    if (a->f32) launch<float>(*a, true, (hipStream_t)stream);
+    else launch<bf16>(*a, true, (hipStream_t)stream);
     STES_LAUNCH_CHECK();
     return STES_OK;
 }
