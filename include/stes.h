@@ -472,7 +472,7 @@ int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h
  * the sum of dh0 over the batch in a fixed order, for an initial state that the batch shares.
  * T = 0 is a call (h_last = h0).  ws: stes_gated_scan_ws_bytes(B, T, H) bytes, contents irrelevant; calls that may overlap need one each.
  * Results do not depend on scheduling beyond the association of the time axis: see stes_scan.hip. */
-#define STES_SCAN_BLOCK 128
+#define STES_SCAN_BLOCK 256
 typedef struct {
     const void* pre; int64_t ld_pre, bs_pre;
     const float* h0; int64_t bs_h0; const int32_t* lengths;

@@ -16,17 +16,38 @@
 
 namespace {
 
-template <typename T, int V> struct Vec;
-template <> struct Vec<bf16, 8> { typedef bf16x8 type; };
-template <> struct Vec<float, 4> { typedef f32x4 type; };
-template <typename T> struct Vec<T, 1> { typedef T type __attribute__((ext_vector_type(1))); };
+// 16 bytes of a row, at any address that is a multiple of the element's size (global memory takes 16-byte accesses there)
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16> { static constexpr int V = 8; typedef bf16x8 type; typedef bf16x8 anywhere __attribute__((aligned(2))); };
+template <> struct Chunk<float> { static constexpr int V = 4; typedef f32x4 type; typedef f32x4 anywhere __attribute__((aligned(4))); };
 
-// z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open)
+// the first `left` elements of a chunk, the whole of it where left >= V
+template <typename T>
+__device__ __forceinline__ typename Chunk<T>::type load_chunk(const T* p, int left) {
+    typename Chunk<T>::type r;
+    if (left >= Chunk<T>::V) r = *reinterpret_cast<const typename Chunk<T>::anywhere*>(p);
+    else {
+#pragma unroll
+        for (int v = 0; v < Chunk<T>::V; ++v) r[v] = v < left ? p[v] : (T)0.f;
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, typename Chunk<T>::type x, int left) {
+    if (left >= Chunk<T>::V) *reinterpret_cast<typename Chunk<T>::anywhere*>(p) = x;
+    else {
+#pragma unroll
+        for (int v = 0; v < Chunk<T>::V; ++v)
+            if (v < left) p[v] = x[v];
+    }
+}
+
+// z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open).  Gates
+// below -86 count as -86 (z = 2^-125 there); the minimum hands NaN on.
 __device__ __forceinline__ void gate_pair(float x, float& z, float& a) {
-    const float t = __expf(-fabsf(x));
-    const float big = __builtin_amdgcn_rcpf(1.f + t), small = t * big;
-    z = x >= 0.f ? big : small;
-    a = x >= 0.f ? small : big;
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(x * -1.4426950408889634f, 125.f));
+    z = __builtin_amdgcn_rcpf(1.f + e);
+    a = e * z;
 }
 
 __device__ __forceinline__ int seq_len(const stes_gated_scan_args& p, int b) {
@@ -49,11 +70,11 @@ __device__ __forceinline__ uint64_t peek(const uint64_t* w) { return __hip_atomi
 __device__ __forceinline__ uint64_t map_word(float A, float B) { return ((uint64_t)__float_as_uint(B) << 32) | (__float_as_uint(A) | 0x80000000u); }
 __device__ __forceinline__ uint64_t state_word(float x) { return ((uint64_t)__float_as_uint(x) << 32) | 1u; }
 
-constexpr int LOOK = 8;                  // blocks looked at in one round trip to memory
+constexpr int LOOK = 4;                  // blocks looked at in one round trip to memory
 constexpr int MAX_ROUNDS = 1 << 22;      // (an exit for a broken workspace: the state becomes NaN)
 
-// The state in front of block `blk` of a channel (blk >= 1): `at` is the channel's word in block 0's row, `row` the words of a row.
-__device__ __forceinline__ float look_back(const Link& l, long at, long row, int blk) {
+// The state in front of block `blk` >= 1 of a channel; `at` is the channel's word in a row of `words` words.
+__device__ __forceinline__ float look_back(const Link& l, long at, long words, int blk) {
     float A = 1.f, B = 0.f;
     int t = blk - 1;
     for (int round = 0; round < MAX_ROUNDS; ++round) {
@@ -61,27 +82,22 @@ __device__ __forceinline__ float look_back(const Link& l, long at, long row, int
 #pragma unroll
         for (int k = 0; k < LOOK; ++k) {
             const int q = t - k < 0 ? 0 : t - k;
-            st[k] = peek(l.state + q * row + at);
-            mp[k] = peek(l.map + q * row + at);
+            st[k] = peek(l.state + q * words + at);
+            mp[k] = peek(l.map + q * words + at);
         }
-        int used = 0;
-        bool found = false, open = true;
-        float x = 0.f;
+        const int before = t;
+        bool open = true;
 #pragma unroll
         for (int k = 0; k < LOOK; ++k) {
-            if (open && t - k >= 0) {
-                if (st[k]) { x = __uint_as_float((uint32_t)(st[k] >> 32)); found = true; open = false; }
-                else if (mp[k]) {
-                    B = A * __uint_as_float((uint32_t)(mp[k] >> 32)) + B;
-                    A = A * __uint_as_float((uint32_t)mp[k] & 0x7fffffffu);
-                    ++used;
-                } else open = false;
-            }
+            if (!open || before - k < 0) continue;
+            if (st[k]) return A * __uint_as_float((uint32_t)(st[k] >> 32)) + B;
+            if (mp[k]) {
+                B = A * __uint_as_float((uint32_t)(mp[k] >> 32)) + B;
+                A = A * __uint_as_float((uint32_t)mp[k] & 0x7fffffffu);
+                --t;                     // (block 0 publishes a state and no map: the walk ends there)
+            } else open = false;
         }
-        if (found) return A * x + B;
-        t -= used;
-        if (t < 0) t = 0;                // (block 0 publishes a state: it is found there)
-        if (!used) __builtin_amdgcn_s_sleep(1);
+        if (t == before) __builtin_amdgcn_s_sleep(1);
     }
     return __builtin_nanf("");
 }
@@ -92,12 +108,13 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(u32x4* __restrict__ w, 
 }
 
 // ---------------------------------------------------------------- tiles
-// A workgroup of NT threads: LPR lanes side by side take LPR * V channels of a frame (256 bytes of bf16 or fp32 a row), NT / LPR
-// segments of L steps one after the other in time.
-template <typename T_, int V_, int LPR_, int L_>
+// A workgroup of NT threads: LPR lanes side by side take 64 channels of a frame (128 bytes of bf16, 256 of fp32), NT / LPR segments
+// of L steps one after the other in time.
+template <typename T_, int LPR_, int L_>
 struct Tile {
     typedef T_ T;
-    static constexpr int V = V_, LPR = LPR_, L = L_, CT = LPR * V, NS = STES_SCAN_BLOCK / L, NT = NS * LPR, NW = NT / 64, SW = 64 / LPR, CPL = CT / 64;
+    static constexpr int V = Chunk<T>::V, LPR = LPR_, L = L_, CT = LPR * V, NS = STES_SCAN_BLOCK / L, NT = NS * LPR, NW = NT / 64, SW = 64 / LPR;
+    static_assert(CT == 64, "a lane of a wave per channel");
 };
 
 struct Place { int b, c0, n, blk; long chain; };
@@ -123,7 +140,7 @@ __device__ __forceinline__ Place place(const stes_gated_scan_args& p, int tiles,
 template <class G, bool JOIN>
 __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_args p, int tiles, long chains, int blocks, unsigned* ticket, Link link) {
     typedef typename G::T T;
-    typedef typename Vec<T, G::V>::type VT;
+    typedef typename Chunk<T>::type VT;
     constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
     __shared__ float sA[G::NS][CT], sB[G::NS][CT];       // maps of the segments, then of what precedes them in their wave
     __shared__ float tA[NW][CT], tB[NW][CT];             // maps of the waves; tB then: the state in front of each
@@ -131,71 +148,72 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
     const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
     const int tid = threadIdx.x, cl = tid % G::LPR, seg = tid / G::LPR, lane = tid & 63, wave = tid >> 6;
     const int c = at.c0 + cl * V, n = at.n, s0 = at.blk * STES_SCAN_BLOCK + seg * L;
-    const bool on = c < p.H;
+    const int left = p.H - c;
+    const bool on = left > 0;
     const long H = p.H, step = p.reverse ? -p.ld_pre : p.ld_pre;
     const T* row = (const T*)p.pre + at.b * p.bs_pre + c + (p.reverse ? (long)(n - 1 - s0) : (long)s0) * p.ld_pre;
     VT g[L], cand[L];
 #pragma unroll
     for (int j = 0; j < L; ++j)
         if (on && s0 + j < n) {
-            g[j] = *reinterpret_cast<const VT*>(row + j * step);
-            cand[j] = *reinterpret_cast<const VT*>(row + j * step + H);
+            g[j] = load_chunk<T>(row + j * step, left);
+            cand[j] = load_chunk<T>(row + j * step + H, left);
         }
     float a[L][V], u[L][V], A[V], B[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-        const bool live = on && s0 + j < n;
+        if (on && s0 + j < n) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float z, k;
-            gate_pair((float)g[j][v], z, k);
-            a[j][v] = live ? k : 1.f;
-            u[j][v] = live ? z * (float)cand[j][v] : 0.f;
-            A[v] *= a[j][v];
-            B[v] = a[j][v] * B[v] + u[j][v];
+            for (int v = 0; v < V; ++v) {
+                float z;
+                gate_pair((float)g[j][v], z, a[j][v]);
+                u[j][v] = z * (float)cand[j][v];
+                A[v] *= a[j][v];
+                B[v] = a[j][v] * B[v] + u[j][v];
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { a[j][v] = 1.f; u[j][v] = 0.f; }
         }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v]; sB[seg][cl * V + v] = B[v]; }
     wave_lds_fence();
-#pragma unroll
-    for (int q = 0; q < G::CPL; ++q) {
-        const int ch = q * 64 + lane;
-        float fa = 1.f, fb = 0.f;
+    {
+        float fa = 1.f, fb = 0.f;                            // lane = channel
 #pragma unroll
         for (int i = 0; i < SW; ++i) {
-            const float ia = sA[wave * SW + i][ch], ib = sB[wave * SW + i][ch];
-            sA[wave * SW + i][ch] = fa;
-            sB[wave * SW + i][ch] = fb;
+            const float ia = sA[wave * SW + i][lane], ib = sB[wave * SW + i][lane];
+            sA[wave * SW + i][lane] = fa;
+            sB[wave * SW + i][lane] = fb;
             fb = ia * fb + ib;
             fa = ia * fa;
         }
-        tA[wave][ch] = fa;
-        tB[wave][ch] = fb;
+        tA[wave][lane] = fa;
+        tB[wave][lane] = fb;
     }
     __syncthreads();
-    if (tid < CT) {
-        const int ch = at.c0 + tid;
-        const bool live = ch < p.H;
+    if (wave == 0) {
+        const int ch = at.c0 + lane;
         float x = 0.f, fa[NW], fb[NW], mA = 1.f, mB = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][tid]; fb[w] = tB[w][tid]; mB = fa[w] * mB + fb[w]; mA = fa[w] * mA; }
-        const long word = at.chain * CT + tid, words = chains * CT;
-        if (live) {
-            if (at.blk == 0) x = p.h0 ? p.h0[at.b * p.bs_h0 + ch] : 0.f;
-            else if (JOIN) {
+        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][lane]; fb[w] = tB[w][lane]; mB = fa[w] * mB + fb[w]; mA = fa[w] * mA; }
+        const long word = at.chain * CT + lane, words = chains * CT;
+        if (ch < p.H) {
+            if (!JOIN || at.blk == 0) x = p.h0 ? p.h0[at.b * p.bs_h0 + ch] : 0.f;
+            else {
                 if (at.blk + 1 < blocks) publish(link.map + at.blk * words + word, map_word(mA, mB));
                 x = look_back(link, word, words, at.blk);
             }
             const float end = mA * x + mB;
             if (JOIN && at.blk + 1 < blocks) publish(link.state + at.blk * words + word, state_word(end));
-            if (p.states) p.states[((long)at.b * blocks + at.blk) * H + ch] = x;
             if (at.blk + 1 == blocks && p.h_last) p.h_last[at.b * p.bs_hl + ch] = end;
+            if (p.states) p.states[((long)at.b * blocks + at.blk) * H + ch] = x;
         }
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { tB[w][tid] = x; x = fa[w] * x + fb[w]; }
+        for (int w = 0; w < NW; ++w) { tB[w][lane] = x; x = fa[w] * x + fb[w]; }
     }
     __syncthreads();
     if (!on) return;
@@ -212,7 +230,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
             x[v] = a[j][v] * x[v] + u[j][v];
             o[v] = (T)(s < n ? x[v] : 0.f);
         }
-        if (s < p.T) *reinterpret_cast<VT*>(out + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h) = o;
+        if (s < p.T) store_chunk<T>(out + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h, o, left);
     }
 }
 
@@ -220,16 +238,17 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
 template <class G, bool JOIN>
 __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_args p, int tiles, long chains, int blocks, unsigned* ticket, Link link) {
     typedef typename G::T T;
-    typedef typename Vec<T, G::V>::type VT;
+    typedef typename Chunk<T>::type VT;
     constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
     __shared__ float sA[G::NS][CT], sB[G::NS][CT], sR[G::NS][CT], sS[G::NS][CT];
-    __shared__ float tA[NW][CT], tB[NW][CT], tR[NW][CT];
+    __shared__ float tA[NW][CT], tB[NW][CT], tR[NW][CT];             // tB and tR then: what comes to a wave from either side
     __shared__ unsigned drawn;
     const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
     const int blk = blocks - 1 - at.blk;
     const int tid = threadIdx.x, cl = tid % G::LPR, seg = tid / G::LPR, lane = tid & 63, wave = tid >> 6;
     const int c = at.c0 + cl * V, n = at.n, s0 = blk * STES_SCAN_BLOCK + seg * L;
-    const bool on = c < p.H;
+    const int left = p.H - c;
+    const bool on = left > 0;
     const long H = p.H, t0 = p.reverse ? (long)(n - 1 - s0) : (long)s0, sign = p.reverse ? -1 : 1;
     const T* row = (const T*)p.pre + at.b * p.bs_pre + c + t0 * p.ld_pre;
     const T* drow = p.dh ? (const T*)p.dh + at.b * p.bs_dh + c + t0 * p.ld_dh : nullptr;
@@ -240,9 +259,9 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
 #pragma unroll
         for (int v = 0; v < V; ++v) d[j][v] = (T)0.f;
         if (live) {
-            g[j] = *reinterpret_cast<const VT*>(row + sign * j * p.ld_pre);
-            cand[j] = *reinterpret_cast<const VT*>(row + sign * j * p.ld_pre + H);
-            if (drow) d[j] = *reinterpret_cast<const VT*>(drow + sign * j * p.ld_dh);
+            g[j] = load_chunk<T>(row + sign * j * p.ld_pre, left);
+            cand[j] = load_chunk<T>(row + sign * j * p.ld_pre + H, left);
+            if (drow) d[j] = load_chunk<T>(drow + sign * j * p.ld_dh, left);
         }
     }
     // the segment's maps, forwards (A, B) and backwards (A, R)
@@ -251,58 +270,55 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
     for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; R[v] = 0.f; }
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-        const bool live = on && s0 + j < n;
+        if (on && s0 + j < n) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float z, k;
-            gate_pair((float)g[j][v], z, k);
-            k = live ? k : 1.f;
-            const float u = live ? z * (float)cand[j][v] : 0.f;
-            B[v] = k * B[v] + u;
-            A[v] *= k;
-            R[v] += A[v] * (float)d[j][v];               // d_j reaches the segment's front through a_0 .. a_j
+            for (int v = 0; v < V; ++v) {
+                float z, k;
+                gate_pair((float)g[j][v], z, k);
+                B[v] = k * B[v] + z * (float)cand[j][v];
+                A[v] *= k;
+                R[v] += A[v] * (float)d[j][v];           // d_j reaches the segment's front through a_0 .. a_j
+            }
         }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v]; sB[seg][cl * V + v] = B[v]; sR[seg][cl * V + v] = R[v]; }
     wave_lds_fence();
+    {
+        float ia[SW], ib[SW], ir[SW], fa = 1.f, fb = 0.f, ra = 1.f, rr = 0.f;          // lane = channel
 #pragma unroll
-    for (int q = 0; q < G::CPL; ++q) {
-        const int ch = q * 64 + lane;
-        float ia[SW], ib[SW], ir[SW], fa = 1.f, fb = 0.f, ra = 1.f, rr = 0.f;
-#pragma unroll
-        for (int i = 0; i < SW; ++i) { ia[i] = sA[wave * SW + i][ch]; ib[i] = sB[wave * SW + i][ch]; ir[i] = sR[wave * SW + i][ch]; }
+        for (int i = 0; i < SW; ++i) { ia[i] = sA[wave * SW + i][lane]; ib[i] = sB[wave * SW + i][lane]; ir[i] = sR[wave * SW + i][lane]; }
 #pragma unroll
         for (int i = 0; i < SW; ++i) {
-            sA[wave * SW + i][ch] = fa;
-            sB[wave * SW + i][ch] = fb;
+            sA[wave * SW + i][lane] = fa;
+            sB[wave * SW + i][lane] = fb;
             fb = ia[i] * fb + ib[i];
             fa = ia[i] * fa;
         }
 #pragma unroll
         for (int i = SW - 1; i >= 0; --i) {
-            sS[wave * SW + i][ch] = ra;
-            sR[wave * SW + i][ch] = rr;
+            sS[wave * SW + i][lane] = ra;
+            sR[wave * SW + i][lane] = rr;
             rr = ia[i] * rr + ir[i];
             ra = ia[i] * ra;
         }
-        tA[wave][ch] = fa;
-        tB[wave][ch] = fb;
-        tR[wave][ch] = rr;
+        tA[wave][lane] = fa;
+        tB[wave][lane] = fb;
+        tR[wave][lane] = rr;
     }
     __syncthreads();
-    if (tid < CT) {
-        const int ch = at.c0 + tid;
+    if (wave == 0) {
+        const int ch = at.c0 + lane;
         float fa[NW], fb[NW], fr[NW], mA = 1.f, mR = 0.f, x = 0.f, k = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][tid]; fb[w] = tB[w][tid]; fr[w] = tR[w][tid]; }
+        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][lane]; fb[w] = tB[w][lane]; fr[w] = tR[w][lane]; }
 #pragma unroll
         for (int w = NW - 1; w >= 0; --w) { mR = fa[w] * mR + fr[w]; mA = fa[w] * mA; }
-        const long word = at.chain * CT + tid, words = chains * CT;
+        const long word = at.chain * CT + lane, words = chains * CT;
         if (ch < p.H) {
             x = p.states[((long)at.b * blocks + blk) * H + ch];
-            if (at.blk == 0) k = p.dh_last ? p.dh_last[at.b * p.bs_dhl + ch] : 0.f;
-            else if (JOIN) {
+            if (!JOIN || at.blk == 0) k = p.dh_last ? p.dh_last[at.b * p.bs_dhl + ch] : 0.f;
+            else {
                 if (blk) publish(link.map + at.blk * words + word, map_word(mA, mR));
                 k = look_back(link, word, words, at.blk);
             }
@@ -311,9 +327,9 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
             if (!blk && p.dh0) p.dh0[at.b * H + ch] = front;
         }
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { tB[w][tid] = x; x = fa[w] * x + fb[w]; }
+        for (int w = 0; w < NW; ++w) { tB[w][lane] = x; x = fa[w] * x + fb[w]; }
 #pragma unroll
-        for (int w = NW - 1; w >= 0; --w) { tR[w][tid] = k; k = fa[w] * k + fr[w]; }
+        for (int w = NW - 1; w >= 0; --w) { tR[w][lane] = k; k = fa[w] * k + fr[w]; }
     }
     __syncthreads();
     if (!on) return;
@@ -353,8 +369,8 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
             for (int v = 0; v < V; ++v) og[v] = oc[v] = (T)0.f;
         }
         T* o = out + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_dpre;
-        *reinterpret_cast<VT*>(o) = og;
-        *reinterpret_cast<VT*>(o + H) = oc;
+        store_chunk<T>(o, og, left);
+        store_chunk<T>(o + H, oc, left);
     }
 }
 
@@ -362,12 +378,13 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
 // T <= SHORT: a thread walks all steps of V channels; nothing is shared (frames of streams, one at a time).
 constexpr int SHORT = 8;
 
-template <typename T, int V, bool BWD>
+template <typename T, bool BWD>
 __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_args p, long groups) {
-    typedef typename Vec<T, V>::type VT;
+    typedef typename Chunk<T>::type VT;
+    constexpr int V = Chunk<T>::V;
     const long id = (long)blockIdx.x * 64 + threadIdx.x, per = (p.H + V - 1) / V;
     if (id >= groups) return;
-    const int b = (int)(id / per), c = (int)(id - b * per) * V, n = seq_len(p, b);
+    const int b = (int)(id / per), c = (int)(id - b * per) * V, n = seq_len(p, b), left = p.H - c;
     const long H = p.H;
     const T* pre = (const T*)p.pre + b * p.bs_pre + c;
     const T* dh = BWD && p.dh ? (const T*)p.dh + b * p.bs_dh + c : nullptr;
@@ -376,16 +393,18 @@ __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_ar
     for (int s = 0; s < SHORT; ++s)
         if (s < n) {
             const long t = p.reverse ? n - 1 - s : s;
-            g[s] = *reinterpret_cast<const VT*>(pre + t * p.ld_pre);
-            cand[s] = *reinterpret_cast<const VT*>(pre + t * p.ld_pre + H);
-            if (BWD && dh) d[s] = *reinterpret_cast<const VT*>(dh + t * p.ld_dh);
+            g[s] = load_chunk<T>(pre + t * p.ld_pre, left);
+            cand[s] = load_chunk<T>(pre + t * p.ld_pre + H, left);
+            if (BWD && dh) d[s] = load_chunk<T>(dh + t * p.ld_dh, left);
         }
     float x[V], before[BWD ? SHORT : 1][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        if (BWD) x[v] = p.T ? p.states[b * H + c + v] : 0.f;
+        x[v] = 0.f;
+        if (v >= left) continue;
+        if (BWD) { if (p.T) x[v] = p.states[b * H + c + v]; }
         else {
-            x[v] = p.h0 ? p.h0[b * p.bs_h0 + c + v] : 0.f;
+            if (p.h0) x[v] = p.h0[b * p.bs_h0 + c + v];
             if (p.states && p.T) p.states[b * H + c + v] = x[v];
         }
     }
@@ -403,17 +422,18 @@ __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_ar
             }
             o[v] = (T)(s < n ? x[v] : 0.f);
         }
-        if (!BWD) *reinterpret_cast<VT*>((T*)p.h + b * p.bs_h + c + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h) = o;
+        if (!BWD) store_chunk<T>((T*)p.h + b * p.bs_h + c + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_h, o, left);
     }
     if (!BWD) {
         if (p.h_last)
 #pragma unroll
-            for (int v = 0; v < V; ++v) p.h_last[b * p.bs_hl + c + v] = x[v];
+            for (int v = 0; v < V; ++v)
+                if (v < left) p.h_last[b * p.bs_hl + c + v] = x[v];
         return;
     }
     float k[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) k[v] = p.dh_last ? p.dh_last[b * p.bs_dhl + c + v] : 0.f;
+    for (int v = 0; v < V; ++v) k[v] = p.dh_last && v < left ? p.dh_last[b * p.bs_dhl + c + v] : 0.f;
 #pragma unroll
     for (int s = SHORT - 1; s >= 0; --s) {
         if (s >= p.T) continue;
@@ -431,12 +451,13 @@ __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_ar
             }
         }
         T* o = (T*)p.dpre + b * p.bs_dpre + c + (long)(p.reverse && s < n ? n - 1 - s : s) * p.ld_dpre;
-        *reinterpret_cast<VT*>(o) = og;
-        *reinterpret_cast<VT*>(o + H) = oc;
+        store_chunk<T>(o, og, left);
+        store_chunk<T>(o + H, oc, left);
     }
     if (p.dh0)
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.dh0[b * H + c + v] = k[v];
+        for (int v = 0; v < V; ++v)
+            if (v < left) p.dh0[b * H + c + v] = k[v];
 }
 
 // The gradient of an initial state that the batch shares: the rows added up in order.
@@ -450,11 +471,11 @@ __global__ __launch_bounds__(64) void scan_dh0_sum_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------- host
-constexpr int MIN_CT = 64;                   // the narrowest tile: workspaces are sized for its number of tiles, rounded up
+constexpr int CT = 64;                       // channels of a tile, of either type
 
 int blocks_of(int T) { return (T + STES_SCAN_BLOCK - 1) / STES_SCAN_BLOCK; }
-// words of one kind in the workspace: tiles of 64 or 128 channels alike fit into rows of H rounded up to 128
-long words_of(int B, int T, int H) { return (long)blocks_of(T) * B * ((H + 127) / 128 * 128); }
+// words of one kind in the workspace
+long words_of(int B, int T, int H) { return (long)blocks_of(T) * B * ((H + CT - 1) / CT * CT); }
 
 // rows of `width` elements that a call writes: frames within sequences or the reverse, apart from one another
 bool apart(int64_t ld, int T, int64_t bs, int B, int64_t width) {
@@ -469,7 +490,7 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
     STES_CHECK(a->f32 == 0 || a->f32 == 1, STES_ERR_ARG, "stes_gated_scan: f32 is 0 (bf16) or 1 (fp32)");
     STES_CHECK(!a->dh0_sum || a->dh0 || !a->B, STES_ERR_ARG, "stes_gated_scan_bwd: dh0_sum needs dh0");
     if (!a->B || !a->H) return STES_OK;
-    STES_CHECK(a->H <= (1 << 24) && (long)a->B * ((a->H + MIN_CT - 1) / MIN_CT) * (blocks_of(a->T) + 1) < (1L << 31), STES_ERR_UNSUPPORTED,
+    STES_CHECK(a->H <= (1 << 24) && (long)a->B * ((a->H + CT - 1) / CT) * (blocks_of(a->T) + 1) < (1L << 31), STES_ERR_UNSUPPORTED,
                "stes_gated_scan: more tiles than a launch holds");
     if (a->T) {
         STES_CHECK(a->pre && a->ld_pre >= 2L * a->H && a->bs_pre >= 0, STES_ERR_ARG, "stes_gated_scan: pre is [B][T][2H]");
@@ -489,11 +510,9 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
     return STES_OK;
 }
 
-// rows that a lane reads or writes 16 bytes of at a time
-bool wide_rows(const void* p, int64_t ld, int64_t bs, int bytes) { return (uintptr_t)p % 16 == 0 && ld * bytes % 16 == 0 && bs * bytes % 16 == 0; }
-
 template <class G, bool BWD>
 void launch_tiles(const stes_gated_scan_args& a, hipStream_t s) {
+    static_assert(G::CT == CT, "the workspace is laid out for tiles of CT channels");
     const int tiles = (a.H + G::CT - 1) / G::CT, blocks = blocks_of(a.T);
     const long chains = (long)a.B * tiles;
     unsigned* ticket = (unsigned*)a.ws;
@@ -510,25 +529,13 @@ void launch_tiles(const stes_gated_scan_args& a, hipStream_t s) {
     }
 }
 
-template <typename T, int V, bool BWD>
-void launch_short(const stes_gated_scan_args& a, hipStream_t s) {
-    const long groups = (long)a.B * ((a.H + V - 1) / V);
-    hipLaunchKernelGGL((scan_short_kernel<T, V, BWD>), dim3((unsigned)((groups + 63) / 64)), dim3(64), 0, s, a, groups);
-}
-
-template <bool BWD>
+template <typename T, bool BWD>
 void scan_launch(const stes_gated_scan_args& a, hipStream_t s) {
-    const int bytes = a.f32 ? 4 : 2;
-    bool wide = a.H * bytes % 16 == 0 && (!a.T || wide_rows(a.pre, a.ld_pre, a.bs_pre, bytes));
-    if (BWD) wide = wide && wide_rows(a.dpre, a.ld_dpre, a.bs_dpre, bytes) && (!a.dh || wide_rows(a.dh, a.ld_dh, a.bs_dh, bytes));
-    else wide = wide && wide_rows(a.h, a.ld_h, a.bs_h, bytes);
     if (a.T <= SHORT) {
-        if (a.f32) { if (wide) launch_short<float, 4, BWD>(a, s); else launch_short<float, 1, BWD>(a, s); }
-        else { if (wide) launch_short<bf16, 8, BWD>(a, s); else launch_short<bf16, 1, BWD>(a, s); }
-        return;
-    }
-    if (a.f32) { if (wide) launch_tiles<Tile<float, 4, 16, 8>, BWD>(a, s); else launch_tiles<Tile<float, 1, 64, 32>, BWD>(a, s); }
-    else { if (wide) launch_tiles<Tile<bf16, 8, 16, 8>, BWD>(a, s); else launch_tiles<Tile<bf16, 1, 64, 32>, BWD>(a, s); }
+        const long groups = (long)a.B * ((a.H + Chunk<T>::V - 1) / Chunk<T>::V);
+        hipLaunchKernelGGL((scan_short_kernel<T, BWD>), dim3((unsigned)((groups + 63) / 64)), dim3(64), 0, s, a, groups);
+    } else if constexpr (sizeof(T) == 2) launch_tiles<Tile<T, 8, 4>, BWD>(a, s);
+    else launch_tiles<Tile<T, 16, 8>, BWD>(a, s);
 }
 
 }  // namespace
@@ -542,7 +549,8 @@ extern "C" int stes_gated_scan_fwd(const stes_gated_scan_args* a, void* stream) 
     const int rc = scan_check(a, false);
     if (rc) return rc;
     if (!a->B || !a->H) return STES_OK;
-    scan_launch<false>(*a, (hipStream_t)stream);
+    if (a->f32) scan_launch<float, false>(*a, (hipStream_t)stream);
+    else scan_launch<bf16, false>(*a, (hipStream_t)stream);
     STES_LAUNCH_CHECK();
     return STES_OK;
 }
@@ -552,7 +560,8 @@ extern "C" int stes_gated_scan_bwd(const stes_gated_scan_args* a, void* stream) 
     if (rc) return rc;
     if (!a->H) return STES_OK;
     if (a->B) {
-        scan_launch<true>(*a, (hipStream_t)stream);
+        if (a->f32) scan_launch<float, true>(*a, (hipStream_t)stream);
+        else scan_launch<bf16, true>(*a, (hipStream_t)stream);
         STES_LAUNCH_CHECK();
     }
     if (a->dh0_sum) {                                       // (zeros for an empty batch)

@@ -107,7 +107,7 @@ GatedScanArgs = _struct("GatedScanArgs", [
     ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
     ("ws", _P), ("ws_bytes", _I64),
     ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
-SCAN_BLOCK = 128            # STES_SCAN_BLOCK in include/stes.h
+SCAN_BLOCK = 256            # STES_SCAN_BLOCK in include/stes.h
 
 DistillArgs = _struct("DistillArgs", [
     ("logits", _P), ("ld", _I64), ("f32", _I32),
