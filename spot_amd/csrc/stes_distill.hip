@@ -14,16 +14,43 @@ template <> struct Vec<bf16, 8> { typedef bf16x8 type; };
 template <> struct Vec<float, 4> { typedef f32x4 type; };
 template <typename T> struct Vec<T, 1> { typedef T type __attribute__((ext_vector_type(1))); };
 
-constexpr float LOG2E = 1.4426950408889634f;
+// Everything is in base 2: the card's exp and log are.
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+
+// v of another lane of the wave: CTRL names it as DPP does; lanes that have none, or whose row is not in ROWS, get `none`
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
 
 // reductions over the G lanes of an aligned lane group
 template <int G> __device__ __forceinline__ float group_max(float v) {
+    if constexpr (G == 64) {                                 // (all lanes active; six DPP steps instead of six trips through LDS)
+        constexpr float low = -INFINITY;
+        v = fmaxf(v, dpp<ROW_SHR + 1, 0xf>(low, v));
+        v = fmaxf(v, dpp<ROW_SHR + 2, 0xf>(low, v));
+        v = fmaxf(v, dpp<ROW_SHR + 4, 0xf>(low, v));
+        v = fmaxf(v, dpp<ROW_SHR + 8, 0xf>(low, v));
+        v = fmaxf(v, dpp<ROW_BCAST15, 0xa>(low, v));
+        v = fmaxf(v, dpp<ROW_BCAST31, 0xc>(low, v));
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+    }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
 template <int G> __device__ __forceinline__ float group_sum(float v) {
+    if constexpr (G == 64) {
+        v += dpp<ROW_SHR + 1, 0xf>(0.f, v);
+        v += dpp<ROW_SHR + 2, 0xf>(0.f, v);
+        v += dpp<ROW_SHR + 4, 0xf>(0.f, v);
+        v += dpp<ROW_SHR + 8, 0xf>(0.f, v);
+        v += dpp<ROW_BCAST15, 0xa>(0.f, v);
+        v += dpp<ROW_BCAST31, 0xc>(0.f, v);
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+    }
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
@@ -67,16 +94,28 @@ __device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, long m,
     if (!entries) return e;
     float w = v > -INFINITY ? exp2_((v - mx) * ct) : 0.f;
     w *= 1.f / group_sum<G>(w);
-    // merge duplicates
-    float whole = 0.f;
-    int first = G;
-    for (int j = 0; j < p.k; ++j) {
-        const int aj = from<G>(e.at, j, lane);
-        const float pj = from<G>(w, j, lane);
-        if (aj == e.at) { whole += pj; first = first < j ? first : j; }
+    // merge duplicates, which hardly ever occur: a wave first asks whether there are any
+    float whole = w;
+    int first = l;
+    bool twice = true;
+    if constexpr (G == 64) {
+        twice = false;
+        for (int j = 0; j < p.k; ++j) {
+            const int aj = from<G>(e.at, j, lane);
+            twice = twice || (aj >= 0 && __popcll(__ballot(e.at == aj)) > 1);
+        }
+    }
+    if (twice) {
+        whole = 0.f;
+        first = G;
+        for (int j = 0; j < p.k; ++j) {
+            const int aj = from<G>(e.at, j, lane);
+            const float pj = from<G>(w, j, lane);
+            if (aj == e.at) { whole += pj; first = first < j ? first : j; }
+        }
     }
     e.p = whole;
-    if (first != l || !(whole > 0.f) || e.at >= p.V) e.at = -1;
+    if (first != l || !(whole >= 1.17549435e-38f) || e.at >= p.V) e.at = -1;       // (what is not a normal number counts as nothing)
     return e;
 }
 
@@ -86,10 +125,8 @@ __device__ __forceinline__ float row_factor(const stes_distill_args& p, float w,
     return bad ? __builtin_nanf("") : f;
 }
 
-// A lane's part of KL = sum P (log P - log q), for the class that it holds: s is the class's logit
-__device__ __forceinline__ float kl_part(const Entry& e, float s, float mx, float sum, float it) {
-    return e.at >= 0 ? e.p * (logf(e.p) - ((s - mx) * it - logf(sum))) : 0.f;
-}
+// A lane's part of KL / ln 2 = sum P (log2 P - log2 q), for a class of probability P and logit s; ls = log2(sum)
+__device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, float ct) { return P * (log2_(P) - ((s - mx) * ct - ls)); }
 
 // A workgroup's part of the loss; the only one of a launch is the loss.
 __device__ __forceinline__ void leave(const stes_distill_args& p, float* part, float sum, double factor) {
@@ -107,7 +144,7 @@ __global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_a
     constexpr int E = 8, RPB = 256 / G;
     __shared__ double red[4];
     const int lane = threadIdx.x & 63, l = threadIdx.x % G;
-    const float it = 1.f / p.temperature, ct = it * LOG2E;
+    const float ct = LOG2E / p.temperature;
     double total = 0.0;
     for (int r = 0; r < rounds; ++r) {
         const long m = ((long)blockIdx.x * rounds + r) * RPB + threadIdx.x / G;
@@ -149,11 +186,11 @@ __global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_a
         }
         if (MODE & LOSS) {
             float kl = 0.f;
-            const float ls = logf(sum);
+            const float ls = log2_(sum);
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (pv[e] > 0.f) kl += pv[e] * (logf(pv[e]) - ((x[e] - mx) * it - ls));
-            kl = group_sum<G>(kl);
+                if (pv[e] > 0.f) kl += kl_part(pv[e], x[e], mx, ls, ct);
+            kl = LN2 * group_sum<G>(kl);
             if (t.bad) kl = __builtin_nanf("");
             if (counts && l == 0) total += (double)(w * kl);
         }
@@ -214,6 +251,20 @@ template <int TEAM> struct Team {
     }
 };
 
+// f(i, row[i]) for i = i0, i0 + TEAM, ... below n, four loads in flight
+template <int TEAM, typename VT, typename F>
+__device__ __forceinline__ void walk(const VT* row, int i0, int n, F f) {
+    int i = i0;
+    for (; i + 3 * TEAM < n; i += 4 * TEAM) {
+        VT y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = row[i + u * TEAM];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f(i + u * TEAM, y[u]);
+    }
+    for (; i < n; i += TEAM) f(i, row[i]);
+}
+
 template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
 __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(const stes_distill_args p, float* __restrict__ part, double factor) {
     typedef typename Vec<TS, W>::type VS;
@@ -227,7 +278,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
     float out = 0.f;
     if (row) {
         const TS* s = (const TS*)p.logits + m * p.ld;
-        const float it = 1.f / p.temperature, ct = it * LOG2E;
+        const float ct = LOG2E / p.temperature;
         const float w = p.weight ? p.weight[m] : 1.f;
         const int V = p.V;
         // [0, head) single, then nv vectors, then [tail, V) single
@@ -253,8 +304,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
             if (STREAM) {
                 // running maximum and sum: a thread's sum is scaled when its maximum rises
                 float acc = 0.f;
-                for (int i = i0; i < nv; i += TEAM) {
-                    const VS y = sv[i];
+                auto take = [&](const VS& y) {
                     float top = (float)y[0];
 #pragma unroll
                     for (int e = 1; e < W; ++e) top = fmaxf(top, (float)y[e]);
@@ -268,7 +318,8 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
                         for (int e = 0; e < W; ++e) add += (float)y[e] == -INFINITY ? 0.f : __builtin_nanf("");
                     }
                     acc += add;
-                }
+                };
+                walk<TEAM>(sv, i0, nv, [&](int, const VS& y) { take(y); });
                 if (x1 > -INFINITY || x1 != x1) acc += exp2_((x1 - mx) * ct);
                 const float own = mx;
                 mx = Tm::max_(mx, red);
@@ -295,7 +346,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
         }
         if (!(MODE & STATS_IN) && p.stats && i0 == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = sum; }
         if ((MODE & LOSS) && threadIdx.x % TEAM < 64) {
-            float kl = group_sum<64>(kl_part(t, st, mx, sum, it));
+            float kl = LN2 * group_sum<64>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), ct) : 0.f);
             if (t.bad) kl = __builtin_nanf("");
             out = counts ? w * kl : 0.f;
         }
@@ -319,7 +370,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
                     }
                     dv[i] = o;
                 };
-                if (STREAM) for (int i = i0; i < nv; i += TEAM) put(i, sv[i]);
+                if (STREAM) walk<TEAM>(sv, i0, nv, put);
                 else {
 #pragma unroll
                     for (int i = 0; i < N; ++i)
@@ -412,6 +463,7 @@ int launch_rows(const stes_distill_args& a, hipStream_t s) {
             if (vecs <= 256 * 8) return launch_row<TS, TG, W, 256, 8, false, MODE>(a, s);
             if (vecs <= 512 * 8) return launch_row<TS, TG, W, 512, 8, false, MODE>(a, s);
             if (vecs <= 1024 * 8) return launch_row<TS, TG, W, 1024, 8, false, MODE>(a, s);
+            if (vecs <= 1024 * 16 && (MODE & GRAD)) return launch_row<TS, TG, W, 1024, 16, false, MODE>(a, s);
             return launch_row<TS, TG, W, 1024, 1, true, MODE>(a, s);
         }
     }
