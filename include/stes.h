@@ -470,7 +470,10 @@ int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h
  * Backward: l_s = dh_s + a_{s+1} l_{s+1} (+ dh_last at s = len-1), d gate = l_s (cand_s - x_{s-1}) z a, d cand = l_s z,
  * dh0 [B][H] = a_0 l_0 (dh_last where len = 0).  dh or dh_last may be NULL (zeros); dh0 may be NULL; dh0_sum [H] (optional, needs dh0):
  * the sum of dh0 over the batch in a fixed order, for an initial state that the batch shares.
- * T = 0 is a call (h_last = h0).  ws: stes_gated_scan_ws_bytes(B, T, H) bytes, contents irrelevant; calls that may overlap need one each.
+ * T = 0 is a call (h_last = h0).  ws: stes_gated_scan_ws_bytes(B, T, H) bytes, aligned to 16; calls that may overlap need one each.
+ * Its contents are irrelevant unless ws_zero != 0 says that they are zero, which spares the launch that clears them (they are
+ * not zero afterwards).  scrub (forward, optional): scrub_bytes of memory, multiples of 16, that the call leaves zero on the way: the
+ * workspace of the backward pass to come.
  * Results do not depend on scheduling beyond the association of the time axis: see stes_scan.hip. */
 #define STES_SCAN_BLOCK 256
 typedef struct {
@@ -479,7 +482,8 @@ typedef struct {
     void* h; int64_t ld_h, bs_h; float* h_last; int64_t bs_hl; float* states;
     const void* dh; int64_t ld_dh, bs_dh; const float* dh_last; int64_t bs_dhl;
     void* dpre; int64_t ld_dpre, bs_dpre; float* dh0; float* dh0_sum;
-    void* ws; int64_t ws_bytes;
+    void* ws; int64_t ws_bytes; int32_t ws_zero;
+    void* scrub; int64_t scrub_bytes;
     int32_t B, T, H, f32, reverse;
 } stes_gated_scan_args;
 int64_t stes_gated_scan_ws_bytes(int B, int T, int H);

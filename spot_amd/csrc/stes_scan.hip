@@ -195,6 +195,10 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
         tB[wave][lane] = fb;
     }
     __syncthreads();
+    if (JOIN && wave != 0 && p.scrub) {                      // (while the first wave looks back)
+        u32x4* w = (u32x4*)p.scrub;
+        for (long i = (long)blockIdx.x * (G::NT - 64) + tid - 64; i < p.scrub_bytes / 16; i += (long)gridDim.x * (G::NT - 64)) w[i] = (u32x4){0u, 0u, 0u, 0u};
+    }
     if (wave == 0) {
         const int ch = at.c0 + lane;
         float x = 0.f, fa[NW], fb[NW], mA = 1.f, mB = 0.f;
@@ -503,6 +507,8 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
         const int64_t need = stes_gated_scan_ws_bytes(a->B, a->T, a->H);
         STES_CHECK(need == 0 || (a->ws && a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0), STES_ERR_ARG, "stes_gated_scan: workspace too small or not aligned to 16 bytes");
     }
+    STES_CHECK(!a->scrub || (!bwd && a->T > STES_SCAN_BLOCK && a->scrub_bytes >= 0 && a->scrub_bytes % 16 == 0 && (uintptr_t)a->scrub % 16 == 0), STES_ERR_ARG,
+               "stes_gated_scan_fwd: scrub goes with a forward pass of more than STES_SCAN_BLOCK steps, in multiples of 16 bytes");
     STES_CHECK(!a->h0 || a->bs_h0 == 0 || a->bs_h0 >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h0 overlap");
     STES_CHECK(!a->h_last || a->bs_hl >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h_last overlap");
     STES_CHECK(!(a->h_last && a->h_last == a->h0) || a->bs_h0 == a->bs_hl, STES_ERR_ARG, "stes_gated_scan: a state in place keeps its row stride");
@@ -520,7 +526,7 @@ void launch_tiles(const stes_gated_scan_args& a, hipStream_t s) {
     const Link link{words, words + words_of(a.B, a.T, a.H)};
     if (blocks > 1) {
         const long n = stes_gated_scan_ws_bytes(a.B, a.T, a.H) / 16;
-        hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (u32x4*)a.ws, n);
+        if (!a.ws_zero) hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, (u32x4*)a.ws, n);
         if (BWD) hipLaunchKernelGGL((scan_bwd_kernel<G, true>), dim3((unsigned)(chains * blocks)), dim3(G::NT), 0, s, a, tiles, chains, blocks, ticket, link);
         else hipLaunchKernelGGL((scan_fwd_kernel<G, true>), dim3((unsigned)(chains * blocks)), dim3(G::NT), 0, s, a, tiles, chains, blocks, ticket, link);
     } else {

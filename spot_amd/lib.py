@@ -105,7 +105,7 @@ GatedScanArgs = _struct("GatedScanArgs", [
     ("h", _P), ("ld_h", _I64), ("bs_h", _I64), ("h_last", _P), ("bs_hl", _I64), ("states", _P),
     ("dh", _P), ("ld_dh", _I64), ("bs_dh", _I64), ("dh_last", _P), ("bs_dhl", _I64),
     ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
-    ("ws", _P), ("ws_bytes", _I64),
+    ("ws", _P), ("ws_bytes", _I64), ("ws_zero", _I32), ("scrub", _P), ("scrub_bytes", _I64),
     ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
 SCAN_BLOCK = 256            # STES_SCAN_BLOCK in include/stes.h
 

@@ -55,7 +55,7 @@ def _apart(t, width):
     return outer[1] == 1 or outer[0] >= inner[0] * (inner[1] - 1) + width
 
 
-def _forward(pre, h0, lengths, reverse, out, state_out, keep_states):
+def _forward(pre, h0, lengths, reverse, out, state_out, keep_states, scrub=None):
     B, T, W = pre.shape
     H, dev = W // 2, pre.device
     h = pre.new_empty(B, T, H) if out is None else out
@@ -74,7 +74,8 @@ def _forward(pre, h0, lengths, reverse, out, state_out, keep_states):
             None if lengths is None else lengths.data_ptr(),
             h.data_ptr(), ld_h, bs_h, last.data_ptr(), bs_hl, None if states is None else states.data_ptr(),
             None, 0, 0, None, 0, None, 0, 0, None, None,
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), 0,
+            None if scrub is None else scrub.data_ptr(), 0 if scrub is None else scrub.numel(),
             B, T, H, _ELEMENT[pre.dtype], reverse)
         lib.call("stes_gated_scan_fwd", C.byref(a))
     return h, last, states
@@ -85,7 +86,11 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, pre, h0, lengths, reverse):
         ctx.set_materialize_grads(False)
-        h, last, states = _forward(pre, h0, lengths, reverse, None, None, True)
+        # the forward kernel clears the backward pass's workspace on the way, which spares that a launch
+        B, T, W = pre.shape
+        ws = _workspace(B, T, W // 2, pre.device)
+        h, last, states = _forward(pre, h0, lengths, reverse, None, None, True, ws)
+        ctx.clean = [] if ws is None else [ws]
         ctx.save_for_backward(pre, lengths, states)
         ctx.reverse = reverse
         ctx.h0_dim = 0 if h0 is None or not ctx.needs_input_grad[1] else h0.dim()
@@ -96,17 +101,19 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         pre, lengths, states = ctx.saved_tensors
         with lib.on_device(pre.device):
-            return _backward(pre, lengths, states, ctx.reverse, ctx.h0_dim, dh, dlast)
+            # (clean once; a captured backward pass may be replayed without its forward and clears a workspace of its own)
+            ws = ctx.clean.pop() if ctx.clean and not torch.cuda.is_current_stream_capturing() else None
+            return _backward(pre, lengths, states, ctx.reverse, ctx.h0_dim, dh, dlast, ws)
 
 
-def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast):
+def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast, clean_ws):
     B, T, W = pre.shape
     H, dev = W // 2, pre.device
     dpre = torch.empty(B, T, W, dtype=pre.dtype, device=dev)
     dh0 = torch.empty(B, H, dtype=torch.float32, device=dev) if h0_dim else None
     total = torch.empty(H, dtype=torch.float32, device=dev) if h0_dim == 1 else None
     if H and (B or total is not None):
-        ws = _workspace(B, T, H, dev)
+        ws, ws_zero = (clean_ws, 1) if clean_ws is not None else (_workspace(B, T, H, dev), 0)
         ld, bs = _strides(pre, T, W)
         ld_dh = bs_dh = 0
         if dh is not None:
@@ -119,7 +126,7 @@ def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast):
             pre.data_ptr(), ld, bs, None, 0, None if lengths is None else lengths.data_ptr(), None, 0, 0, None, 0, states.data_ptr(),
             None if dh is None else dh.data_ptr(), ld_dh, bs_dh, None if dlast is None else dlast.data_ptr(), H,
             dpre.data_ptr(), W, T * W, None if dh0 is None else dh0.data_ptr(), None if total is None else total.data_ptr(),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), ws_zero, None, 0,
             B, T, H, _ELEMENT[pre.dtype], reverse)
         lib.call("stes_gated_scan_bwd", C.byref(a))
     return dpre, (total if h0_dim == 1 else dh0), None, None

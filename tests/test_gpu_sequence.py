@@ -188,6 +188,31 @@ def test_gated_scan_gradient_from_final_state_alone():
         _check(g[1], ref["dh0"], ref["dh0_err"], "dh0")
 
 
+@pytest.mark.parametrize("T", [30, 700])
+def test_gated_scan_backward_twice_and_captured_apart_from_its_forward(T):
+    """The second backward pass through a graph, and a captured one that is replayed without its forward, give the bits of the first."""
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, dh, dlast = _scan_inputs(2, T, 96, BF, False, "rows", seed=T)
+    d, dl = dh.cuda(), dlast.cuda()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        p, s = pre.cuda().requires_grad_(), start.cuda().requires_grad_()
+        y = gated_scan(p, s)
+        first = torch.autograd.grad(y, (p, s), (d, dl), retain_graph=True)
+        again = torch.autograd.grad(y, (p, s), (d, dl), retain_graph=True)
+        z = gated_scan(p, s)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            out = torch.autograd.grad(z, (p, s), (d, dl), retain_graph=True)
+        for _ in range(3):
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(first, out))
+            out[0].zero_()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
 def test_gated_scan_gradient_against_differences():
     from spot_amd.recurrence import gated_scan
     pre, start, lengths, dh, dlast = _scan_inputs(3, 150, 24, F32, True, "shared", seed=3)

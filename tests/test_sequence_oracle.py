@@ -111,12 +111,14 @@ def _scan_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(B=-1), dict(T=-1), dict(H=-1), dict(f32=2), dict(pre=None), dict(h=None), dict(ld_pre=15), dict(ld_h=7), dict(bs_h=31), dict(bs_h=0),
-                                dict(bs_hl=7), dict(h0=512, bs_h0=3), dict(h0=256, bs_h0=0), dict(h0=256, bs_h0=9), dict(B=70000000, H=1 << 20)])
+                                dict(bs_hl=7), dict(h0=512, bs_h0=3), dict(h0=256, bs_h0=0), dict(h0=256, bs_h0=9), dict(scrub=256, scrub_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, ws=264),
+                                dict(T=1000, bs_pre=16000, bs_h=8000, ws_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, scrub=256, scrub_bytes=8),
+                                dict(B=70000000, H=1 << 20)])
 def test_scan_forward_refuses(kw):
     _refused("stes_gated_scan_fwd", _scan_args(**kw))
 
 
-@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256)])
+@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256), dict(scrub=256)])
 def test_scan_backward_refuses(kw):
     _refused("stes_gated_scan_bwd", _scan_args(**kw))
 
