@@ -54,11 +54,14 @@ class DataParallelTrainer:
             self.eng.weights_dirty = True
         self.reducer = BucketReducer(dist, self.eng.flat_grad) if dist is not None else None
 
-    def step(self, frame, label, xy):
+    def step(self, frame, label, xy, distill=None):
+        """distill: as in E2EModel.train_step; without a "denom" of its own the frames of ALL ranks count (the same number on each)."""
         den = None
+        if distill is not None and self.dist is not None and distill.get("denom") is None:
+            distill = {**distill, "denom": float(label.numel() * self.dist.get_world_size())}
         if self.dist is not None:
             den = loss_denominators(label, self.fg_weight)
             self.dist.all_reduce(den, op=self.dist.ReduceOp.SUM)
-        out = self.model.train_step(frame, label, xy, self.lr, fg_weight=self.fg_weight, ext_denoms=den,
+        out = self.model.train_step(frame, label, xy, self.lr, fg_weight=self.fg_weight, ext_denoms=den, distill=distill,
                                     on_ready=self.reducer, after_backward=(lambda eng: self.reducer.wait()) if self.reducer else None)
         return out

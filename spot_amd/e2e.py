@@ -18,6 +18,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import lib
+from .distill import topk_distill_loss
 from .engine import BF, Engine
 from .model.common import MLP, BaseRGBModel, step
 from .model.min_gru import MinRNNPredictor
@@ -133,7 +134,7 @@ class E2EModel(BaseRGBModel):
                 self._engine.weights_dirty = True
             return r
 
-        def forward(self, x):
+        def forward(self, x, stream=None):
             batch_size, true_clip_len, channels, height, width = x.shape
             if self.time_backward:
                 x = x.flip(1)
@@ -156,7 +157,7 @@ class E2EModel(BaseRGBModel):
                     loc = None
             else:
                 # a padded clip is un-padded before the heads, as the reference does (train_e2e_spatial.py:440-442)
-                logits, loc, feat = eng.forward(x, train=self.training, head_T=true_clip_len, pad_T=pad_T)
+                logits, loc, feat = eng.forward(x, train=self.training, head_T=true_clip_len, pad_T=pad_T, stream=stream)
                 logits, feat = logits.clone(), feat.float()
                 loc = loc.clone() if loc is not None else None
             if self.time_backward:
@@ -187,8 +188,11 @@ class E2EModel(BaseRGBModel):
         self._temporal_arch = temporal_arch
 
     # ------------------------------------------------------------------ reference API
-    def epoch(self, loader, optimizer=None, scaler=None, lr_scheduler=None, acc_grad_iter=1, fg_weight=5):
-        """reference train_e2e_spatial.py:507-625 (tqdm bar dropped; losses identical)."""
+    def epoch(self, loader, optimizer=None, scaler=None, lr_scheduler=None, acc_grad_iter=1, fg_weight=5, distill_weight=0.0,
+              distill_temperature=1.0):
+        """reference train_e2e_spatial.py:507-625 (tqdm bar dropped; losses identical).  With distill_weight > 0 a training epoch adds
+        distill_weight times the distillation loss from a teacher's top logits (spot_amd.distill) of batches that hold
+        `teacher_idx` and `teacher_val` [B, T, k]; the returned dict then has it as "distill"."""
         if optimizer is None:
             self._model.eval()
         else:
@@ -198,6 +202,9 @@ class E2EModel(BaseRGBModel):
         if fg_weight != 1:
             ce_kwargs["weight"] = torch.FloatTensor([1] + [fg_weight] * (self._num_classes - 1)).to(self.device)
         sums = {"sum": 0.0, "cls": 0.0, "loc": 0.0, "contrast": 0.0}
+        distilling = optimizer is not None and distill_weight > 0
+        if distilling:
+            sums["distill"] = 0.0
         with torch.no_grad() if optimizer is None else nullcontext():
             for batch_idx, batch in enumerate(loader):
                 frame = batch["frame"].to(self.device)
@@ -217,6 +224,11 @@ class E2EModel(BaseRGBModel):
                     xy_loss = F.l1_loss(loc.reshape(-1, 2).sigmoid(), target_xy, reduction="none").sum(dim=-1)
                     loss_loc = (xy_loss * event_mask).sum() / (event_mask.sum() + 1e-6)
                 loss = loss_cls + loss_loc
+                if distilling and "teacher_idx" in batch:
+                    loss_distill = topk_distill_loss(preds["im_feat"], batch["teacher_idx"].to(self.device), batch["teacher_val"].to(self.device),
+                                                     distill_temperature)
+                    loss = loss + distill_weight * loss_distill
+                    sums["distill"] += loss_distill.detach().item()
                 if optimizer is not None:
                     step(optimizer, scaler, loss / acc_grad_iter, lr_scheduler=lr_scheduler,
                          backward_only=(batch_idx + 1) % acc_grad_iter != 0)
@@ -262,11 +274,44 @@ class E2EModel(BaseRGBModel):
             loc = pred_dict["loc_feat"].reshape(seq.shape[0], -1, 2).sigmoid() if self._model._predict_location else None
         return scores, loc
 
+    # ------------------------------------------------------------------ frame streams (minGRU heads)
+    def new_stream(self, n=1):
+        """The head's state at the start of n frame streams, for predict_stream: fp32 [n, hidden] per layer."""
+        if self._temporal_arch != "mingru" or self._model.time_backward:
+            raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
+        return [h.detach().to(self.device, torch.float32).expand(n, -1).clone() for h in self._model._pred_fine.h0]
+
+    def predict_stream(self, seq, state):
+        """predict_async() for the next frames of n streams (`state` of new_stream(n), updated in place): seq [n * W, T, C, H, W] holds W
+        clips of every stream, one after the other in time.  Clips are independent in the backbone (T = clip_len where it
+        shifts channels in time, a shorter T is zero-padded there; T = 1 is a frame at a time for the plain backbone), while the
+        minGRU head runs over a stream's W * T frames as one sequence that starts where the last call's ended: a video's scores
+        do not depend on how it is cut into calls."""
+        if self._temporal_arch != "mingru" or self._model.time_backward:
+            raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
+        n, hidden = (state[0].shape if len(state) else (0, 0))
+        layers = self._model._pred_fine
+        if (len(state) != layers.n_layers or hidden != layers.hidden_size or n < 1 or seq.shape[0] < 1 or seq.shape[0] % n
+                or any(s.shape != state[0].shape for s in state)):
+            raise lib.StesError(f"predict_stream: {seq.shape[0]} clips and a state of {len(state)} layers {[tuple(s.shape) for s in state]} "
+                                "do not fit: clips are a multiple of the streams of new_stream()")
+        if seq.device != torch.device(self.device) and str(seq.device) != str(self.device):
+            seq = seq.to(self.device, non_blocking=True)
+        if self._model.training:
+            self._model.eval()
+        with torch.no_grad():
+            pred_dict = self._model(seq, stream=state)
+            scores = torch.softmax(pred_dict["im_feat"], axis=2)
+            loc = pred_dict["loc_feat"].reshape(seq.shape[0], -1, 2).sigmoid() if self._model._predict_location else None
+        return scores, loc
+
     # ------------------------------------------------------------------ fused training step (HIP loss + backward + AdamW)
     def train_step(self, frame, label, xy, lr, fg_weight=5.0, grad_scale=1.0, ext_denoms=None, optimizer_step=True,
-                   after_backward=None, grad_mul=1.0, on_ready=None):
+                   after_backward=None, grad_mul=1.0, on_ready=None, distill=None):
         """One optimisation step entirely on the device.  frame [B,T,C,H,W] f32 (normalised) or uint8 (decoded), label [B,T] int64, xy [B,T,2] f32.
-        Returns the device tensor {sum, cls, loc, sum of class weights, number of event frames} (no host sync)."""
+        distill: {"idx", "val" [B,T,k], "temperature" 1.0, "weight" 1.0, "frame_weight" [B,T] or None, "denom" or None (all frames)}:
+        `weight` times the distillation loss from a teacher's top logits (spot_amd.distill) joins the loss.
+        Returns the device tensor {sum, cls, loc, sum of class weights, number of event frames, distillation loss, ...} (no host sync)."""
         m = self._model
         m.train()
         eng = m.engine
@@ -275,7 +320,7 @@ class E2EModel(BaseRGBModel):
         eng.forward(frame, train=True)
         eng.attach_grads(zero=True)
         out = eng.loss_backward(label.reshape(-1), xy.reshape(-1, 2) if xy is not None else None, self._num_classes,
-                                fg_weight=fg_weight, grad_scale=grad_scale, ext_denoms=ext_denoms, on_ready=on_ready)
+                                fg_weight=fg_weight, grad_scale=grad_scale, ext_denoms=ext_denoms, on_ready=on_ready, distill=distill)
         if after_backward is not None:
             after_backward(eng)
         if optimizer_step:

@@ -20,9 +20,11 @@ import torch
 import torch.nn as nn
 
 from . import lib
+from .distill import topk_distill_grad
 from .model.modules import GRUPrediction
 from .model.min_gru import MinRNNPredictor
 from .model.shift import GatedShift, TemporalShift
+from .recurrence import gated_scan
 from .regnet import ConvBnAct
 
 BF = torch.bfloat16
@@ -765,11 +767,13 @@ class Engine:
         N, T = N_bb, self.T
 
     # ------------------------------------------------------------------ forward
-    def forward(self, x, train, head_T=None, pad_T=None):
+    def forward(self, x, train, head_T=None, pad_T=None, stream=None):
         """x: [B, T, C, H, W] on the device (T == clip_len when a temporal shift is present): fp32 as the reference loader
         hands it over (already normalised), or uint8 decoded frames, which the stem normalises itself with `input_mean` /
         `input_std` (reference dataset/frame.py:16-17,29,124).  A uint8 batch of shorter clips is padded to pad_T frames
         inside the stem kernel (zero frames after normalisation, reference train_e2e_spatial.py:427-430).
+        stream (minGRU heads, evaluation): one fp32 state [n, hidden] per layer.  The B clips are n streams' next B / n clips each, in
+        order; the head runs over every stream as one sequence that starts from its state and leaves its last state there.
         Returns (logits [B,Th,classes] f32, loc [B,Th,2] f32 | None, feat [B,Th,F] bf16), Th = head_T or T."""
         B, Tx, Cin, H, W = x.shape
         if Cin != self.in_chans:
@@ -830,9 +834,9 @@ class Engine:
             lib.call("stes_clip_gate_fwd", p(self.feat), p(self.ca_gate), p(self.feat_in), B, T, Fd)
         if self.Th != T:
             self.feat_h.view(B, self.Th, self.feat_dim).copy_(self.feat_in.view(B, T, self.feat_dim)[:, :self.Th])
-        return self._heads_forward(train)
+        return self._heads_forward(train, stream)
 
-    def _heads_forward(self, train):
+    def _heads_forward(self, train, stream=None):
         N, B, T, Fd = self.Nh, self.B, self.Th, self.feat_dim
         feat = self.feat_h
         p = lib.ptr
@@ -875,7 +879,11 @@ class Engine:
             for i, lin in enumerate(self.min_lin):
                 Hh = lin.N // 2
                 lib.gemm(xin, lin.w_bf, self.min_pre[i], N, 2 * Hh, in_dim, bias=lin.b)
-                lib.call("stes_mingru_scan_fwd", p(self.min_pre[i]), p(self.impl._pred_fine.h0[i]), p(self.min_h[i]), B, T, Hh)
+                if stream is None:
+                    lib.call("stes_mingru_scan_fwd", p(self.min_pre[i]), p(self.impl._pred_fine.h0[i]), p(self.min_h[i]), B, T, Hh)
+                else:
+                    n = stream[i].shape[0]
+                    gated_scan(self.min_pre[i].view(n, N // n, 2 * Hh), stream[i], out=self.min_h[i].view(n, N // n, Hh), state_out=stream[i])
                 xin, in_dim = self.min_h[i], Hh
             self.fc_in = xin
             lib.gemm(xin, self.fc.w_bf, self.logits, N, self.fc.N, in_dim, bias=self.fc.b)
@@ -1019,7 +1027,9 @@ class Engine:
             on_ready(*self.buckets["rest"])
 
     # ------------------------------------------------------------------ fused training step
-    def loss_backward(self, label, xy, num_classes, fg_weight=5.0, grad_scale=1.0, ext_denoms=None, on_ready=None):
+    def loss_backward(self, label, xy, num_classes, fg_weight=5.0, grad_scale=1.0, ext_denoms=None, on_ready=None, distill=None):
+        """distill: {"idx", "val" [N, k], "temperature", "weight", "frame_weight" [N] | None, "denom" | None}: `weight` times the
+        distillation loss from a teacher's top logits joins the loss (loss_buf[0]); loss_buf[5] is the distillation loss itself."""
         N = self.N
         p = lib.ptr
         ncp = _rup(num_classes, 8)
@@ -1027,6 +1037,14 @@ class Engine:
         dloc = self.scratch("dloc", N * 8).view(N, 8) if self.loc is not None else None
         lib.call("stes_loss", p(self.logits), num_classes, p(self.loc_out) if self.loc is not None else None, 2, p(label), p(xy), N,
                  num_classes, float(fg_weight), float(grad_scale), p(ext_denoms), p(self.loss_buf), p(dl), p(dloc))
+        if distill is not None:
+            # (the class gradient is rounded to bf16 between the two losses, as it is in front of every product that reads it)
+            w, fw = float(distill.get("weight", 1.0)), distill.get("frame_weight")
+            kd, _ = topk_distill_grad(self.logits.view(N, num_classes), distill["idx"].reshape(N, -1), distill["val"].reshape(N, -1),
+                                      distill.get("temperature", 1.0), None if fw is None else fw.reshape(N), distill.get("denom"),
+                                      grad_scale=w * grad_scale, out=dl[:, :num_classes], accumulate=True)
+            self.loss_buf[5:6].copy_(kd.view(1))
+            self.loss_buf[0:1].add_(kd.view(1), alpha=w)
         self.backward(dl, dloc, on_ready=on_ready)
         return self.loss_buf
 

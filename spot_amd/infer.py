@@ -49,14 +49,20 @@ def pad_last_window(clip, clip_len, mean=IMAGENET_MEAN, std=IMAGENET_STD):
 
 
 def run_inference(model, frames, classes, clip_len, batch_size=16, postprocess=True, rank=0, world=1, video="video",
-                  gather=None):
+                  gather=None, carry_state=False):
     """model: E2EModel; frames [n_frames, C, H, W]: float tensor (normalised; host or device), uint8 tensor (decoded), or a
-    numpy array / memory map of either.  Returns the reference's
+    numpy array / memory map of either.  carry_state (minGRU heads): the head runs over the video as one sequence, its state handed
+    from window to window, instead of starting again in every window.  Returns the reference's
     [{'video', 'events'}] list (after score filter 0.15 and NMS 3 when postprocess)."""
     n_frames = frames.shape[0]
     acc = ScoreAccumulator(n_frames, len(classes) + 1)
     full_batch_seen = False
     pipelined = hasattr(model, "predict_async")
+    state = None
+    if carry_state:
+        if world != 1:
+            raise NotImplementedError("carry_state: the windows of a video follow one another (one process)")
+        state = model.new_stream()
     pending = None
 
     def take(starts, scores, loc):
@@ -84,7 +90,7 @@ def run_inference(model, frames, classes, clip_len, batch_size=16, postprocess=T
         if pipelined:
             # this batch is enqueued before the previous one's results are read back: the host's launches for it overlap the
             # GPU's work on the previous batch instead of following the read-back's wait
-            cur = model.predict_async(batch)
+            cur = model.predict_async(batch) if state is None else model.predict_stream(batch, state)
             if pending is not None:
                 take(*pending)
             pending = (starts, cur[0], cur[1])
@@ -123,6 +129,7 @@ def main(argv=None):
     p.add_argument("--classes", type=str, default="block dig net pass receive score serve set spike")
     p.add_argument("--device", type=str, default="cuda")
     p.add_argument("--no_postprocess", action="store_true")
+    p.add_argument("--carry_state", action="store_true", help="minGRU heads: the head's state is handed from window to window")
     args = p.parse_args(argv)
     from .e2e import E2EModel
     classes = args.classes.split()
@@ -141,7 +148,7 @@ def main(argv=None):
     model.load(torch.load(os.path.abspath(args.checkpoint_path), map_location="cpu", weights_only=True))
     frames = np.load(args.frames, mmap_mode="r")
     pred_events, _ = run_inference(model, frames, classes, args.clip_len, args.batch_size, postprocess=not args.no_postprocess,
-                                   video=os.path.basename(args.frames))
+                                   video=os.path.basename(args.frames), carry_state=args.carry_state)
     os.makedirs(args.save_dir, exist_ok=True)
     with open(os.path.join(args.save_dir, "predictions.json"), "w") as fp:
         json.dump(pred_events, fp)

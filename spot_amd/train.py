@@ -8,6 +8,8 @@ the GPU under `--augment` (spot_amd/augment.py).  `frame_dir` holds shards `trai
     frame uint8 [n, clip_len, 3, H, W]   decoded RGB frames (the stem normalises them on the GPU)
     label int64 [n, clip_len]            0 = background
     xy    float32 [n, clip_len, 2]       event location in [0, 1]
+    teacher_idx int [n, clip_len, k], teacher_val float [n, clip_len, k]   optional: a teacher's best classes per frame and their
+                                         logits (its `im_feat`.topk(k)), what --distill_weight trains against
 
 or is the literal string `synthetic[:n_clips]`, or -- the reference's own layout -- holds JPEG frames `<video>/000123.jpg` with the
 label files `data/<dataset>/{train,val}.json` (spot_amd/dataset.py: the reference's frame reader and clip sampler; frames of
@@ -77,6 +79,9 @@ def get_args(argv=None):
     p.add_argument("--augment", action="store_true",
                    help="the reference loader's random augmentation (dataset/frame.py:78-140) on the GPU; shards may then hold "
                         "frames of any size (validation clips are resized to crop_dim)")
+    p.add_argument("--distill_weight", type=float, default=0.0,
+                   help="weight of the distillation loss from a teacher's top logits (shards with teacher_idx and teacher_val)")
+    p.add_argument("--distill_temperature", type=float, default=1.0)
     return p.parse_args(argv)
 
 
@@ -100,6 +105,7 @@ class ClipShards:
         for f in self.files:
             with np.load(f) as z:
                 frame, label, xy = z["frame"], z["label"], z["xy"]
+                teacher = {k: z[k] for k in ("teacher_idx", "teacher_val") if k in z.files}
             for i in range(0, label.shape[0] - self.batch_size + 1, self.batch_size):
                 b += 1
                 if b > todo:
@@ -107,8 +113,12 @@ class ClipShards:
                 if (b - 1) % self.world != self.rank:
                     continue
                 s = slice(i, i + self.batch_size)
-                yield {"frame": torch.from_numpy(frame[s]), "label": torch.from_numpy(label[s]).long(),
+                out = {"frame": torch.from_numpy(frame[s]), "label": torch.from_numpy(label[s]).long(),
                        "xy": torch.from_numpy(xy[s]).float()}
+                if len(teacher) == 2:
+                    out["teacher_idx"] = torch.from_numpy(teacher["teacher_idx"][s].astype(np.int32))
+                    out["teacher_val"] = torch.from_numpy(teacher["teacher_val"][s].astype(np.float32))
+                yield out
 
 
 class SyntheticClips:
@@ -383,20 +393,30 @@ def import_adamw_state(model, optimizer):
             eng.adam_v[o:o + n].copy_(st["exp_avg_sq"].reshape(-1))
 
 
-def fused_epoch(trainer, loader, lr_scheduler, device, with_xy=True):
-    """One training epoch through the fused step; the loss is read back once, at the end.  Returns the reference's dict."""
+def fused_epoch(trainer, loader, lr_scheduler, device, with_xy=True, distill_weight=0.0, distill_temperature=1.0):
+    """One training epoch through the fused step; the loss is read back once, at the end.  Returns the reference's dict (and
+    "distill" where a teacher's logits are trained against)."""
     import warnings
-    total = torch.zeros(3, device=device)
+    total, total_distill = torch.zeros(3, device=device), torch.zeros(1, device=device)
     for batch in loader:
         trainer.lr = lr_scheduler.get_last_lr()[0]
+        distill = None
+        if distill_weight > 0 and "teacher_idx" in batch:
+            distill = {"idx": batch["teacher_idx"].to(device), "val": batch["teacher_val"].to(device), "temperature": distill_temperature,
+                       "weight": distill_weight}
         out = trainer.step(batch["frame"].to(device, non_blocking=True), batch["label"].to(device),
-                           batch["xy"].to(device) if with_xy else None)
+                           batch["xy"].to(device) if with_xy else None, distill=distill)
         total += out[:3]
+        if distill is not None:
+            total_distill += out[5:6]
         with warnings.catch_warnings():           # the torch optimizer only carries the schedule here; it never steps
             warnings.simplefilter("ignore", UserWarning)
             lr_scheduler.step()
     s, c, l = (total / max(1, len(loader))).tolist()
-    return {"sum": s, "cls": c, "loc": l, "contrast": 0.0}
+    losses = {"sum": s, "cls": c, "loc": l, "contrast": 0.0}
+    if distill_weight > 0:
+        losses["distill"] = total_distill.item() / max(1, len(loader))
+    return losses
 
 
 def scaler_state(scaler):
@@ -429,6 +449,9 @@ def main(args):
     if getattr(args, "mixup", False) and (fused or args.predict_location):
         raise NotImplementedError("--mixup gives soft labels: the fused step and the location loss take class indices "
                                   "(the reference's location loss fails on them too, train_e2e_spatial.py:582-591)")
+    distilling = {"distill_weight": getattr(args, "distill_weight", 0.0), "distill_temperature": getattr(args, "distill_temperature", 1.0)}
+    if distilling["distill_weight"] > 0 and getattr(args, "mixup", False):
+        raise NotImplementedError("--distill_weight: a teacher's logits belong to unmixed clips (not with --mixup)")
     classes = load_classes(args)
     model = E2EModel(len(classes) + 1, args.feature_arch, args.temporal_arch, clip_len=args.clip_len, modality=args.modality,
                      device=args.device, predict_location=args.predict_location, pred_loc_arch=args.pred_loc_arch,
@@ -452,9 +475,9 @@ def main(args):
         os.makedirs(args.save_dir, exist_ok=True)
     for epoch in range(epoch, num_epochs):
         if fused:
-            train_loss = fused_epoch(trainer, train_loader, lr_scheduler, args.device, args.predict_location)
+            train_loss = fused_epoch(trainer, train_loader, lr_scheduler, args.device, args.predict_location, **distilling)
         else:
-            train_loss = model.epoch(train_loader, optimizer, scaler, lr_scheduler=lr_scheduler, acc_grad_iter=args.acc_grad_iter)
+            train_loss = model.epoch(train_loader, optimizer, scaler, lr_scheduler=lr_scheduler, acc_grad_iter=args.acc_grad_iter, **distilling)
         if dist is not None:
             # BatchNorm running statistics are rank-local during training; validation, evaluation and the checkpoint all
             # use rank 0's, so that the criterion describes the weights that are saved

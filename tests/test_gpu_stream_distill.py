@@ -1,0 +1,205 @@
+"""The gated scan and the distillation loss inside the model: frame streams of the minGRU head (predict_stream, run_inference with
+carry_state) and training against a teacher's top logits (train_step, epoch, the training driver)."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def rel(a, b):
+    a, b = torch.as_tensor(a).double().flatten().cpu(), torch.as_tensor(b).double().flatten().cpu()
+    return float((a - b).norm() / (b.norm() + 1e-12))
+
+
+def _model(arch="rny008", tarch="mingru", clip_len=4, seed=3):
+    from oracle import stes_oracle as O
+    from spot_amd.e2e import E2EModel
+    om = O.Impl(7, arch, tarch, clip_len=clip_len, predict_location=True)
+    O.randomize_(om, seed=seed)
+    m = E2EModel(7, arch, tarch, clip_len=clip_len, modality="rgb", device="cuda", predict_location=True, verbose=False)
+    m._model.load_state_dict(om.state_dict(), strict=True)
+    with torch.no_grad():                    # an initial state that is not zero, gates that remember for tens of frames
+        for i, h in enumerate(m._model._pred_fine.h0):
+            h.copy_(torch.randn(h.shape, generator=torch.Generator().manual_seed(i)) * 0.5)
+        for layer in m._model._pred_fine.rnn_layers:
+            layer.linear_z.bias.sub_(3.0)
+    return m
+
+
+def _frames(n, seed=0, dim=64):
+    return torch.randint(0, 256, (n, 3, dim, dim), generator=torch.Generator().manual_seed(seed), dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("arch,cuts", [("rny008", (24,)), ("rny008", (1,) * 24), ("rny008", (5, 1, 11, 7)), ("rny008_tsm", (4,) * 6), ("rny008_gsm", (8, 16))])
+def test_stream_scores_do_not_depend_on_the_cut(arch, cuts):
+    """A video in one call, in calls of any length, a frame at a time; with a backbone that shifts channels in time, any number of
+    its clips a call.  (The backbone runs on batches of other shapes then: its features differ by bf16 roundings.)"""
+    T = 4
+    m = _model(arch, clip_len=T)
+    x = _frames(24).cuda()
+    state = m.new_stream()
+    want, wloc = m.predict_stream(x.view(6, T, 3, 64, 64), state)
+    want, wloc, wstate = want.view(24, 7), wloc.view(24, 2), [s.clone() for s in state]
+    state, got, loc, at = m.new_stream(), [], [], 0
+    for n in cuts:
+        part = x[at:at + n]
+        part = part[None] if arch == "rny008" else part.view(n // T, T, 3, 64, 64)
+        s, l = m.predict_stream(part, state)
+        got.append(s.reshape(n, 7))
+        loc.append(l.reshape(n, 2))
+        at += n
+    assert rel(torch.cat(got), want) < 1e-2 and rel(torch.cat(loc), wloc) < 1e-2
+    for a, b in zip(state, wstate):
+        assert rel(a, b) < 1e-2
+    again = m.predict_stream(x.view(6, T, 3, 64, 64), m.new_stream())[0].view(24, 7)
+    assert torch.equal(again, want)
+    # the state matters: windows that start again give other scores
+    alone = m.predict_async(x.view(6, T, 3, 64, 64))[0].view(24, 7)
+    assert torch.allclose(alone[:4], want[:4], atol=2e-2) and rel(alone[8:], want[8:]) > 3e-2
+
+
+def test_stream_of_one_clip_equals_the_clip():
+    """A stream that starts anew is the same head as predict(): same kernels around it, the same recurrence from the same h0."""
+    m = _model("rny008", clip_len=16)
+    x = _frames(32, 1).cuda().view(2, 16, 3, 64, 64)
+    a, la = m.predict_async(x)
+    b, lb = m.predict_stream(x, m.new_stream(2))
+    # states differ by their association in fp32, which moves a stored bf16 state by one step now and then
+    assert float((a - b).abs().max()) < 2e-2 and torch.equal(la, lb)
+
+
+def test_streams_side_by_side_equal_streams_alone():
+    m = _model("rny008_tsm", clip_len=4)
+    x = torch.stack([_frames(16, s) for s in (1, 2, 3)]).cuda().view(3, 4, 4, 3, 64, 64)
+    state = m.new_stream(3)
+    got = [m.predict_stream(x[:, lo:hi].reshape(-1, 4, 3, 64, 64), state)[0].view(3, hi - lo, 4, 7) for lo, hi in ((0, 1), (1, 4))]
+    got = torch.cat(got, 1)
+    for i in range(3):
+        one = m.new_stream()
+        w = m.predict_stream(x[i], one)[0]
+        assert rel(got[i], w) < 1e-2
+        for a, b in zip(state, one):
+            assert rel(a[i], b[0]) < 1e-2
+
+
+def test_stream_with_a_padded_last_clip():
+    m = _model("rny008_tsm", clip_len=8)
+    x = _frames(11, 5).cuda()
+    state = m.new_stream()
+    a = m.predict_stream(x[None, :8], state)[0]
+    b = m.predict_stream(x[None, 8:], state)[0]
+    assert a.shape == (1, 8, 7) and b.shape == (1, 3, 7) and bool(torch.isfinite(b).all())
+
+
+def test_inference_carries_the_state():
+    from spot_amd.infer import run_inference
+    m = _model("rny008", clip_len=4)
+    x = _frames(22, 7)
+    classes = ["c%d" % i for i in range(1, 7)]
+    _, scores = run_inference(m, x, classes, 4, batch_size=2, postprocess=False, carry_state=True)
+    state = m.new_stream()
+    want = m.predict_stream(x.cuda()[None], state)[0][0]
+    assert rel(scores[:22], want) < 1e-2
+    _, fresh = run_inference(m, x, classes, 4, batch_size=2, postprocess=False)
+    assert rel(fresh[8:22], want[8:]) > 3e-2
+    with pytest.raises(NotImplementedError):
+        run_inference(m, x, classes, 4, world=2, carry_state=True)
+
+
+def test_stream_refusals():
+    from spot_amd import lib
+    from spot_amd.e2e import E2EModel
+    for kw in (dict(temporal_arch="gru"), dict(temporal_arch=""), dict(temporal_arch="mingru", time_backward=True)):
+        m = E2EModel(7, "rny008", clip_len=4, modality="rgb", device="cuda", verbose=False, **kw)
+        with pytest.raises(NotImplementedError):
+            m.new_stream()
+        with pytest.raises(NotImplementedError):
+            m.predict_stream(_frames(4)[None], [])
+    m = _model()
+    x = _frames(12).view(3, 4, 3, 64, 64)
+    for state in ([], m.new_stream()[:2], m.new_stream(2), [s[:0] for s in m.new_stream()], [s[:, :5] for s in m.new_stream()]):
+        with pytest.raises(lib.StesError):
+            m.predict_stream(x, state)
+    with pytest.raises(lib.StesError):
+        m.predict_stream(x[:0], m.new_stream())
+
+
+# ------------------------------------------------------------------------------------------------------------ training
+def _batch(B=2, T=4, k=3, seed=2):
+    g = torch.Generator().manual_seed(seed)
+    val, idx = (torch.randn(B, T, 7, generator=g) * 3).topk(k, 2)
+    idx[0, 1] = -1
+    label = torch.randint(0, 7, (B, T), generator=g)
+    label[0, 0], label[1, 1] = 0, 3
+    return (torch.randn(B, T, 3, 64, 64, generator=g).cuda(), label.cuda(), torch.rand(B, T, 2, generator=g).cuda(), idx.cuda(), val.cuda())
+
+
+@pytest.fixture
+def fixed_order():
+    """BatchNorm statistics of the training forward in a fixed order, so that separate runs of it have the same bits."""
+    from spot_amd import lib
+    lib.set_deterministic(True)
+    try:
+        yield
+    finally:
+        lib.set_deterministic(False)
+
+
+def test_train_step_with_a_teacher_matches_the_autograd_loop(fixed_order):
+    """train_step(distill=...): the loss and the head's gradients against cross entropy + L1 + topk_distill_loss through autograd."""
+    import torch.nn.functional as F
+    from spot_amd.distill import topk_distill_loss
+    frame, label, xy, idx, val = _batch()
+    m = _model("rny008_tsm")
+    out = m.train_step(frame, label, xy, 0.0, optimizer_step=False,
+                       distill={"idx": idx, "val": val, "temperature": 2.0, "weight": 0.7}).clone()
+    eng = m._model.engine
+    got = {n: eng.grad(p).clone() for n, p in m._model.named_parameters() if n.startswith("_pred_fine") and p.requires_grad}
+    m2 = _model("rny008_tsm")
+    m2._model.train()
+    d = m2._model(frame)
+    cls = F.cross_entropy(d["im_feat"].reshape(-1, 7), label.reshape(-1), weight=torch.tensor([1.0] + [5.0] * 6).cuda())
+    mask = (label != 0).float().reshape(-1)
+    loc = (F.l1_loss(d["loc_feat"].reshape(-1, 2).sigmoid(), xy.reshape(-1, 2), reduction="none").sum(1) * mask).sum() / (mask.sum() + 1e-6)
+    kd = topk_distill_loss(d["im_feat"], idx, val, 2.0)
+    (cls + loc + 0.7 * kd).backward()
+    np.testing.assert_allclose(out[:3].cpu().numpy(), [float(cls + loc + 0.7 * kd), float(cls), float(loc)], rtol=1e-4)
+    np.testing.assert_allclose(float(out[5]), float(kd), rtol=1e-4)
+    for n, p in m2._model.named_parameters():
+        if n in got:
+            assert rel(got[n], p.grad) < 2e-2, n          # (class gradients rounded to bf16 once there, twice here)
+    # without a teacher the step is what it was, with weight 0 as well
+    m3, m4 = _model("rny008_tsm"), _model("rny008_tsm")
+    a = m3.train_step(frame, label, xy, 0.0, optimizer_step=False)[:3].clone()
+    b = m4.train_step(frame, label, xy, 0.0, optimizer_step=False, distill={"idx": idx, "val": val, "weight": 0.0})[:3].clone()
+    np.testing.assert_allclose(a.cpu().numpy(), out[:3].cpu().numpy() - np.array([0.7 * float(kd), 0, 0]), rtol=1e-4)
+    assert torch.equal(a, b)
+
+
+def test_epoch_with_a_teacher():
+    frame, label, xy, idx, val = _batch()
+    m = _model("rny008_tsm")
+    opt, scaler = m.get_optimizer({"lr": 1e-4})
+    batch = {"frame": frame, "label": label, "xy": xy, "teacher_idx": idx.int(), "teacher_val": val}
+    r = m.epoch([batch], opt, scaler, distill_weight=0.5, distill_temperature=2.0)
+    np.testing.assert_allclose(r["sum"], r["cls"] + r["loc"] + 0.5 * r["distill"], rtol=1e-5)
+    assert r["distill"] > 0
+    assert "distill" not in m.epoch([batch], opt, scaler) and "distill" not in m.epoch([batch], distill_weight=0.5)
+
+
+def test_train_driver_with_a_teacher(tmp_path):
+    """Shards that hold a teacher's top logits, through the reference-style loop and through the fused step."""
+    from spot_amd import train as TR
+    g = np.random.default_rng(0)
+    for split, n in (("train", 4), ("val", 2)):
+        np.savez(tmp_path / f"{split}_0.npz", frame=g.integers(0, 256, (n, 4, 3, 64, 64), dtype=np.uint8), label=g.integers(0, 7, (n, 4)),
+                 xy=g.random((n, 4, 2), dtype=np.float32), teacher_idx=np.argsort(g.random((n, 4, 7)), 2)[..., :3].astype(np.int16),
+                 teacher_val=g.normal(size=(n, 4, 3)).astype(np.float16))
+    base = ["ds", str(tmp_path), "-m", "rny008_tsm", "-t", "mingru", "--clip_len", "4", "--crop_dim", "64", "--batch_size", "2",
+            "--warm_up_epochs", "1", "--num_epochs", "2", "--predict_location", "--num_classes", "6", "--criterion", "loss"]
+    for extra in (["--distill_weight", "0.5", "--distill_temperature", "2"], ["--distill_weight", "0.5", "--fused"], []):
+        _, losses, _ = TR.main(TR.get_args(base + ["-s", str(tmp_path / ("run%d" % len(extra)))] + extra))
+        assert len(losses) == 2 and all(np.isfinite(l["train"]) and np.isfinite(l["val"]) for l in losses)
+    with pytest.raises(NotImplementedError):
+        TR.main(TR.get_args([a for a in base if a != "--predict_location"] + ["-s", str(tmp_path / "x"), "--distill_weight", "1", "--mixup"]))
