@@ -471,9 +471,9 @@ int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h
  * dh0 [B][H] = a_0 l_0 (dh_last where len = 0).  dh or dh_last may be NULL (zeros); dh0 may be NULL; dh0_sum [H] (optional, needs dh0):
  * the sum of dh0 over the batch in a fixed order, for an initial state that the batch shares.
  * T = 0 is a call (h_last = h0).  ws: stes_gated_scan_ws_bytes(B, T, H) bytes, aligned to 16; calls that may overlap need one each.
- * Its contents are irrelevant unless ws_zero != 0 says that they are zero, which spares the launch that clears them (they are
- * not zero afterwards).  scrub (forward, optional): scrub_bytes of memory, multiples of 16, that the call leaves zero on the way: the
- * workspace of the backward pass to come.
+ * Its contents are irrelevant unless ws_zero != 0 says that they are zero, which spares the launch that clears them (they are not
+ * zero afterwards).  scrub (optional, with T > STES_SCAN_BLOCK): scrub_bytes of other memory, a multiple of 16, that the call leaves zero on
+ * the way: what a caller that alternates between two workspaces on one stream used in the call before.
  * Results do not depend on scheduling beyond the association of the time axis: see stes_scan.hip. */
 #define STES_SCAN_BLOCK 256
 typedef struct {

@@ -24,6 +24,18 @@ template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, f
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
 constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
+constexpr int QUAD_XOR1 = 0xB1, QUAD_XOR2 = 0x4E, ROW_HALF_MIRROR = 0x141, ROW_MIRROR = 0x140;
+
+// f over the G < 64 lanes of a lane group, the result in all of them.  (Once the lanes of a quad hold the same, mirroring eight lanes
+// swaps its quads; likewise on.)
+template <int G, typename F> __device__ __forceinline__ float group_fold(float v, F f) {
+    v = f(v, dpp<QUAD_XOR1, 0xf>(v, v));
+    v = f(v, dpp<QUAD_XOR2, 0xf>(v, v));
+    if (G >= 8) v = f(v, dpp<ROW_HALF_MIRROR, 0xf>(v, v));
+    if (G >= 16) v = f(v, dpp<ROW_MIRROR, 0xf>(v, v));
+    if (G >= 32) v = f(v, __shfl_xor(v, 16, 64));
+    return v;
+}
 
 // reductions over the G lanes of an aligned lane group
 template <int G> __device__ __forceinline__ float group_max(float v) {
@@ -37,9 +49,7 @@ template <int G> __device__ __forceinline__ float group_max(float v) {
         v = fmaxf(v, dpp<ROW_BCAST31, 0xc>(low, v));
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
     }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    return group_fold<G>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 template <int G> __device__ __forceinline__ float group_sum(float v) {
     if constexpr (G == 64) {
@@ -51,9 +61,7 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
         v += dpp<ROW_BCAST31, 0xc>(0.f, v);
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
     }
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    return group_fold<G>(v, [](float a, float b) { return a + b; });
 }
 template <int G> __device__ __forceinline__ bool group_any(bool b, int lane) {
     const uint64_t m = __ballot(b);
@@ -73,27 +81,34 @@ template <int G> __device__ __forceinline__ int from(int v, int j, int lane) {
 }
 template <int G> __device__ __forceinline__ float from(float v, int j, int lane) { return __int_as_float(from<G>(__float_as_int(v), j, lane)); }
 
-// The teacher's distribution of row m, an entry per lane of a group of G >= k lanes (`l`: the lane's place in it).  A class that is
-// listed more than once has its whole probability at its first place; the later places hold none.  With entries == false only
-// what the row is worth (some, bad) is found out.
-template <int G>
-__device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, long m, bool row, int l, int lane, float ct, bool entries) {
-    Entry e;
-    e.at = -1;
-    float v = -INFINITY;
+struct Listed { int at; float v; };      // one place of a row's list as it was loaded: index (< 0: unused, V: beyond the classes) and value
+
+__device__ __forceinline__ Listed load_listed(const stes_distill_args& p, long m, bool row, int l) {
+    Listed e{-1, -INFINITY};
     if (row && l < p.k) {
         const long o = m * p.ld_idx + l, i = p.idx_i64 ? ((const int64_t*)p.idx)[o] : (long)((const int32_t*)p.idx)[o];
         const long ov = m * p.ld_val + l;
         const float u = p.val_f32 ? ((const float*)p.val)[ov] : (float)((const bf16*)p.val)[ov];
-        if (i >= 0) { e.at = i >= p.V ? p.V : (int)i; v = u; }
+        if (i >= 0) { e.at = i >= p.V ? p.V : (int)i; e.v = u; }
     }
+    return e;
+}
+
+// The teacher's distribution of a row, an entry per lane of a group of G >= k lanes (`l`: the lane's place in it).  A class that is
+// listed more than once has its whole probability at its first place; the later places hold none.  With entries == false only
+// what the row is worth (some, bad) is found out.
+template <int G>
+__device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, const Listed& in, int l, int lane, float ct, bool entries) {
+    Entry e;
+    e.at = in.at;
+    const float v = in.v;
     const float mx = group_max<G>(v);                       // (fmaxf passes over NaN: those are caught below)
     e.bad = group_any<G>(e.at >= p.V || v != v || v == INFINITY, lane);
     e.some = mx > -INFINITY || e.bad;
     e.p = 0.f;
     if (!entries) return e;
     float w = v > -INFINITY ? exp2_((v - mx) * ct) : 0.f;
-    w *= 1.f / group_sum<G>(w);
+    w *= __builtin_amdgcn_rcpf(group_sum<G>(w));
     // merge duplicates, which hardly ever occur: a wave first asks whether there are any
     float whole = w;
     int first = l;
@@ -119,9 +134,9 @@ __device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, long m,
     return e;
 }
 
-// the factor of a row's gradient
-__device__ __forceinline__ float row_factor(const stes_distill_args& p, float w, bool bad) {
-    const float f = (float)((double)p.temperature / p.denom) * p.grad_scale * w * (p.upstream ? p.upstream[0] : 1.f);
+// the factor of a row's gradient; `scale` = grad_scale temperature / denom
+__device__ __forceinline__ float row_factor(const stes_distill_args& p, float scale, float w, bool bad) {
+    const float f = scale * w * (p.upstream ? p.upstream[0] : 1.f);
     return bad ? __builtin_nanf("") : f;
 }
 
@@ -129,32 +144,52 @@ __device__ __forceinline__ float row_factor(const stes_distill_args& p, float w,
 __device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, float ct) { return P * (log2_(P) - ((s - mx) * ct - ls)); }
 
 // A workgroup's part of the loss; the only one of a launch is the loss.
-__device__ __forceinline__ void leave(const stes_distill_args& p, float* part, float sum, double factor) {
+__device__ __forceinline__ void leave(const stes_distill_args& p, float* part, double sum, double factor) {
     if (gridDim.x == 1) *p.loss = (float)(sum * factor);
-    else part[blockIdx.x] = sum;
+    else part[blockIdx.x] = (float)sum;
 }
 
 enum { LOSS = 1, GRAD = 2, STATS_IN = 4 };           // what a launch does
 
 // ---------------------------------------------------------------- short rows
-// V <= 8 G and k <= G: a group of G lanes per row, at most 8 classes a lane, neighbouring lanes neighbouring classes.  256 / G rows a
-// workgroup and round; a workgroup's rows follow from its index alone, and so does the order of its sum.
-template <typename TS, typename TG, int G, int MODE>
-__global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_args p, int rounds, float* __restrict__ part, double factor) {
-    constexpr int E = 8, RPB = 256 / G;
-    __shared__ double red[4];
-    const int lane = threadIdx.x & 63, l = threadIdx.x % G;
-    const float ct = LOG2E / p.temperature;
-    double total = 0.0;
-    for (int r = 0; r < rounds; ++r) {
-        const long m = ((long)blockIdx.x * rounds + r) * RPB + threadIdx.x / G;
+// V <= 8 G and k <= G: a group of G lanes per row, at most 8 classes a lane, neighbouring lanes neighbouring classes.  BLOCK / G rows a
+// workgroup and round, the next round's rows loaded ahead; a workgroup's rows follow from its index alone, and so does the order
+// of its sum.
+template <typename TS, int G> struct ShortRow {
+    static constexpr int E = 8;
+    TS x[E];
+    Listed listed;
+    float w;
+    __device__ __forceinline__ void load(const stes_distill_args& p, long m, int l) {
         const bool row = m < p.M;
         const TS* s = (const TS*)p.logits + m * p.ld;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = row && e * G + l < p.V ? s[e * G + l] : (TS)0.f;
+        w = row ? (p.weight ? p.weight[m] : 1.f) : 0.f;
+        listed = load_listed(p, m, row, l);
+    }
+};
+
+template <typename TS, typename TG, int G, int BLOCK, int MODE>
+__global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill_args p, int rounds, float* __restrict__ part, double factor, float scale) {
+    constexpr int E = 8, RPB = BLOCK / G;
+    __shared__ double red[BLOCK / 64];
+    const int lane = threadIdx.x & 63, l = threadIdx.x % G;
+    const float ct = LOG2E / p.temperature;
+    const long first = (long)blockIdx.x * rounds * RPB + threadIdx.x / G;
+    double total = 0.0;
+    ShortRow<TS, G> next;
+    next.load(p, first, l);
+    for (int r = 0; r < rounds; ++r) {
+        const long m = first + r * RPB;
+        const bool row = m < p.M;
+        const ShortRow<TS, G> in = next;
+        if (r + 1 < rounds) next.load(p, m + RPB, l);
         float x[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = row && e * G + l < p.V ? (float)s[e * G + l] : -INFINITY;
-        const float w = row ? (p.weight ? p.weight[m] : 1.f) : 0.f;
-        const Entry t = teacher_row<G>(p, m, row, l, lane, ct, true);
+        for (int e = 0; e < E; ++e) x[e] = row && e * G + l < p.V ? (float)in.x[e] : -INFINITY;
+        const float w = in.w;
+        const Entry t = teacher_row<G>(p, in.listed, l, lane, ct, true);
         const bool counts = t.some && w != 0.f;
         float mx, sum;
         if (MODE & STATS_IN) { mx = row ? p.stats[2 * m] : 0.f; sum = row ? p.stats[2 * m + 1] : 1.f; }
@@ -195,7 +230,7 @@ __global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_a
             if (counts && l == 0) total += (double)(w * kl);
         }
         if ((MODE & GRAD) && row) {
-            const float f = row_factor(p, w, t.bad), inv = 1.f / sum;
+            const float f = row_factor(p, scale, w, t.bad), inv = __builtin_amdgcn_rcpf(sum);
             TG* d = (TG*)p.dlogits + m * p.ld_d;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -213,7 +248,11 @@ __global__ __launch_bounds__(256) void distill_short_kernel(const stes_distill_a
         for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
         if (lane == 0) red[threadIdx.x >> 6] = total;
         __syncthreads();
-        if (threadIdx.x == 0) leave(p, part, (float)(red[0] + red[1] + red[2] + red[3]), factor);
+        if (threadIdx.x == 0) {
+            total = 0.0;
+            for (int w = 0; w < BLOCK / 64; ++w) total += red[w];
+            leave(p, part, total, factor);
+        }
     }
 }
 
@@ -266,7 +305,7 @@ __device__ __forceinline__ void walk(const VT* row, int i0, int n, F f) {
 }
 
 template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(const stes_distill_args p, float* __restrict__ part, double factor) {
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(const stes_distill_args p, float* __restrict__ part, double factor, float scale) {
     typedef typename Vec<TS, W>::type VS;
     typedef typename Vec<TG, W>::type VG;
     typedef Team<TEAM> Tm;
@@ -294,7 +333,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
             for (int i = 0; i < N; ++i)
                 if (i * TEAM + i0 < nv) x[i] = sv[i * TEAM + i0];
         }
-        const Entry t = teacher_row<64>(p, m, true, lane, lane, ct, threadIdx.x % TEAM < 64);
+        const Entry t = teacher_row<64>(p, load_listed(p, m, true, lane), lane, lane, ct, threadIdx.x % TEAM < 64);
         const float st = t.at >= 0 ? (float)s[t.at] : 0.f;
         const bool counts = t.some && w != 0.f;
         float mx = 0.f, sum = 1.f;
@@ -355,7 +394,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
             if (!counts) {
                 if (!p.accumulate) for (int v = i0; v < V; v += TEAM) d[v] = (TG)0.f;
             } else {
-                const float f = row_factor(p, w, t.bad), fq = f / sum;
+                const float f = row_factor(p, scale, w, t.bad), fq = f * __builtin_amdgcn_rcpf(sum);
                 const bool mine = threadIdx.x % TEAM < 64 && t.at >= 0;
                 const float old = mine && p.accumulate ? (float)d[t.at] : 0.f;
                 if (p.accumulate) Tm::sync();                // (the listed classes are read before anyone adds to them)
@@ -430,13 +469,20 @@ int distill_check(const stes_distill_args* a, bool bwd) {
 }
 
 double loss_factor(const stes_distill_args& a) { return (double)a.temperature * a.temperature / a.denom; }
+float grad_factor(const stes_distill_args& a) { return (float)((double)a.grad_scale * a.temperature / a.denom); }
 
 template <typename TS, typename TG, int G, int MODE>
 int launch_short(const stes_distill_args& a, hipStream_t s) {
+    // A loss of a few rounds of one large workgroup is done in one launch.  1,024 frames of 7 classes: 12 us on the GPU and 16 us a call
+    // from Python; many workgroups and the launch that adds up what they leave: 5 + 4 us and 19 us a call.
+    if ((MODE & LOSS) && a.M <= 4 * (1024 / G)) {
+        hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, 1024, MODE>), dim3(1), dim3(1024), 0, s, a, (a.M + 1024 / G - 1) / (1024 / G), a.ws, loss_factor(a), grad_factor(a));
+        return 1;
+    }
     constexpr int RPB = 256 / G;
     const long teams = ((long)a.M + RPB - 1) / RPB;
     const int rounds = (int)((teams + 2047) / 2048), blocks = (int)((teams + rounds - 1) / rounds);
-    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a));
+    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, 256, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a), grad_factor(a));
     return blocks;
 }
 
@@ -444,7 +490,7 @@ template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MOD
 int launch_row(const stes_distill_args& a, hipStream_t s) {
     constexpr int RPB = TEAM == 64 ? 4 : 1;
     const int blocks = (int)(((long)a.M + RPB - 1) / RPB);
-    hipLaunchKernelGGL((distill_row_kernel<TS, TG, W, TEAM, N, STREAM, MODE>), dim3(blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, s, a, a.ws, loss_factor(a));
+    hipLaunchKernelGGL((distill_row_kernel<TS, TG, W, TEAM, N, STREAM, MODE>), dim3(blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, s, a, a.ws, loss_factor(a), grad_factor(a));
     return blocks;
 }
 

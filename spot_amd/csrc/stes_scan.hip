@@ -137,6 +137,14 @@ __device__ __forceinline__ Place place(const stes_gated_scan_args& p, int tiles,
     return r;
 }
 
+// A workgroup's share of the memory that the launch leaves zero, written by all but its first wave.
+template <class G>
+__device__ __forceinline__ void scrub(const stes_gated_scan_args& p) {
+    u32x4* w = (u32x4*)p.scrub;
+    constexpr int N = G::NT - 64;
+    for (long i = (long)blockIdx.x * N + threadIdx.x - 64; i < p.scrub_bytes / 16; i += (long)gridDim.x * N) w[i] = (u32x4){0u, 0u, 0u, 0u};
+}
+
 template <class G, bool JOIN>
 __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_args p, int tiles, long chains, int blocks, unsigned* ticket, Link link) {
     typedef typename G::T T;
@@ -195,10 +203,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
         tB[wave][lane] = fb;
     }
     __syncthreads();
-    if (JOIN && wave != 0 && p.scrub) {                      // (while the first wave looks back)
-        u32x4* w = (u32x4*)p.scrub;
-        for (long i = (long)blockIdx.x * (G::NT - 64) + tid - 64; i < p.scrub_bytes / 16; i += (long)gridDim.x * (G::NT - 64)) w[i] = (u32x4){0u, 0u, 0u, 0u};
-    }
+    if (JOIN && wave != 0 && p.scrub) scrub<G>(p);           // (while the first wave looks back)
     if (wave == 0) {
         const int ch = at.c0 + lane;
         float x = 0.f, fa[NW], fb[NW], mA = 1.f, mB = 0.f;
@@ -311,6 +316,7 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
         tR[wave][lane] = rr;
     }
     __syncthreads();
+    if (JOIN && wave != 0 && p.scrub) scrub<G>(p);
     if (wave == 0) {
         const int ch = at.c0 + lane;
         float fa[NW], fb[NW], fr[NW], mA = 1.f, mR = 0.f, x = 0.f, k = 0.f;
@@ -507,8 +513,8 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
         const int64_t need = stes_gated_scan_ws_bytes(a->B, a->T, a->H);
         STES_CHECK(need == 0 || (a->ws && a->ws_bytes >= need && (uintptr_t)a->ws % 16 == 0), STES_ERR_ARG, "stes_gated_scan: workspace too small or not aligned to 16 bytes");
     }
-    STES_CHECK(!a->scrub || (!bwd && a->T > STES_SCAN_BLOCK && a->scrub_bytes >= 0 && a->scrub_bytes % 16 == 0 && (uintptr_t)a->scrub % 16 == 0), STES_ERR_ARG,
-               "stes_gated_scan_fwd: scrub goes with a forward pass of more than STES_SCAN_BLOCK steps, in multiples of 16 bytes");
+    STES_CHECK(!a->scrub || (a->T > STES_SCAN_BLOCK && a->scrub_bytes >= 0 && a->scrub_bytes % 16 == 0 && (uintptr_t)a->scrub % 16 == 0), STES_ERR_ARG,
+               "stes_gated_scan: scrub goes with more than STES_SCAN_BLOCK steps, in multiples of 16 bytes");
     STES_CHECK(!a->h0 || a->bs_h0 == 0 || a->bs_h0 >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h0 overlap");
     STES_CHECK(!a->h_last || a->bs_hl >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h_last overlap");
     STES_CHECK(!(a->h_last && a->h_last == a->h0) || a->bs_h0 == a->bs_hl, STES_ERR_ARG, "stes_gated_scan: a state in place keeps its row stride");

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import threading
 
 import torch
 
@@ -26,10 +27,48 @@ def _ws_bytes(B, T, H):
     return lib.lib().stes_gated_scan_ws_bytes(B, T, H)
 
 
-def _workspace(B, T, H, dev):
-    """A workspace of this call's own (None where none is needed): calls on two streams and two graphs never share one."""
-    n = _ws_bytes(B, T, H)
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+class _Workspaces:
+    """The two workspaces that the calls on one stream take in turn: a call finds its own zero and leaves the one of the call before
+    zero, so none needs a launch that clears.  A call's launch happens under the lock: what is clean follows the stream's order."""
+
+    def __init__(self):
+        self.lock, self.pair, self.turn, self.dirty = threading.Lock(), None, 0, [0, 0]
+
+
+_KEPT_BYTES = 16 << 20              # larger workspaces are not kept: clearing them is a small part of such calls (2 % of the data)
+_kept = {}                          # (device, stream) -> _Workspaces
+
+
+def _call(entry, a, dev):
+    """One call of the library with the workspace that it needs.  A captured call gets one of its own, cleared in the graph: a
+    graph may be replayed on any stream, next to others."""
+    n = _ws_bytes(a.B, a.T, a.H)
+    if not n:
+        lib.call(entry, C.byref(a))
+        return
+    a.ws_bytes = n
+    if n > _KEPT_BYTES or torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.ws = ws.data_ptr()
+        lib.call(entry, C.byref(a))
+        return
+    key = (dev.index, lib.stream())
+    k = _kept.get(key)
+    if k is None:
+        k = _kept.setdefault(key, _Workspaces())
+    with k.lock:
+        if k.pair is None or k.pair[0].numel() < n:
+            k.pair, k.turn, k.dirty = [torch.zeros(n, dtype=torch.uint8, device=dev) for _ in range(2)], 0, [0, 0]
+        i, j = k.turn, 1 - k.turn
+        a.ws, a.ws_zero = k.pair[i].data_ptr(), 1
+        if k.dirty[j]:
+            a.scrub, a.scrub_bytes = k.pair[j].data_ptr(), k.dirty[j]
+        try:
+            lib.call(entry, C.byref(a))
+        except Exception:
+            k.pair = None
+            raise
+        k.dirty[i], k.dirty[j], k.turn = n, 0, j
 
 
 def _row_stride(t, B, H, name):
@@ -55,7 +94,7 @@ def _apart(t, width):
     return outer[1] == 1 or outer[0] >= inner[0] * (inner[1] - 1) + width
 
 
-def _forward(pre, h0, lengths, reverse, out, state_out, keep_states, scrub=None):
+def _forward(pre, h0, lengths, reverse, out, state_out, keep_states):
     B, T, W = pre.shape
     H, dev = W // 2, pre.device
     h = pre.new_empty(B, T, H) if out is None else out
@@ -65,7 +104,6 @@ def _forward(pre, h0, lengths, reverse, out, state_out, keep_states, scrub=None)
         last, bs_hl = state_out, _row_stride(state_out, B, H, "state_out")
     states = torch.empty(B, -(-T // lib.SCAN_BLOCK), H, dtype=torch.float32, device=dev) if keep_states else None
     if B and H:
-        ws = _workspace(B, T, H, dev)
         ld, bs = _strides(pre, T, W)
         ld_h, bs_h = _strides(h, T, H)
         a = lib.GatedScanArgs(
@@ -74,10 +112,8 @@ def _forward(pre, h0, lengths, reverse, out, state_out, keep_states, scrub=None)
             None if lengths is None else lengths.data_ptr(),
             h.data_ptr(), ld_h, bs_h, last.data_ptr(), bs_hl, None if states is None else states.data_ptr(),
             None, 0, 0, None, 0, None, 0, 0, None, None,
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), 0,
-            None if scrub is None else scrub.data_ptr(), 0 if scrub is None else scrub.numel(),
-            B, T, H, _ELEMENT[pre.dtype], reverse)
-        lib.call("stes_gated_scan_fwd", C.byref(a))
+            None, 0, 0, None, 0, B, T, H, _ELEMENT[pre.dtype], reverse)
+        _call("stes_gated_scan_fwd", a, dev)
     return h, last, states
 
 
@@ -86,11 +122,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, pre, h0, lengths, reverse):
         ctx.set_materialize_grads(False)
-        # the forward kernel clears the backward pass's workspace on the way, which spares that a launch
-        B, T, W = pre.shape
-        ws = _workspace(B, T, W // 2, pre.device)
-        h, last, states = _forward(pre, h0, lengths, reverse, None, None, True, ws)
-        ctx.clean = [] if ws is None else [ws]
+        h, last, states = _forward(pre, h0, lengths, reverse, None, None, True)
         ctx.save_for_backward(pre, lengths, states)
         ctx.reverse = reverse
         ctx.h0_dim = 0 if h0 is None or not ctx.needs_input_grad[1] else h0.dim()
@@ -101,19 +133,16 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         pre, lengths, states = ctx.saved_tensors
         with lib.on_device(pre.device):
-            # (clean once; a captured backward pass may be replayed without its forward and clears a workspace of its own)
-            ws = ctx.clean.pop() if ctx.clean and not torch.cuda.is_current_stream_capturing() else None
-            return _backward(pre, lengths, states, ctx.reverse, ctx.h0_dim, dh, dlast, ws)
+            return _backward(pre, lengths, states, ctx.reverse, ctx.h0_dim, dh, dlast)
 
 
-def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast, clean_ws):
+def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast):
     B, T, W = pre.shape
     H, dev = W // 2, pre.device
     dpre = torch.empty(B, T, W, dtype=pre.dtype, device=dev)
     dh0 = torch.empty(B, H, dtype=torch.float32, device=dev) if h0_dim else None
     total = torch.empty(H, dtype=torch.float32, device=dev) if h0_dim == 1 else None
     if H and (B or total is not None):
-        ws, ws_zero = (clean_ws, 1) if clean_ws is not None else (_workspace(B, T, H, dev), 0)
         ld, bs = _strides(pre, T, W)
         ld_dh = bs_dh = 0
         if dh is not None:
@@ -126,9 +155,8 @@ def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast, clean_ws):
             pre.data_ptr(), ld, bs, None, 0, None if lengths is None else lengths.data_ptr(), None, 0, 0, None, 0, states.data_ptr(),
             None if dh is None else dh.data_ptr(), ld_dh, bs_dh, None if dlast is None else dlast.data_ptr(), H,
             dpre.data_ptr(), W, T * W, None if dh0 is None else dh0.data_ptr(), None if total is None else total.data_ptr(),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), ws_zero, None, 0,
-            B, T, H, _ELEMENT[pre.dtype], reverse)
-        lib.call("stes_gated_scan_bwd", C.byref(a))
+            None, 0, 0, None, 0, B, T, H, _ELEMENT[pre.dtype], reverse)
+        _call("stes_gated_scan_bwd", a, dev)
     return dpre, (total if h0_dim == 1 else dh0), None, None
 
 

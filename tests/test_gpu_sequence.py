@@ -346,6 +346,49 @@ def test_gated_scan_on_another_stream_and_two_calls_at_once(T):
         assert torch.equal(h, want) and torch.equal(last, wl)
 
 
+def test_gated_scan_calls_of_changing_sizes_share_a_stream():
+    """Calls of growing and shrinking sizes one after the other on one stream (they take two kept workspaces in turn), forward and
+    backward, from two threads at once, next to a captured call that is replayed among them."""
+    import threading
+    from spot_amd.recurrence import gated_scan
+    sizes = [(1, 300, 64), (3, 1000, 200), (1, 257, 8), (2, 5000, 64), (1, 300, 64), (4, 600, 130), (1, 20000, 8), (3, 1000, 200)]
+    inputs = [_scan_inputs(B, T, H, BF, False, "rows", seed=T + H)[:2] for B, T, H in sizes]
+    inputs = [(a.cuda().requires_grad_(), b.cuda()) for a, b in inputs]
+
+    def one(i):
+        p, s = inputs[i]
+        h, last = gated_scan(p, s)
+        return h.detach(), last.detach(), torch.autograd.grad(h, p, torch.ones_like(h))[0]
+    want = []
+    for i in range(len(sizes)):
+        p, s = inputs[i]
+        with torch.cuda.stream(torch.cuda.Stream()):                    # a stream of its own: workspaces of its own
+            want.append(one(i))
+        torch.cuda.synchronize()
+    cap = inputs[1][0].detach()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = gated_scan(cap, inputs[1][1])
+    bad = []
+
+    def work(seed):
+        with torch.cuda.stream(shared):
+            for i in np.random.default_rng(seed).integers(0, len(sizes), 40):
+                bad.extend([i] if not all(torch.equal(a, b) for a, b in zip(one(i), want[i])) else [])
+    shared = torch.cuda.Stream()
+    shared.wait_stream(torch.cuda.current_stream())
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for _ in range(5):
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[1][0]) and torch.equal(out[1], want[1][1])
+    for t in threads:
+        t.join(100)
+    assert not bad
+
+
 @pytest.mark.parametrize("T", [1, 64, 700])
 def test_gated_scan_in_graphs(T):
     """Forward and backward captured, replayed several times with new inputs and eager work in between, next to a second graph of the

@@ -118,7 +118,7 @@ def test_scan_forward_refuses(kw):
     _refused("stes_gated_scan_fwd", _scan_args(**kw))
 
 
-@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256), dict(scrub=256)])
+@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256), dict(scrub=256, scrub_bytes=16)])
 def test_scan_backward_refuses(kw):
     _refused("stes_gated_scan_bwd", _scan_args(**kw))
 
