@@ -23,7 +23,10 @@ __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x
 template <int CTRL, int ROWS> __device__ __forceinline__ float dpp(float none, float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
-constexpr int ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) {       // (every lane has a source)
+    return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+}
+constexpr int ROW_ROR = 0x120, ROW_SHR = 0x110, ROW_BCAST15 = 0x142, ROW_BCAST31 = 0x143;
 constexpr int QUAD_XOR1 = 0xB1, QUAD_XOR2 = 0x4E, ROW_HALF_MIRROR = 0x141, ROW_MIRROR = 0x140;
 
 // f over the G < 64 lanes of a lane group, the result in all of them.  (Once the lanes of a quad hold the same, mirroring eight lanes
@@ -35,6 +38,12 @@ template <int G, typename F> __device__ __forceinline__ float group_fold(float v
     if (G >= 16) v = f(v, dpp<ROW_MIRROR, 0xf>(v, v));
     if (G >= 32) v = f(v, __shfl_xor(v, 16, 64));
     return v;
+}
+
+// What another lane of this wave wrote to LDS is read next (a wave's LDS accesses are executed in order; this keeps the compiler's).
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // reductions over the G lanes of an aligned lane group
@@ -81,6 +90,32 @@ template <int G> __device__ __forceinline__ int from(int v, int j, int lane) {
 }
 template <int G> __device__ __forceinline__ float from(float v, int j, int lane) { return __int_as_float(from<G>(__float_as_int(v), j, lane)); }
 
+// a ^ b is zero where a key is found again N or fewer places further on in its row of 16 lanes, which closes into a ring
+template <int N> struct Ring {
+    static __device__ __forceinline__ unsigned nearest(unsigned a, unsigned b) {
+        const unsigned here = a ^ dpp<ROW_ROR + N>(b), nearer = Ring<N - 1>::nearest(a, b);
+        return here < nearer ? here : nearer;
+    }
+};
+template <> struct Ring<0> { static __device__ __forceinline__ unsigned nearest(unsigned, unsigned) { return ~0u; } };
+
+// Whether the lane's class is held by another lane of its group as well; of two lanes that share one at least one says so.  Half a ring
+// of 16 holds every pair once; a group of more lanes compares its rows of 16 with one another.
+template <int G>
+__device__ __forceinline__ bool listed_twice(int at, int lane, int k) {
+    const unsigned key = at < 0 ? 0x80000000u | (unsigned)lane : (unsigned)at ^ (G < 16 ? (unsigned)(lane / G) << 24 : 0u);
+    unsigned d = Ring<(G < 8 ? G - 1 : G == 8 ? 7 : 8)>::nearest(key, key);
+    if (G >= 32 && k > 16) {
+#pragma unroll
+        for (int o = 16; o < G; o += 16) {
+            const unsigned other = (unsigned)__shfl_xor((int)key, o, 64), x = key ^ other, y = Ring<8>::nearest(key, other);
+            d = min(d, min(x, y));
+            if (o == 16 && k <= 32) break;
+        }
+    }
+    return d == 0;
+}
+
 struct Listed { int at; float v; };      // one place of a row's list as it was loaded: index (< 0: unused, V: beyond the classes) and value
 
 __device__ __forceinline__ Listed load_listed(const stes_distill_args& p, long m, bool row, int l) {
@@ -109,18 +144,10 @@ __device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, const L
     if (!entries) return e;
     float w = v > -INFINITY ? exp2_((v - mx) * ct) : 0.f;
     w *= __builtin_amdgcn_rcpf(group_sum<G>(w));
-    // merge duplicates, which hardly ever occur: a wave first asks whether there are any
+    // merge duplicates, which hardly ever occur
     float whole = w;
     int first = l;
-    bool twice = true;
-    if constexpr (G == 64) {
-        twice = false;
-        for (int j = 0; j < p.k; ++j) {
-            const int aj = from<G>(e.at, j, lane);
-            twice = twice || (aj >= 0 && __popcll(__ballot(e.at == aj)) > 1);
-        }
-    }
-    if (twice) {
+    if (__any(listed_twice<G>(e.at, lane, p.k))) {
         whole = 0.f;
         first = G;
         for (int j = 0; j < p.k; ++j) {
@@ -152,11 +179,10 @@ __device__ __forceinline__ void leave(const stes_distill_args& p, float* part, d
 enum { LOSS = 1, GRAD = 2, STATS_IN = 4 };           // what a launch does
 
 // ---------------------------------------------------------------- short rows
-// V <= 8 G and k <= G: a group of G lanes per row, at most 8 classes a lane, neighbouring lanes neighbouring classes.  BLOCK / G rows a
+// V <= E G and k <= G: a group of G lanes per row, at most E classes a lane, neighbouring lanes neighbouring classes.  BLOCK / G rows a
 // workgroup and round, the next round's rows loaded ahead; a workgroup's rows follow from its index alone, and so does the order
 // of its sum.
-template <typename TS, int G> struct ShortRow {
-    static constexpr int E = 8;
+template <typename TS, int G, int E> struct ShortRow {
     TS x[E];
     Listed listed;
     float w;
@@ -170,20 +196,26 @@ template <typename TS, int G> struct ShortRow {
     }
 };
 
-template <typename TS, typename TG, int G, int BLOCK, int MODE>
+template <typename TS, typename TG, int G, int E, int BLOCK, int MODE>
 __global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill_args p, int rounds, float* __restrict__ part, double factor, float scale) {
-    constexpr int E = 8, RPB = BLOCK / G;
+    constexpr int RPB = BLOCK / G;
     __shared__ double red[BLOCK / 64];
+    __shared__ float target[MODE & GRAD ? BLOCK * E : 1];    // P of the rows at work, zero but for the listed classes
     const int lane = threadIdx.x & 63, l = threadIdx.x % G;
+    float* const mine = target + (MODE & GRAD ? threadIdx.x / G * (G * E) : 0);
+    if (MODE & GRAD) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine[e * G + l] = 0.f;
+    }
     const float ct = LOG2E / p.temperature;
     const long first = (long)blockIdx.x * rounds * RPB + threadIdx.x / G;
     double total = 0.0;
-    ShortRow<TS, G> next;
+    ShortRow<TS, G, E> next;
     next.load(p, first, l);
     for (int r = 0; r < rounds; ++r) {
         const long m = first + r * RPB;
         const bool row = m < p.M;
-        const ShortRow<TS, G> in = next;
+        const ShortRow<TS, G, E> in = next;
         if (r + 1 < rounds) next.load(p, m + RPB, l);
         float x[E];
 #pragma unroll
@@ -209,38 +241,31 @@ __global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill
             sum = group_sum<G>(sum);
             if (p.stats && row && l == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = sum; }
         }
-        float pv[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) pv[e] = 0.f;
-        for (int j = 0; j < p.k; ++j) {                      // hand every entry to the lane whose registers hold its class
-            const int aj = from<G>(t.at, j, lane);
-            const float pj = from<G>(t.p, j, lane);
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (aj == e * G + l) pv[e] = pj;
-        }
         if (MODE & LOSS) {
-            float kl = 0.f;
-            const float ls = log2_(sum);
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (pv[e] > 0.f) kl += kl_part(pv[e], x[e], mx, ls, ct);
-            kl = LN2 * group_sum<G>(kl);
+            const float st = t.at >= 0 ? (float)((const TS*)p.logits)[m * p.ld + t.at] : 0.f;
+            float kl = LN2 * group_sum<G>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), ct) : 0.f);
             if (t.bad) kl = __builtin_nanf("");
             if (counts && l == 0) total += (double)(w * kl);
         }
-        if ((MODE & GRAD) && row) {
-            const float f = row_factor(p, scale, w, t.bad), inv = __builtin_amdgcn_rcpf(sum);
-            TG* d = (TG*)p.dlogits + m * p.ld_d;
+        if (MODE & GRAD) {
+            if (t.at >= 0) mine[t.at] = t.p;
+            wave_lds_fence();
+            if (row) {
+                const float f = row_factor(p, scale, w, t.bad), inv = __builtin_amdgcn_rcpf(sum);
+                TG* d = (TG*)p.dlogits + m * p.ld_d;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int v = e * G + l;
-                if (v < p.V) {
-                    const float g = counts ? f * (q[e] * inv - pv[e]) : 0.f;
-                    if (!p.accumulate) d[v] = (TG)g;
-                    else if (counts) d[v] = (TG)((float)d[v] + g);
+                for (int e = 0; e < E; ++e) {
+                    const int v = e * G + l;
+                    if (v < p.V) {
+                        const float g = counts ? f * (q[e] * inv - mine[v]) : 0.f;
+                        if (!p.accumulate) d[v] = (TG)g;
+                        else if (counts) d[v] = (TG)((float)d[v] + g);
+                    }
                 }
             }
+            wave_lds_fence();
+            if (t.at >= 0) mine[t.at] = 0.f;
+            wave_lds_fence();
         }
     }
     if (MODE & LOSS) {
@@ -471,19 +496,24 @@ int distill_check(const stes_distill_args* a, bool bwd) {
 double loss_factor(const stes_distill_args& a) { return (double)a.temperature * a.temperature / a.denom; }
 float grad_factor(const stes_distill_args& a) { return (float)((double)a.grad_scale * a.temperature / a.denom); }
 
-template <typename TS, typename TG, int G, int MODE>
+template <typename TS, typename TG, int G, int E, int MODE>
 int launch_short(const stes_distill_args& a, hipStream_t s) {
     // A loss of a few rounds of one large workgroup is done in one launch.  1,024 frames of 7 classes: 12 us on the GPU and 16 us a call
     // from Python; many workgroups and the launch that adds up what they leave: 5 + 4 us and 19 us a call.
     if ((MODE & LOSS) && a.M <= 4 * (1024 / G)) {
-        hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, 1024, MODE>), dim3(1), dim3(1024), 0, s, a, (a.M + 1024 / G - 1) / (1024 / G), a.ws, loss_factor(a), grad_factor(a));
+        hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 1024, MODE>), dim3(1), dim3(1024), 0, s, a, (a.M + 1024 / G - 1) / (1024 / G), a.ws, loss_factor(a), grad_factor(a));
         return 1;
     }
     constexpr int RPB = 256 / G;
     const long teams = ((long)a.M + RPB - 1) / RPB;
     const int rounds = (int)((teams + 2047) / 2048), blocks = (int)((teams + rounds - 1) / rounds);
-    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, 256, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a), grad_factor(a));
+    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 256, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a), grad_factor(a));
     return blocks;
+}
+
+template <typename TS, typename TG, int G, int MODE>
+int launch_group(const stes_distill_args& a, hipStream_t s) {
+    return a.V <= 8 * G ? launch_short<TS, TG, G, 8, MODE>(a, s) : launch_short<TS, TG, G, 16, MODE>(a, s);
 }
 
 template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
@@ -500,30 +530,26 @@ int launch_rows(const stes_distill_args& a, hipStream_t s) {
     if constexpr (W == 1) {
         return launch_row<TS, TG, 1, 256, 1, true, MODE>(a, s);
     } else {
-        if constexpr ((MODE & STATS_IN) != 0) {              // nothing is reduced: read, write
-            if (a.V <= 64 * 8 * W) return launch_row<TS, TG, W, 64, 1, true, MODE>(a, s);
-            return launch_row<TS, TG, W, 256, 1, true, MODE>(a, s);
-        } else {
-            const int vecs = (a.V + W - 1) / W;
-            if (vecs <= 64 * 8) return launch_row<TS, TG, W, 64, 8, false, MODE>(a, s);
-            if (vecs <= 256 * 8) return launch_row<TS, TG, W, 256, 8, false, MODE>(a, s);
-            if (vecs <= 512 * 8) return launch_row<TS, TG, W, 512, 8, false, MODE>(a, s);
-            if (vecs <= 1024 * 8) return launch_row<TS, TG, W, 1024, 8, false, MODE>(a, s);
-            if (vecs <= 1024 * 16 && (MODE & GRAD)) return launch_row<TS, TG, W, 1024, 16, false, MODE>(a, s);
-            return launch_row<TS, TG, W, 1024, 1, true, MODE>(a, s);
-        }
+        const int vecs = (a.V + W - 1) / W;
+        if (vecs <= 64 * 8) return launch_row<TS, TG, W, 64, 8, false, MODE>(a, s);
+        if (vecs <= 256 * 8) return launch_row<TS, TG, W, 256, 8, false, MODE>(a, s);
+        if (vecs <= 512 * 8) return launch_row<TS, TG, W, 512, 8, false, MODE>(a, s);
+        if (vecs <= 1024 * 8) return launch_row<TS, TG, W, 1024, 8, false, MODE>(a, s);
+        if (vecs <= 1024 * 16 && (MODE & GRAD)) return launch_row<TS, TG, W, 1024, 16, false, MODE>(a, s);
+        return launch_row<TS, TG, W, 1024, 1, true, MODE>(a, s);
     }
 }
 
 template <typename TS, typename TG, int MODE>
 int launch_mode(const stes_distill_args& a, hipStream_t s) {
     if (a.V <= 8 * 64) {
-        const int g = a.k > (a.V + 7) / 8 ? a.k : (a.V + 7) / 8;
-        if (g <= 4) return launch_short<TS, TG, 4, MODE>(a, s);
-        if (g <= 8) return launch_short<TS, TG, 8, MODE>(a, s);
-        if (g <= 16) return launch_short<TS, TG, 16, MODE>(a, s);
-        if (g <= 32) return launch_short<TS, TG, 32, MODE>(a, s);
-        return launch_short<TS, TG, 64, MODE>(a, s);
+        // as few lanes a row as hold its list and, 16 classes a lane, its logits
+        const int g = a.k > (a.V + 15) / 16 ? a.k : (a.V + 15) / 16;
+        if (g <= 4) return launch_group<TS, TG, 4, MODE>(a, s);
+        if (g <= 8) return launch_group<TS, TG, 8, MODE>(a, s);
+        if (g <= 16) return launch_group<TS, TG, 16, MODE>(a, s);
+        if (g <= 32) return launch_group<TS, TG, 32, MODE>(a, s);
+        return launch_short<TS, TG, 64, 8, MODE>(a, s);
     }
     if constexpr (sizeof(TS) == sizeof(TG)) {
         // 16-byte accesses need the rows of logits and of dlogits at the same offset from a 16-byte boundary
