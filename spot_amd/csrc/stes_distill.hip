@@ -484,6 +484,7 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(bwd || a->loss, STES_ERR_ARG, "stes_distill: loss is needed");
     if (!a->M) return STES_OK;
     STES_CHECK(a->V < 0x7fff0000, STES_ERR_UNSUPPORTED, "stes_distill: too many classes");
+    STES_CHECK(a->V <= 8 * 64 || a->M < (1 << 22), STES_ERR_UNSUPPORTED, "stes_distill: more rows than a launch holds (2^32 threads)");
     STES_CHECK(a->logits && a->idx && a->val, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->ld >= a->V && a->ld_idx >= a->k && a->ld_val >= a->k, STES_ERR_ARG, "stes_distill: rows overlap");
     STES_CHECK(!a->dlogits || a->ld_d >= a->V, STES_ERR_ARG, "stes_distill: rows of dlogits overlap");

@@ -8,10 +8,10 @@
 //
 // Joining the blocks of a sequence (T > STES_SCAN_BLOCK): workgroups draw tickets, all channels of a block of time before the
 // next block, and a workgroup waits for lower tickets only, whose workgroups have started before it and wait for lower ones
-// still: every wait ends.  Each block publishes its map (A, B) as soon as it has it and its final state when it knows the one in
-// front; a later block walks back over published maps to the nearest published state.  Both are single 64-bit words that are
-// valid when they are not zero (A >= 0 carries its sign bit set, a state a one beside it), so relaxed atomics of agent
-// scope carry them and no fence or cache write-back is needed.  Words are cleared by a kernel in front of every call.
+// still: every wait ends.  Each block publishes its map (A, B) as soon as it has it and the state behind it when it knows the one in
+// front; a later block walks back over published maps to the nearest published state.  Results do not depend on when words
+// arrive.  Maps and states are single 64-bit words that are valid when they are not zero (A >= 0 carries its sign bit set, a state a
+// one beside it), so relaxed atomics of agent scope carry them and no fence or cache write-back is needed.
 #include "stes_common.h"
 
 namespace {
@@ -70,34 +70,45 @@ __device__ __forceinline__ uint64_t peek(const uint64_t* w) { return __hip_atomi
 __device__ __forceinline__ uint64_t map_word(float A, float B) { return ((uint64_t)__float_as_uint(B) << 32) | (__float_as_uint(A) | 0x80000000u); }
 __device__ __forceinline__ uint64_t state_word(float x) { return ((uint64_t)__float_as_uint(x) << 32) | 1u; }
 
+// a state through a block's map: one operation everywhere, so that it rounds alike everywhere
+__device__ __forceinline__ float through(float A, float B, float x) { return __builtin_fmaf(A, x, B); }
+
 constexpr int LOOK = 4;                  // blocks looked at in one round trip to memory
+constexpr int REACH = 32;                // maps that a walk keeps; with so many it waits for the state behind them
 constexpr int MAX_ROUNDS = 1 << 22;      // (an exit for a broken workspace: the state becomes NaN)
 
-// The state in front of block `blk` >= 1 of a channel; `at` is the channel's word in a row of `words` words.
-__device__ __forceinline__ float look_back(const Link& l, long at, long words, int blk) {
-    float A = 1.f, B = 0.f;
-    int t = blk - 1;
+// The state in front of block `blk` >= 1 of a channel (lane = channel): a walk back to the nearest published state, then that state
+// through the maps of the blocks between, in their order.  Every state is its block's map of the state in front, so that is the same
+// sequence of operations, and the same bits, wherever the walk ends.  `at` is the channel's word in a row of `words` words.
+__device__ __forceinline__ float look_back(const Link& l, uint64_t (*kept)[64], long at, long words, int blk) {
+    const int lane = threadIdx.x & 63;
+    int depth = 0;                       // maps kept, of the blocks blk - 1, blk - 2, ...
     for (int round = 0; round < MAX_ROUNDS; ++round) {
         uint64_t st[LOOK], mp[LOOK];
 #pragma unroll
         for (int k = 0; k < LOOK; ++k) {
-            const int q = t - k < 0 ? 0 : t - k;
+            const int q = blk - 1 - depth - k < 0 ? 0 : blk - 1 - depth - k;
             st[k] = peek(l.state + q * words + at);
             mp[k] = peek(l.map + q * words + at);
         }
-        const int before = t;
-        bool open = true;
+        const int before = depth;
+        bool open = true, found = false;
+        float x = 0.f;
 #pragma unroll
         for (int k = 0; k < LOOK; ++k) {
-            if (!open || before - k < 0) continue;
-            if (st[k]) return A * __uint_as_float((uint32_t)(st[k] >> 32)) + B;
-            if (mp[k]) {
-                B = A * __uint_as_float((uint32_t)(mp[k] >> 32)) + B;
-                A = A * __uint_as_float((uint32_t)mp[k] & 0x7fffffffu);
-                --t;                     // (block 0 publishes a state and no map: the walk ends there)
-            } else open = false;
+            if (!open || blk - 1 - before - k < 0) continue;
+            if (st[k]) { x = __uint_as_float((uint32_t)(st[k] >> 32)); found = true; open = false; }
+            else if (mp[k] && depth < REACH) kept[depth++][lane] = mp[k];          // (block 0 publishes a state and no map)
+            else open = false;
         }
-        if (t == before) __builtin_amdgcn_s_sleep(1);
+        if (found) {
+            for (int d = depth - 1; d >= 0; --d) {
+                const uint64_t m = kept[d][lane];
+                x = through(__uint_as_float((uint32_t)m & 0x7fffffffu), __uint_as_float((uint32_t)(m >> 32)), x);
+            }
+            return x;
+        }
+        if (depth == before) __builtin_amdgcn_s_sleep(1);
     }
     return __builtin_nanf("");
 }
@@ -152,6 +163,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
     constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
     __shared__ float sA[G::NS][CT], sB[G::NS][CT];       // maps of the segments, then of what precedes them in their wave
     __shared__ float tA[NW][CT], tB[NW][CT];             // maps of the waves; tB then: the state in front of each
+    __shared__ uint64_t kept[JOIN ? REACH : 1][64];
     __shared__ unsigned drawn;
     const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
     const int tid = threadIdx.x, cl = tid % G::LPR, seg = tid / G::LPR, lane = tid & 63, wave = tid >> 6;
@@ -214,9 +226,9 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
             if (!JOIN || at.blk == 0) x = p.h0 ? p.h0[at.b * p.bs_h0 + ch] : 0.f;
             else {
                 if (at.blk + 1 < blocks) publish(link.map + at.blk * words + word, map_word(mA, mB));
-                x = look_back(link, word, words, at.blk);
+                x = look_back(link, kept, word, words, at.blk);
             }
-            const float end = mA * x + mB;
+            const float end = through(mA, mB, x);
             if (JOIN && at.blk + 1 < blocks) publish(link.state + at.blk * words + word, state_word(end));
             if (at.blk + 1 == blocks && p.h_last) p.h_last[at.b * p.bs_hl + ch] = end;
             if (p.states) p.states[((long)at.b * blocks + at.blk) * H + ch] = x;
@@ -251,6 +263,7 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
     constexpr int V = G::V, L = G::L, CT = G::CT, SW = G::SW, NW = G::NW;
     __shared__ float sA[G::NS][CT], sB[G::NS][CT], sR[G::NS][CT], sS[G::NS][CT];
     __shared__ float tA[NW][CT], tB[NW][CT], tR[NW][CT];             // tB and tR then: what comes to a wave from either side
+    __shared__ uint64_t kept[JOIN ? REACH : 1][64];
     __shared__ unsigned drawn;
     const Place at = place<G, JOIN>(p, tiles, chains, ticket, &drawn);
     const int blk = blocks - 1 - at.blk;
@@ -279,15 +292,17 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
     for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; R[v] = 0.f; }
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-        if (on && s0 + j < n) {
+        // (selects, not a branch: the gates then stay in registers for the passes below; recomputed, 60 % more time on short sequences)
+        const bool live = on && s0 + j < n;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float z, k;
-                gate_pair((float)g[j][v], z, k);
-                B[v] = k * B[v] + z * (float)cand[j][v];
-                A[v] *= k;
-                R[v] += A[v] * (float)d[j][v];           // d_j reaches the segment's front through a_0 .. a_j
-            }
+        for (int v = 0; v < V; ++v) {
+            float z, k;
+            gate_pair((float)g[j][v], z, k);
+            k = live ? k : 1.f;
+            const float u = live ? z * (float)cand[j][v] : 0.f;
+            B[v] = k * B[v] + u;
+            A[v] *= k;
+            R[v] += A[v] * (float)d[j][v];               // d_j reaches the segment's front through a_0 .. a_j
         }
     }
 #pragma unroll
@@ -330,9 +345,9 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
             if (!JOIN || at.blk == 0) k = p.dh_last ? p.dh_last[at.b * p.bs_dhl + ch] : 0.f;
             else {
                 if (blk) publish(link.map + at.blk * words + word, map_word(mA, mR));
-                k = look_back(link, word, words, at.blk);
+                k = look_back(link, kept, word, words, at.blk);
             }
-            const float front = mA * k + mR;
+            const float front = through(mA, mR, k);
             if (JOIN && blk) publish(link.state + at.blk * words + word, state_word(front));
             if (!blk && p.dh0) p.dh0[at.b * H + ch] = front;
         }
@@ -500,8 +515,8 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
     STES_CHECK(a->f32 == 0 || a->f32 == 1, STES_ERR_ARG, "stes_gated_scan: f32 is 0 (bf16) or 1 (fp32)");
     STES_CHECK(!a->dh0_sum || a->dh0 || !a->B, STES_ERR_ARG, "stes_gated_scan_bwd: dh0_sum needs dh0");
     if (!a->B || !a->H) return STES_OK;
-    STES_CHECK(a->H <= (1 << 24) && (long)a->B * ((a->H + CT - 1) / CT) * (blocks_of(a->T) + 1) < (1L << 31), STES_ERR_UNSUPPORTED,
-               "stes_gated_scan: more tiles than a launch holds");
+    STES_CHECK(a->H <= (1 << 24) && a->B <= (1 << 24) && (long)a->B * ((a->H + CT - 1) / CT) * (blocks_of(a->T) + 1) < (1L << 23), STES_ERR_UNSUPPORTED,
+               "stes_gated_scan: more tiles than a launch holds (2^32 threads)");
     if (a->T) {
         STES_CHECK(a->pre && a->ld_pre >= 2L * a->H && a->bs_pre >= 0, STES_ERR_ARG, "stes_gated_scan: pre is [B][T][2H]");
         if (!bwd) STES_CHECK(a->h && apart(a->ld_h, a->T, a->bs_h, a->B, a->H), STES_ERR_ARG, "stes_gated_scan_fwd: h is [B][T][H], rows apart");

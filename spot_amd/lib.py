@@ -270,6 +270,9 @@ def guard_leaves(node):
     eager graph of the same leaf lives would pull that stream into the capture, which ends the process.  Eager calls mark
     their leaves' nodes, captured ones refuse marked nodes."""
     for n, _ in node.next_functions:
+        for _ in range(4):                           # (through the views and copies that a call makes of a leaf)
+            if n is not None and len(n.next_functions) == 1:
+                n = n.next_functions[0][0]
         if n is not None and not n.next_functions:
             mark = n.metadata
             if not torch.cuda.is_current_stream_capturing():

@@ -177,6 +177,26 @@ def test_gated_scan_strides_and_alignment(dtype, H, off):
     _check(g, ref["dpre"], ref["dpre_err"], "dpre")
 
 
+@pytest.mark.parametrize("B,T,H", [(1, 30000, 96), (40, 2000, 64), (3, 5000, 300)])
+def test_gated_scan_gives_the_same_bits_every_time(B, T, H):
+    """fp32 results do not depend on which blocks of a sequence finish first: calls alone, back to back and next to another stream's."""
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, _, dlast = _scan_inputs(B, T, H, F32, False, "rows", seed=B, gate=(-5.0, 1.0))
+    p, s, dl = pre.cuda().requires_grad_(), start.cuda().requires_grad_(), dlast.cuda()
+
+    def one():
+        h, last = gated_scan(p, s)
+        return (h.detach(), last.detach()) + torch.autograd.grad((h, last), (p, s), (torch.ones_like(h), dl))
+    want = one()
+    torch.cuda.synchronize()
+    side, noise = torch.cuda.Stream(), torch.empty(1 << 26, device="cuda")
+    for r in range(12):
+        if r > 5:
+            with torch.cuda.stream(side):
+                noise.mul_(1.5)
+        assert all(torch.equal(a, b) for a, b in zip(one(), want)), r
+
+
 def test_gated_scan_gradient_from_final_state_alone():
     from spot_amd.recurrence import gated_scan
     for T in (1, 5, 200):

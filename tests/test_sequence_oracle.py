@@ -113,7 +113,7 @@ def _scan_args(**kw):
 @pytest.mark.parametrize("kw", [dict(B=-1), dict(T=-1), dict(H=-1), dict(f32=2), dict(pre=None), dict(h=None), dict(ld_pre=15), dict(ld_h=7), dict(bs_h=31), dict(bs_h=0),
                                 dict(bs_hl=7), dict(h0=512, bs_h0=3), dict(h0=256, bs_h0=0), dict(h0=256, bs_h0=9), dict(scrub=256, scrub_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, ws=264),
                                 dict(T=1000, bs_pre=16000, bs_h=8000, ws_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, scrub=256, scrub_bytes=8),
-                                dict(B=70000000, H=1 << 20)])
+                                dict(B=70000000, H=1 << 20), dict(B=1 << 23, T=1, H=64, ld_pre=128, bs_pre=128, bs_h=64, ld_h=64, bs_hl=64)])
 def test_scan_forward_refuses(kw):
     _refused("stes_gated_scan_fwd", _scan_args(**kw))
 
@@ -136,7 +136,7 @@ def _distill_args(**kw):
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(V=0), dict(k=0), dict(k=65, ld_idx=65, ld_val=65), dict(temperature=0.0), dict(temperature=-1.0),
                                 dict(temperature=float("nan")), dict(temperature=float("inf")), dict(denom=0.0), dict(denom=float("nan")),
                                 dict(logits=None), dict(idx=None), dict(val=None), dict(loss=None), dict(ld=6), dict(ld_idx=3), dict(ld_val=3),
-                                dict(dlogits=512, ld_d=6), dict(dlogits=256, ld_d=7), dict(ws_floats=0), dict(ws=None)])
+                                dict(dlogits=512, ld_d=6), dict(dlogits=256, ld_d=7), dict(M=1 << 22, V=1000, ld=1000), dict(ws_floats=0), dict(ws=None)])
 def test_distill_refuses(kw):
     _refused("stes_distill", _distill_args(**kw))
 
