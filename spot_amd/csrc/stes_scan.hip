@@ -485,13 +485,19 @@ __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_ar
             if (v < left) p.dh0[b * H + c + v] = k[v];
 }
 
-// The gradient of an initial state that the batch shares: the rows added up in order.
-__global__ __launch_bounds__(64) void scan_dh0_sum_kernel(const float* __restrict__ dh0, float* __restrict__ out, int B, int H) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= H) return;
+// The gradient of an initial state that the batch shares: 16 strands of rows per channel, each added up in order, then the strands.
+__global__ __launch_bounds__(1024) void scan_dh0_sum_kernel(const float* __restrict__ dh0, float* __restrict__ out, int B, int H) {
+    __shared__ float part[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), strand = threadIdx.x >> 6;
     float s = 0.f;
-#pragma unroll 8
-    for (int b = 0; b < B; ++b) s += dh0[(long)b * H + c];
+    if (c < H) {
+#pragma unroll 4
+        for (int b = strand; b < B; b += 16) s += dh0[(long)b * H + c];
+    }
+    part[strand][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (strand || c >= H) return;
+    for (int k = 1; k < 16; ++k) s += part[k][threadIdx.x];
     out[c] = s;
 }
 
@@ -592,7 +598,7 @@ extern "C" int stes_gated_scan_bwd(const stes_gated_scan_args* a, void* stream) 
         STES_LAUNCH_CHECK();
     }
     if (a->dh0_sum) {                                       // (zeros for an empty batch)
-        hipLaunchKernelGGL(scan_dh0_sum_kernel, dim3((a->H + 63) / 64), dim3(64), 0, (hipStream_t)stream, a->dh0, a->dh0_sum, a->B, a->H);
+        hipLaunchKernelGGL(scan_dh0_sum_kernel, dim3((a->H + 63) / 64), dim3(1024), 0, (hipStream_t)stream, a->dh0, a->dh0_sum, a->B, a->H);
         STES_LAUNCH_CHECK();
     }
     return STES_OK;

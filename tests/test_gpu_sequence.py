@@ -76,7 +76,7 @@ SCAN_CASES = [  # B, T, H, dtype, ragged, reverse, h0
     (2, 129, 7, F32, False, False, "rows"), (6, 255, 12, F32, True, False, "rows"), (3, 256, 68, BF, True, False, "rows"),
     (2, 257, 260, F32, False, True, "shared"), (5, 700, 200, BF, True, False, "rows"), (1, 1000, 264, BF, False, False, "rows"),
     (1, 1025, 130, F32, False, True, "rows"), (2, 3001, 9, BF, True, True, "shared"), (1, 9000, 8, F32, False, False, "rows"),
-    (1, 20000, 3, BF, False, True, "rows"), (40, 130, 64, BF, True, False, "shared"),
+    (1, 20000, 3, BF, False, True, "rows"), (40, 130, 64, BF, True, False, "shared"), (700, 2, 70, F32, True, False, "shared"),
 ]
 
 
