@@ -474,7 +474,8 @@ int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h
  * Its contents are irrelevant unless ws_zero != 0 says that they are zero, which spares the launch that clears them (they are not
  * zero afterwards).  scrub (optional, with T > STES_SCAN_BLOCK): scrub_bytes of other memory, a multiple of 16, that the call leaves zero on
  * the way: what a caller that alternates between two workspaces on one stream used in the call before.
- * Results do not depend on scheduling beyond the association of the time axis: see stes_scan.hip. */
+ * Results do not depend on scheduling; another T or another start associates the time axis differently (a whole sequence and its
+ * parts agree to fp32 rounding).  Fewer than 2^23 tiles of 64 channels x STES_SCAN_BLOCK steps a call. */
 #define STES_SCAN_BLOCK 256
 typedef struct {
     const void* pre; int64_t ld_pre, bs_pre;

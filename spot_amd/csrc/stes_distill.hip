@@ -5,6 +5,11 @@
 // short row) in registers as it was loaded, takes the maximum, the sum of exp, and writes q straight from the registers; the listed
 // classes, k of V, are written over by the lanes that hold them.  Rows too long for a workgroup's registers are read twice (the
 // second time mostly from the cache).
+//
+// Measured (a copy of 1 GiB runs at 4,980 GB/s): loss and gradient in one pass of 8,192 x 32,003 bf16 206 us (5.1 TB/s); of
+// 2,048 x 50,001 fp32 loss 73 to 110 us and gradient 148 us (5.6 TB/s and, behind the gradient's writes, 3.7; 5.5 TB/s); 16,384 x 1,000
+// bf16 15 and 16 us (bound by the teacher's part of a row, some 200 instructions a wave, and its chain of loads: index, then logit);
+// short rows are bound by instructions too: 131,072 x 300 bf16 loss 52 us, gradient 65 us.
 #include "stes_common.h"
 
 namespace {
@@ -544,7 +549,8 @@ int launch_rows(const stes_distill_args& a, hipStream_t s) {
 template <typename TS, typename TG, int MODE>
 int launch_mode(const stes_distill_args& a, hipStream_t s) {
     if (a.V <= 8 * 64) {
-        // as few lanes a row as hold its list and, 16 classes a lane, its logits
+        // As few lanes a row as hold its list and, 16 classes a lane, its logits: a wave's instructions then serve the most rows
+        // (131,072 x 300 bf16, 30 listed: loss 52 us with 16 classes a lane, 80 us with 8; 131,072 x 40 fp32: 13.0 and 13.9 us).
         const int g = a.k > (a.V + 15) / 16 ? a.k : (a.V + 15) / 16;
         if (g <= 4) return launch_group<TS, TG, 4, MODE>(a, s);
         if (g <= 8) return launch_group<TS, TG, 8, MODE>(a, s);
