@@ -501,7 +501,7 @@ int stes_loss(const float* logits, int64_t ldl, const float* loc, int64_t ldloc,
               uint16_t* dlogits, uint16_t* dloc, void* stream);
 /* Distillation from a teacher's top logits, beside stes_loss (no counterpart in the reference).  Per row m of logits [M][V]
  * (bf16 or fp32), with idx / val [M][k] the teacher's top classes and their logits (k <= STES_DISTILL_MAX_K; idx int64 or int32, val fp32
- * or bf16) and tau = temperature:
+ * or bf16) and tau = temperature (1e-6 to 1e6):
  *   p = softmax(val[m] / tau) over the entries with idx >= 0,  P_v = sum of p over the entries with idx = v,
  *   q = softmax(logits[m] / tau) over all V classes,  KL_m = sum_v P_v (log P_v - log q_v)  (entries with P_v = 0 count nothing)
  *   loss = tau^2 / denom * sum_m weight[m] KL_m,   dlogits[m][v] = grad_scale * upstream * weight[m] tau / denom * (q_v - P_v)

@@ -146,7 +146,10 @@ __device__ __forceinline__ Entry teacher_row(const stes_distill_args& p, const L
     e.bad = group_any<G>(e.at >= p.V || v != v || v == INFINITY, lane);
     e.some = mx > -INFINITY || e.bad;
     e.p = 0.f;
-    if (!entries) return e;
+    if (!entries) {
+        e.at = -1;
+        return e;
+    }
     float w = v > -INFINITY ? exp2_((v - mx) * ct) : 0.f;
     w *= __builtin_amdgcn_rcpf(group_sum<G>(w));
     // merge duplicates, which hardly ever occur
@@ -484,7 +487,7 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->M >= 0 && a->V >= 1 && a->k >= 1, STES_ERR_ARG, "stes_distill: M >= 0, V >= 1 and k >= 1");
     STES_CHECK(a->k <= STES_DISTILL_MAX_K, STES_ERR_UNSUPPORTED, "stes_distill: at most 64 teacher classes a row");
-    STES_CHECK(a->temperature > 0.f && a->temperature < INFINITY, STES_ERR_ARG, "stes_distill: the temperature is positive");
+    STES_CHECK(a->temperature >= 1e-6f && a->temperature <= 1e6f, STES_ERR_ARG, "stes_distill: the temperature lies between 1e-6 and 1e6");
     STES_CHECK(a->denom > 0.0, STES_ERR_ARG, "stes_distill: the denominator is positive");
     STES_CHECK(bwd || a->loss, STES_ERR_ARG, "stes_distill: loss is needed");
     if (!a->M) return STES_OK;

@@ -95,8 +95,8 @@ def _check(logits, idx, val, weight, temperature, denom):
     if torch.is_grad_enabled() and (val.requires_grad or (weight is not None and weight.requires_grad)):
         _refuse("the teacher's logits and the weights are constants: detach them")
     temperature = float(temperature)
-    if not 0.0 < temperature < math.inf:
-        _refuse(f"the temperature is positive, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        _refuse(f"the temperature lies between 1e-6 and 1e6, got {temperature}")
     s = _flat(logits, V)
     denom = float(max(1, s.shape[0]) if denom is None else denom)
     if not 0.0 < denom < math.inf:

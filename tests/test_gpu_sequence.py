@@ -135,6 +135,22 @@ def test_gated_scan_padding_is_not_looked_at(dtype, T, H, reverse):
     assert float(got[0][1, 1:].abs().max()) == 0 and float(got[2][1, 1:].abs().max()) == 0
 
 
+def test_gated_scan_of_one_sequence_seen_several_times():
+    """pre expanded over the batch (no memory of its own per sequence), from other states and over other lengths: gradients of the
+    sequences add up in the one that is there."""
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, dh, dlast = _scan_inputs(3, 280, 20, F32, False, "rows", seed=6)
+    n = torch.tensor([280, 3, 0], dtype=torch.int32)
+    p, s = pre[:1].cuda().requires_grad_(), start.cuda().requires_grad_()
+    h, last = gated_scan(p.expand(3, 280, 40), s, n.cuda())
+    g = torch.autograd.grad((h, last), (p, s), (dh.cuda(), dlast.cuda()))
+    ref = SO.gated_scan(_np(pre[:1]).repeat(3, 0), _np(start), _np(n), False, _np(dh), _np(dlast), need_grad=True)
+    _check(h, ref["h"], ref["h_err"], "h")
+    _check(last, ref["last"], ref["last_err"], "last")
+    _check(g[0], ref["dpre"].sum(0, keepdims=True), ref["dpre_err"].sum(0, keepdims=True) + 4 * SO.U * np.abs(ref["dpre"]).sum(0, keepdims=True), "dpre")
+    _check(g[1], ref["dh0"], ref["dh0_err"], "dh0")
+
+
 def test_gated_scan_clamps_lengths():
     from spot_amd.recurrence import gated_scan
     pre, start, _, _, _ = _scan_inputs(3, 140, 8, BF, False, "rows", seed=0)
@@ -675,6 +691,30 @@ def test_distill_leading_dimensions_and_empty():
     assert float(topk_distill_grad(e, torch.zeros(0, 2, dtype=torch.int64, device="cuda"), torch.zeros(0, 2, device="cuda"))[0]) == 0.0
 
 
+@pytest.mark.parametrize("V", [6, 300, 5000, 40000, 200000])
+def test_distill_one_row_and_views(V):
+    """A single row without a leading dimension, transposed and expanded logits: copies where the kernels need them."""
+    from spot_amd.distill import topk_distill_grad, topk_distill_loss
+    s, idx, val, w = _kl_inputs(4, V, 3, F32, V + 7, False, True)
+    ref = SO.topk_distill(_np(s[:1]), _np(idx[:1]), _np(val[:1]), 2.0, _np(w[:1]))
+    loss, g = topk_distill_grad(s[0].cuda(), idx[0].cuda(), val[0].cuda(), 2.0, w[0].cuda())
+    _check(loss, ref["loss"], ref["loss_err"], "one row")
+    _check(g[None], ref["dlogits"], ref["dlogits_err"], "one row")
+    want = topk_distill_grad(s.cuda(), idx.cuda(), val.cuda(), 2.0, w.cuda())
+    x = s.t().contiguous().cuda().requires_grad_()
+    loss = topk_distill_loss(x.t(), idx.t().contiguous().cuda().t(), val.t().contiguous().cuda().t(), 2.0, w.cuda())
+    g, = torch.autograd.grad(loss, x)
+    assert torch.equal(loss, want[0])
+    _check(g.t(), _np(want[1]), 4 * SO.U * np.abs(_np(want[1])), "transposed")
+    y = s[:1].cuda().requires_grad_()
+    loss = topk_distill_loss(y.expand(4, V), idx[:1].cuda().expand(4, 3), val[:1].cuda().expand(4, 3), 2.0, w.cuda())
+    g, = torch.autograd.grad(loss, y)
+    ref = SO.topk_distill(_np(s[:1]).repeat(4, 0), _np(idx[:1]).repeat(4, 0), _np(val[:1]).repeat(4, 0), 2.0, _np(w))
+    _check(loss, ref["loss"], ref["loss_err"], "expanded")
+    total = ref["dlogits"].sum(0, keepdims=True)
+    _check(g, total, ref["dlogits_err"].sum(0, keepdims=True) + 4 * SO.U * np.abs(ref["dlogits"]).sum(0, keepdims=True), "expanded")
+
+
 def test_distill_gradient_against_differences():
     from spot_amd.distill import topk_distill_loss
     s, idx, val, w = _kl_inputs(64, 40, 6, F32, 3, True, True)
@@ -742,7 +782,7 @@ def test_distill_refusals():
     s, i, v = torch.zeros(4, 7, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda"), torch.zeros(4, 2, device="cuda")
     for kw in (dict(logits=s.half()), dict(idx=i.short()), dict(idx=i[:3]), dict(idx=i.cpu()), dict(val=v.double()), dict(val=v[:, :1]),
                dict(idx=i.repeat(1, 40), val=v.repeat(1, 40)), dict(idx=i[:, :0], val=v[:, :0]), dict(temperature=0.0), dict(temperature=-1),
-               dict(temperature=NAN), dict(temperature=INF), dict(denom=0.0), dict(denom=-2.0), dict(denom=NAN), dict(weight=torch.ones(4)),
+               dict(temperature=NAN), dict(temperature=INF), dict(temperature=1e-40), dict(denom=0.0), dict(denom=-2.0), dict(denom=NAN), dict(weight=torch.ones(4)),
                dict(weight=torch.ones(3, device="cuda")), dict(weight=torch.ones(4, device="cuda", dtype=BF)), dict(logits=s[:, :0]),
                dict(val=v.clone().requires_grad_()), dict(weight=torch.ones(4, device="cuda", requires_grad=True))):
         for f in (topk_distill_loss, topk_distill_grad):

@@ -134,7 +134,7 @@ def _distill_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(V=0), dict(k=0), dict(k=65, ld_idx=65, ld_val=65), dict(temperature=0.0), dict(temperature=-1.0),
-                                dict(temperature=float("nan")), dict(temperature=float("inf")), dict(denom=0.0), dict(denom=float("nan")),
+                                dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-7), dict(temperature=2e6), dict(denom=0.0), dict(denom=float("nan")),
                                 dict(logits=None), dict(idx=None), dict(val=None), dict(loss=None), dict(ld=6), dict(ld_idx=3), dict(ld_val=3),
                                 dict(dlogits=512, ld_d=6), dict(dlogits=256, ld_d=7), dict(M=1 << 22, V=1000, ld=1000), dict(ws_floats=0), dict(ws=None)])
 def test_distill_refuses(kw):
