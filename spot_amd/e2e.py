@@ -284,11 +284,14 @@ class E2EModel(BaseRGBModel):
     def predict_stream(self, seq, state):
         """predict_async() for the next frames of n streams (`state` of new_stream(n), updated in place): seq [n * W, T, C, H, W] holds W
         clips of every stream, one after the other in time.  Clips are independent in the backbone (T = clip_len where it
-        shifts channels in time, a shorter T is zero-padded there; T = 1 is a frame at a time for the plain backbone), while the
+        shifts channels in time, a shorter T is zero-padded there; T = 1 is a frame at a time for the plain backbone; one clip without
+        the leading dimension will do), while the
         minGRU head runs over a stream's W * T frames as one sequence that starts where the last call's ended: a video's scores
         do not depend on how it is cut into calls."""
         if self._temporal_arch != "mingru" or self._model.time_backward:
             raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
+        if seq.dim() == 4:
+            seq = seq.unsqueeze(0)
         n, hidden = (state[0].shape if len(state) else (0, 0))
         layers = self._model._pred_fine
         if (len(state) != layers.n_layers or hidden != layers.hidden_size or n < 1 or seq.shape[0] < 1 or seq.shape[0] % n
@@ -311,7 +314,8 @@ class E2EModel(BaseRGBModel):
         """One optimisation step entirely on the device.  frame [B,T,C,H,W] f32 (normalised) or uint8 (decoded), label [B,T] int64, xy [B,T,2] f32.
         distill: {"idx", "val" [B,T,k], "temperature" 1.0, "weight" 1.0, "frame_weight" [B,T] or None, "denom" or None (all frames)}:
         `weight` times the distillation loss from a teacher's top logits (spot_amd.distill) joins the loss.
-        Returns the device tensor {sum, cls, loc, sum of class weights, number of event frames, distillation loss, ...} (no host sync)."""
+        Returns the device tensor {sum, cls, loc, sum of class weights, number of event frames, distillation loss (with distill), ...}
+        (no host sync)."""
         m = self._model
         m.train()
         eng = m.engine

@@ -93,9 +93,11 @@ class ClipShards:
     def __init__(self, files, batch_size, rank=0, world=1):
         self.files, self.batch_size, self.rank, self.world = sorted(files), batch_size, rank, world
         self._n = []
+        self.teacher = bool(self.files)                      # every shard holds a teacher's top logits
         for f in self.files:
             with np.load(f) as z:
                 self._n.append(int(z["label"].shape[0]))
+                self.teacher = self.teacher and "teacher_idx" in z.files and "teacher_val" in z.files
 
     def __len__(self):
         return sum(n // self.batch_size for n in self._n) // self.world      # every rank the same number of steps
@@ -146,7 +148,7 @@ class AugmentedClips:
 
     def __init__(self, loader, device, crop_dim, is_eval, seed):
         from .augment import ClipAugmenter
-        self.loader, self.device = loader, device
+        self.loader, self.device, self.teacher = loader, device, getattr(loader, "teacher", False)
         self.aug = ClipAugmenter(crop_dim, is_eval=is_eval, seed=seed)
 
     def __len__(self):
@@ -457,6 +459,8 @@ def main(args):
                      device=args.device, predict_location=args.predict_location, pred_loc_arch=args.pred_loc_arch,
                      time_backward=args.time_backward, use_channel_attention=args.use_channel_attention, verbose=rank == 0)
     train_loader, val_loader = get_loaders(args, len(classes) + 1, rank, world)
+    if distilling["distill_weight"] > 0 and not getattr(train_loader, "teacher", False):
+        raise ValueError("--distill_weight needs training shards that all hold teacher_idx and teacher_val")
     optimizer, scaler = model.get_optimizer({"lr": args.learning_rate})
     num_steps_per_epoch = len(train_loader) // args.acc_grad_iter
     num_epochs, lr_scheduler = get_lr_scheduler(args, optimizer, num_steps_per_epoch)

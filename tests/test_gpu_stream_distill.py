@@ -90,6 +90,8 @@ def test_stream_with_a_padded_last_clip():
     a = m.predict_stream(x[None, :8], state)[0]
     b = m.predict_stream(x[None, 8:], state)[0]
     assert a.shape == (1, 8, 7) and b.shape == (1, 3, 7) and bool(torch.isfinite(b).all())
+    c = m.predict_stream(x[:8], m.new_stream())[0]           # one clip without the leading dimension
+    assert c.shape == a.shape and rel(c, a) < 1e-2
 
 
 def test_inference_carries_the_state():
@@ -203,3 +205,7 @@ def test_train_driver_with_a_teacher(tmp_path):
         assert len(losses) == 2 and all(np.isfinite(l["train"]) and np.isfinite(l["val"]) for l in losses)
     with pytest.raises(NotImplementedError):
         TR.main(TR.get_args([a for a in base if a != "--predict_location"] + ["-s", str(tmp_path / "x"), "--distill_weight", "1", "--mixup"]))
+    np.savez(tmp_path / "train_1.npz", **{k: v for k, v in np.load(tmp_path / "train_0.npz").items() if k != "teacher_val"})
+    for where in (str(tmp_path), "synthetic:4"):             # a shard without a teacher, no shards
+        with pytest.raises(ValueError):
+            TR.main(TR.get_args(["ds", where] + base[2:] + ["-s", str(tmp_path / "y"), "--distill_weight", "1"]))
