@@ -496,9 +496,12 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a->logits && a->idx && a->val, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->ld >= a->V && a->ld_idx >= a->k && a->ld_val >= a->k, STES_ERR_ARG, "stes_distill: rows overlap");
     STES_CHECK(!a->dlogits || a->ld_d >= a->V, STES_ERR_ARG, "stes_distill: rows of dlogits overlap");
-    STES_CHECK(a->dlogits != a->logits, STES_ERR_ARG, "stes_distill: dlogits must not be logits");
     STES_CHECK(!bwd || (a->stats && a->dlogits), STES_ERR_ARG, "stes_distill_bwd: stats and dlogits are needed");
     STES_CHECK(bwd || (a->ws && a->ws_floats >= stes_distill_ws_floats(a->M, a->V)), STES_ERR_ARG, "stes_distill: workspace too small");
+    const int64_t M = a->M;
+    const StesRows d{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, ins[4] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V},
+        {a->idx, a->idx_i64 ? 8 : 4, a->ld_idx, 0, M, 1, a->k}, {a->val, a->val_f32 ? 4 : 2, a->ld_val, 0, M, 1, a->k}, {a->weight, 4, M, 0, 1, 1, M}};
+    for (const StesRows& r : ins) STES_CHECK(!stes_share(d, r), STES_ERR_ARG, "stes_distill: dlogits shares memory with what the call reads");
     return STES_OK;
 }
 

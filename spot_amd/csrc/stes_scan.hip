@@ -549,6 +549,19 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
     STES_CHECK(!a->h_last || a->bs_hl >= a->H, STES_ERR_ARG, "stes_gated_scan: rows of h_last overlap");
     STES_CHECK(!(a->h_last && a->h_last == a->h0) || a->bs_h0 == a->bs_hl, STES_ERR_ARG, "stes_gated_scan: a state in place keeps its row stride");
     STES_CHECK(!bwd || !a->dh_last || a->bs_dhl == 0 || a->bs_dhl >= a->H, STES_ERR_ARG, "stes_gated_scan_bwd: rows of dh_last overlap");
+    const int64_t T = a->T, B = a->B, H = a->H, one = B > 1;
+    const int es = a->f32 ? 4 : 2;
+    const StesRows pre{a->pre, es, a->ld_pre, a->bs_pre, T, B, 2 * H}, h{a->h, es, a->ld_h, a->bs_h, T, B, H}, len{a->lengths, 4, 0, 1, 1, B, 1},
+        h0{a->h0, 4, 0, a->bs_h0, 1, a->bs_h0 ? B : 1, H}, last{a->h_last, 4, 0, a->bs_hl, 1, B, H}, states{a->states, 4, H, blocks_of(a->T) * H, blocks_of(a->T), B, H},
+        dh{a->dh, es, a->ld_dh, a->bs_dh, T, B, H}, dlast{a->dh_last, 4, 0, a->bs_dhl, 1, a->bs_dhl ? B : 1, H},
+        dpre{a->dpre, es, a->ld_dpre, a->bs_dpre, T, B, 2 * H}, dh0{a->dh0, 4, 0, H, 1, B, H}, total{a->dh0_sum, 4, 0, H, 1, 1, H};
+    const StesRows none{};
+    const StesRows outs[3] = {bwd ? dpre : h, bwd ? dh0 : last, bwd ? total : states}, ins[5] = {pre, len, bwd ? states : h0, bwd ? dh : none, bwd ? dlast : none};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 5; ++j)
+            STES_CHECK((i == 1 && j == 2 && !bwd && a->h_last == a->h0) || !stes_share(outs[i], ins[j]), STES_ERR_ARG, "stes_gated_scan: what a call writes shares memory with what it reads");
+        for (int j = 0; j < i; ++j) STES_CHECK(!stes_share(outs[i], outs[j]), STES_ERR_ARG, "stes_gated_scan: two results share memory");
+    }
     return STES_OK;
 }
 

@@ -130,7 +130,8 @@ def topk_distill_loss(logits, idx, val, temperature=1.0, weight=None, denom=None
 def topk_distill_grad(logits, idx, val, temperature=1.0, weight=None, denom=None, grad_scale=1.0, out=None, accumulate=False):
     """The loss of topk_distill_loss and grad_scale times its gradient in ONE pass over the logits, for training steps without autograd.
 
-    out         where the gradient goes: bfloat16 or float32 [..., V] (any row stride), None: a new tensor of the logits' type
+    out         where the gradient goes: bfloat16 or float32 [..., V] (any row stride), None: a new tensor of the logits' type; it shares
+                no memory with what the call reads
     accumulate  add to `out` instead of writing it
     -> (loss, gradient)"""
     s, idx, val, weight, temperature, denom = _check(logits, idx, val, weight, temperature, denom)
@@ -138,12 +139,16 @@ def topk_distill_grad(logits, idx, val, temperature=1.0, weight=None, denom=None
         if accumulate:
             _refuse("accumulate adds to out")
         out = torch.empty(logits.shape, dtype=logits.dtype, device=s.device)
-    elif out.device != s.device or out.dtype not in _ELEMENT or out.shape != logits.shape:
-        _refuse(f"out must be float32 or bfloat16 {list(logits.shape)} on {s.device}")
-    d = out if out.dim() == 2 else out.view(-1, out.shape[-1])
+    elif out.device != s.device or out.dtype not in _ELEMENT or out.shape != logits.shape or (out.requires_grad and torch.is_grad_enabled()):
+        _refuse(f"out must be float32 or bfloat16 {list(logits.shape)} on {s.device}, without gradients")
+    try:
+        d = out if out.dim() == 2 else out.view(-1, out.shape[-1])
+    except RuntimeError:
+        _refuse("rows of out must be one stride apart")
     if not d.is_contiguous() and ((d.shape[1] > 1 and d.stride(1) != 1) or (d.shape[0] > 1 and d.stride(0) < d.shape[1])):
         _refuse("rows of out must be contiguous and not overlap")
     with lib.on_device(s.device):
         loss = torch.empty((), dtype=torch.float32, device=s.device)
         _call("stes_distill", s, idx, val, weight, temperature, denom, float(grad_scale), loss=loss, d=d, accumulate=bool(accumulate))
+        lib.written(out)
     return loss, out

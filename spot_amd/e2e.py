@@ -295,9 +295,10 @@ class E2EModel(BaseRGBModel):
         n, hidden = (state[0].shape if len(state) else (0, 0))
         layers = self._model._pred_fine
         if (len(state) != layers.n_layers or hidden != layers.hidden_size or n < 1 or seq.shape[0] < 1 or seq.shape[0] % n
-                or any(s.shape != state[0].shape for s in state)):
+                or any(s.shape != state[0].shape or s.dtype != torch.float32 or not s.is_contiguous() for s in state)
+                or len({s.data_ptr() for s in state}) != len(state)):
             raise lib.StesError(f"predict_stream: {seq.shape[0]} clips and a state of {len(state)} layers {[tuple(s.shape) for s in state]} "
-                                "do not fit: clips are a multiple of the streams of new_stream()")
+                                "do not fit: clips are a multiple of the streams of new_stream(), states one float32 tensor a layer")
         if seq.device != torch.device(self.device) and str(seq.device) != str(self.device):
             seq = seq.to(self.device, non_blocking=True)
         if self._model.training:

@@ -1040,6 +1040,8 @@ class Engine:
         if distill is not None:
             # (the class gradient is rounded to bf16 between the two losses, as it is in front of every product that reads it)
             w, fw = float(distill.get("weight", 1.0)), distill.get("frame_weight")
+            if any(distill[t].numel() != N * distill[t].shape[-1] for t in ("idx", "val")):
+                raise lib.StesError(f"distill: idx and val hold {N} frames' classes, got {list(distill['idx'].shape)} and {list(distill['val'].shape)}")
             kd, _ = topk_distill_grad(self.logits.view(N, num_classes), distill["idx"].reshape(N, -1), distill["val"].reshape(N, -1),
                                       distill.get("temperature", 1.0), None if fw is None else fw.reshape(N), distill.get("denom"),
                                       grad_scale=w * grad_scale, out=dl[:, :num_classes], accumulate=True)

@@ -264,6 +264,14 @@ def on_device(dev):
     return _HERE_ALREADY if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
+def written(*tensors):
+    """Tells autograd of caller's tensors that a kernel has changed in place, as torch's own in-place functions do: a graph that
+    saved one of them refuses its backward pass."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def guard_leaves(node):
     """For the outputs' `grad_fn` of autograd functions that may be captured into a graph.  The node that accumulates a leaf's gradient
     keeps the stream on which it was made for as long as some autograd graph holds it; a backward pass that is captured while an

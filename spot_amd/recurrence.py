@@ -168,7 +168,8 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
     lengths  int32 [B] on the same device (values are clamped to [0, T]) or None: frames from a sequence's length on are not looked at,
              their h (and their gradients) are zero
     reverse  from a sequence's last frame to its first
-    out, state_out (without gradients only): where h [B, T, H] and the final states float32 [B, H] go; state_out may be h0
+    out, state_out (without gradients only): where h [B, T, H] and the final states float32 [B, H] go; state_out may be h0, apart
+             from that they share no memory with one another or with what the call reads (columns of one buffer do not)
     -> h [B, T, H] in pre's type and the states after the last step, float32 [B, H] (h0 where a sequence is empty)
 
     Differentiable (once) in pre and h0, from h and from the final states.  T = 0 and T = 1 are calls like any other."""
@@ -193,17 +194,15 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
     if out is not None:
         if wants_grad:
             _refuse("out and state_out are for calls without gradients")
-        if out.device != dev or out.dtype != pre.dtype or out.shape != (B, T, H):
-            _refuse(f"out must be {pre.dtype} [{B}, {T}, {H}] on {dev}")
+        if out.device != dev or out.dtype != pre.dtype or out.shape != (B, T, H) or (out.requires_grad and torch.is_grad_enabled()):
+            _refuse(f"out must be {pre.dtype} [{B}, {T}, {H}] on {dev}, without gradients")
         if (H > 1 and out.stride(2) != 1) or not _apart(out, H):
             _refuse("frames of out must be contiguous and not overlap")
-        if out.numel() and out.data_ptr() == pre.data_ptr():
-            _refuse("out must not be pre's memory")
     if state_out is not None:
         if wants_grad:
             _refuse("out and state_out are for calls without gradients")
-        if state_out.device != dev:
-            _refuse(f"state_out must be on {dev}")
+        if state_out.device != dev or (state_out.requires_grad and torch.is_grad_enabled()):
+            _refuse(f"state_out must be on {dev}, without gradients")
         stride = _row_stride(state_out, B, H, "state_out")
         if h0 is not None and state_out.data_ptr() == h0.data_ptr() and B > 1 and (h0.dim() == 1 or h0.stride(0) != stride):
             _refuse("a state in place is h0 itself, one row per sequence")
@@ -213,4 +212,5 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
             lib.guard_leaves(h.grad_fn)
         else:
             h, last, _ = _forward(pre, h0, lengths, bool(reverse), out, state_out, False)
+            lib.written(out, state_out)
     return h, last

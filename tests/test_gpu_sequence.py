@@ -151,6 +151,88 @@ def test_gated_scan_of_one_sequence_seen_several_times():
     _check(g[1], ref["dh0"], ref["dh0_err"], "dh0")
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,H", [(1, 16), (7, 5), (300, 40)])
+def test_gated_scan_in_columns_and_frames_of_one_buffer(T, H, dtype):
+    """The output beside the input in one buffer, in its columns or behind it in time, and states beside one another: as with memory of
+    their own; what would share memory is refused."""
+    from spot_amd import lib
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, _, _ = _scan_inputs(3, T, H, dtype, False, "rows", seed=T)
+    want = gated_scan(pre.cuda(), start.cuda())
+    buf = torch.full((3, T, 3 * H), NAN, dtype=dtype, device="cuda")
+    buf[..., :2 * H] = pre.cuda()
+    st = torch.full((3, 2 * H), NAN, device="cuda")
+    st[:, :H] = start.cuda()
+    h, last = gated_scan(buf[..., :2 * H], st[:, :H], out=buf[..., 2 * H:], state_out=st[:, H:])
+    assert torch.equal(h, want[0]) and torch.equal(last, want[1]) and torch.equal(buf[..., :2 * H], pre.cuda()) and torch.equal(st[:, :H], start.cuda())
+    long = torch.full((3, 2 * T, 2 * H), NAN, dtype=dtype, device="cuda")
+    long[:, :T] = pre.cuda()
+    h, _ = gated_scan(long[:, :T], st[:, :H], out=long[:, T:, :H])
+    assert torch.equal(h, want[0]) and torch.equal(long[:, :T], pre.cuda()) and bool(torch.isnan(long[:, T:, H:]).all())
+    x = buf[..., :2 * H]
+    for kw in (dict(out=x[..., :H]), dict(out=x[..., H:]), dict(out=buf[..., 2 * H - 1:3 * H - 1]), dict(out=long[:, T:, :H], pre=long[:, T:]),
+               dict(state_out=st[:, 1:H + 1]), dict(h0=st[0, :H], state_out=st[:, :H])):
+        with pytest.raises(lib.StesError):
+            gated_scan(kw.pop("pre", x), kw.pop("h0", st[:, :H]), **kw)
+
+
+def test_results_in_place_are_seen_by_autograd():
+    """A graph that saved what a call then overwrites refuses its backward pass, as with torch's own functions; results that ask for
+    gradients are refused."""
+    from spot_amd import lib
+    from spot_amd.distill import topk_distill_grad
+    from spot_amd.recurrence import gated_scan
+    pre, state = torch.zeros(2, 5, 8, device="cuda"), torch.ones(2, 4, device="cuda")
+    out = torch.zeros(2, 5, 4, device="cuda")
+    w = torch.ones(2, 4, device="cuda", requires_grad=True)
+    y = (w * state).sum()
+    gated_scan(pre, state, state_out=state)
+    with pytest.raises(RuntimeError):
+        y.backward()
+    v = torch.ones(2, 5, 4, device="cuda", requires_grad=True)
+    y = (v * out).sum()
+    gated_scan(pre, state, out=out)
+    with pytest.raises(RuntimeError):
+        y.backward()
+    s, i, t = torch.zeros(4, 7, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda"), torch.zeros(4, 2, device="cuda")
+    d, u = torch.zeros(4, 7, device="cuda"), torch.ones(4, 7, device="cuda", requires_grad=True)
+    y = (u * d).sum()
+    topk_distill_grad(s, i, t, out=d)
+    with pytest.raises(RuntimeError):
+        y.backward()
+    for kw in (dict(out=v), dict(state_out=w)):
+        with pytest.raises(lib.StesError):
+            gated_scan(pre, **kw)
+    with pytest.raises(lib.StesError):
+        topk_distill_grad(s, i, t, out=u)
+    with torch.inference_mode():
+        a, b = torch.zeros(2, 5, 4, device="cuda"), torch.zeros(2, 4, device="cuda")
+        gated_scan(pre, b, out=a, state_out=b)
+        topk_distill_grad(s, i, t, out=torch.zeros(4, 7, device="cuda"))
+    with torch.no_grad():
+        gated_scan(pre, out=v)
+
+
+@pytest.mark.parametrize("V", [7, 1000, 40000])
+def test_distill_gradient_beside_the_logits(V):
+    """The gradient in other columns of the logits' buffer; what would share memory, or has no single row stride, is refused."""
+    from spot_amd import lib
+    from spot_amd.distill import topk_distill_grad
+    s, idx, val, w = _kl_inputs(4, V, 3, F32, V, False, True)
+    c = (idx.cuda(), val.cuda(), 2.0, w.cuda())
+    want = topk_distill_grad(s.cuda(), *c)
+    buf = torch.full((4, 2 * V), NAN, device="cuda")
+    buf[:, :V] = s.cuda()
+    loss, d = topk_distill_grad(buf[:, :V], *c, out=buf[:, V:])
+    assert torch.equal(loss, want[0]) and torch.equal(buf[:, V:], want[1]) and torch.equal(buf[:, :V], s.cuda())
+    for out in (buf[:, :V], buf[:, V - 1:2 * V - 1], buf.view(torch.bfloat16)[:, :V]):
+        with pytest.raises(lib.StesError):
+            topk_distill_grad(buf[:, :V], *c, out=out)
+    with pytest.raises(lib.StesError):
+        topk_distill_grad(s.cuda().view(2, 2, V), idx.cuda().view(2, 2, 3), val.cuda().view(2, 2, 3), out=torch.zeros(2, 3, V, device="cuda")[:, :2])
+
+
 def test_gated_scan_clamps_lengths():
     from spot_amd.recurrence import gated_scan
     pre, start, _, _, _ = _scan_inputs(3, 140, 8, BF, False, "rows", seed=0)

@@ -120,7 +120,8 @@ def test_stream_refusals():
             m.predict_stream(_frames(4)[None], [])
     m = _model()
     x = _frames(12).view(3, 4, 3, 64, 64)
-    for state in ([], m.new_stream()[:2], m.new_stream(2), [s[:0] for s in m.new_stream()], [s[:, :5] for s in m.new_stream()]):
+    for state in ([], m.new_stream()[:2], m.new_stream(2), [s[:0] for s in m.new_stream()], [s[:, :5] for s in m.new_stream()],
+                  m.new_stream()[:1] * 3, [s.half() for s in m.new_stream()], m.new_stream()[:2] + [m.new_stream()[2].double()]):
         with pytest.raises(lib.StesError):
             m.predict_stream(x, state)
     with pytest.raises(lib.StesError):
@@ -146,6 +147,15 @@ def fixed_order():
         yield
     finally:
         lib.set_deterministic(False)
+
+
+def test_train_step_refuses_another_clips_teacher():
+    from spot_amd import lib
+    frame, label, xy, idx, val = _batch()
+    m = _model("rny008_tsm")
+    for i, v in ((idx[:1], val[:1]), (idx.repeat(1, 2, 1), val.repeat(1, 2, 1)), (idx, val[:, :2]), (idx[..., :0], val[..., :0])):
+        with pytest.raises(lib.StesError):
+            m.train_step(frame, label, xy, 0.0, optimizer_step=False, distill={"idx": i, "val": v})
 
 
 def test_train_step_with_a_teacher_matches_the_autograd_loop(fixed_order):

@@ -103,7 +103,7 @@ def _refused(entry, a):
 def _scan_args(**kw):
     from spot_amd import lib
     a = lib.GatedScanArgs()
-    base = dict(pre=256, ld_pre=16, bs_pre=64, h=256, ld_h=8, bs_h=32, h_last=256, bs_hl=8, states=256, dpre=256, ld_dpre=16, bs_dpre=64,
+    base = dict(pre=1 << 20, ld_pre=16, bs_pre=64, h=2 << 20, ld_h=8, bs_h=32, h_last=3 << 20, bs_hl=8, states=4 << 20, dpre=5 << 20, ld_dpre=16, bs_dpre=64,
                 ws=256, ws_bytes=1 << 40, B=2, T=4, H=8)
     for n, v in {**base, **kw}.items():
         setattr(a, n, v)
@@ -111,14 +111,20 @@ def _scan_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(B=-1), dict(T=-1), dict(H=-1), dict(f32=2), dict(pre=None), dict(h=None), dict(ld_pre=15), dict(ld_h=7), dict(bs_h=31), dict(bs_h=0),
-                                dict(bs_hl=7), dict(h0=512, bs_h0=3), dict(h0=256, bs_h0=0), dict(h0=256, bs_h0=9), dict(scrub=256, scrub_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, ws=264),
+                                dict(bs_hl=7), dict(h0=512, bs_h0=3), dict(h0=3 << 20, bs_h0=0), dict(h0=3 << 20, bs_h0=9),
+                                dict(h0=(3 << 20) + 4, bs_h0=8), dict(h0=(2 << 20) + 16, bs_h0=8), dict(h=(1 << 20) + 16), dict(h=(1 << 20) - 2), dict(h=(1 << 20) + 32, ld_h=16, bs_h=64, B=1, T=3, ld_pre=23),
+                                dict(h_last=(1 << 20) + 200), dict(h_last=(2 << 20) + 8), dict(states=(2 << 20)), dict(lengths=(3 << 20) + 4), dict(lengths=(2 << 20) - 4),
+                                dict(pre=1 << 20, h=(1 << 20) + 32, ld_pre=23, bs_pre=92, ld_h=23, bs_h=92), dict(pre=1 << 20, h=(1 << 20) + 34, ld_pre=24, bs_pre=96, ld_h=24, bs_h=96),
+                                dict(pre=1 << 20, h=(1 << 20) + 32, ld_pre=24, bs_pre=94, ld_h=24, bs_h=94), dict(scrub=256, scrub_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, ws=264),
                                 dict(T=1000, bs_pre=16000, bs_h=8000, ws_bytes=16), dict(T=1000, bs_pre=16000, bs_h=8000, scrub=256, scrub_bytes=8),
                                 dict(B=70000000, H=1 << 20), dict(B=1 << 23, T=1, H=64, ld_pre=128, bs_pre=128, bs_h=64, ld_h=64, bs_hl=64)])
 def test_scan_forward_refuses(kw):
     _refused("stes_gated_scan_fwd", _scan_args(**kw))
 
 
-@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256), dict(scrub=256, scrub_bytes=16)])
+@pytest.mark.parametrize("kw", [dict(states=None), dict(dpre=None), dict(ld_dpre=15), dict(bs_dpre=63), dict(dh=256, ld_dh=7), dict(dh0_sum=256), dict(scrub=256, scrub_bytes=16),
+                                dict(dpre=1 << 20), dict(dpre=(1 << 20) + 250), dict(dh=(5 << 20) + 16, ld_dh=8, bs_dh=32), dict(dh0=(4 << 20)), dict(dh0=(5 << 20) + 4),
+                                dict(dh0=6 << 20, dh0_sum=(6 << 20) + 32), dict(dh0=6 << 20, dh_last=6 << 20, bs_dhl=8)])
 def test_scan_backward_refuses(kw):
     _refused("stes_gated_scan_bwd", _scan_args(**kw))
 
@@ -126,7 +132,7 @@ def test_scan_backward_refuses(kw):
 def _distill_args(**kw):
     from spot_amd import lib
     a = lib.DistillArgs()
-    base = dict(logits=256, ld=7, idx=256, ld_idx=4, val=256, ld_val=4, M=3, V=7, k=4, temperature=1.0, denom=3.0, grad_scale=1.0, loss=256,
+    base = dict(logits=1 << 20, ld=7, idx=2 << 20, ld_idx=4, val=3 << 20, ld_val=4, M=3, V=7, k=4, temperature=1.0, denom=3.0, grad_scale=1.0, loss=256,
                 ws=256, ws_floats=1 << 40)
     for n, v in {**base, **kw}.items():
         setattr(a, n, v)
@@ -136,7 +142,8 @@ def _distill_args(**kw):
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(V=0), dict(k=0), dict(k=65, ld_idx=65, ld_val=65), dict(temperature=0.0), dict(temperature=-1.0),
                                 dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-7), dict(temperature=2e6), dict(denom=0.0), dict(denom=float("nan")),
                                 dict(logits=None), dict(idx=None), dict(val=None), dict(loss=None), dict(ld=6), dict(ld_idx=3), dict(ld_val=3),
-                                dict(dlogits=512, ld_d=6), dict(dlogits=256, ld_d=7), dict(M=1 << 22, V=1000, ld=1000), dict(ws_floats=0), dict(ws=None)])
+                                dict(dlogits=512, ld_d=6), dict(dlogits=1 << 20, ld_d=7), dict(dlogits=(1 << 20) + 40, ld_d=7), dict(dlogits=(1 << 20) - 2, ld_d=9), dict(dlogits=(2 << 20) + 47, ld_d=7),
+                                dict(dlogits=3 << 20, ld_d=7), dict(weight=(4 << 20) + 20, dlogits=4 << 20, ld_d=7), dict(ld=13, dlogits=(1 << 20) + 14, ld_d=13), dict(M=1 << 22, V=1000, ld=1000), dict(ws_floats=0), dict(ws=None)])
 def test_distill_refuses(kw):
     _refused("stes_distill", _distill_args(**kw))
 
