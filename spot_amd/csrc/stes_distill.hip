@@ -483,6 +483,17 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------- host
+// Up to 512 classes: as few lanes a row (4 to 64) as hold its list and, 16 classes a lane, its logits: a wave's instructions then serve the
+// most rows (131,072 x 300 bf16, 30 listed: loss 52 us with 16 classes a lane, 80 us with 8; 131,072 x 40 fp32: 13.0 and 13.9 us).
+int lanes_of(int V, int k) {
+    const int need = k > (V + 15) / 16 ? k : (V + 15) / 16;
+    int g = 4;
+    while (g < need) g *= 2;
+    return g;
+}
+// rows of up to 512 classes whose loss one workgroup computes in one launch
+int rows_at_once(int g) { return 4 * (1024 / g); }
+
 int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a, STES_ERR_ARG, "stes_distill: null pointer");
     STES_CHECK(a->M >= 0 && a->V >= 1 && a->k >= 1, STES_ERR_ARG, "stes_distill: M >= 0, V >= 1 and k >= 1");
@@ -497,7 +508,8 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a->ld >= a->V && a->ld_idx >= a->k && a->ld_val >= a->k, STES_ERR_ARG, "stes_distill: rows overlap");
     STES_CHECK(!a->dlogits || a->ld_d >= a->V, STES_ERR_ARG, "stes_distill: rows of dlogits overlap");
     STES_CHECK(!bwd || (a->stats && a->dlogits), STES_ERR_ARG, "stes_distill_bwd: stats and dlogits are needed");
-    STES_CHECK(bwd || (a->ws && a->ws_floats >= stes_distill_ws_floats(a->M, a->V)), STES_ERR_ARG, "stes_distill: workspace too small");
+    const int64_t need = bwd ? 0 : stes_distill_ws_floats(a->M, a->V, a->k);
+    STES_CHECK(!need || (a->ws && a->ws_floats >= need), STES_ERR_ARG, "stes_distill: workspace too small");
     const int64_t M = a->M;
     const StesRows d{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, ins[4] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V},
         {a->idx, a->idx_i64 ? 8 : 4, a->ld_idx, 0, M, 1, a->k}, {a->val, a->val_f32 ? 4 : 2, a->ld_val, 0, M, 1, a->k}, {a->weight, 4, M, 0, 1, 1, M}};
@@ -512,7 +524,7 @@ template <typename TS, typename TG, int G, int E, int MODE>
 int launch_short(const stes_distill_args& a, hipStream_t s) {
     // A loss of a few rounds of one large workgroup is done in one launch.  1,024 frames of 7 classes: 12 us on the GPU and 16 us a call
     // from Python; many workgroups and the launch that adds up what they leave: 5 + 4 us and 19 us a call.
-    if ((MODE & LOSS) && a.M <= 4 * (1024 / G)) {
+    if ((MODE & LOSS) && a.M <= rows_at_once(G)) {
         hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 1024, MODE>), dim3(1), dim3(1024), 0, s, a, (a.M + 1024 / G - 1) / (1024 / G), a.ws, loss_factor(a), grad_factor(a));
         return 1;
     }
@@ -555,13 +567,11 @@ int launch_rows(const stes_distill_args& a, hipStream_t s) {
 template <typename TS, typename TG, int MODE>
 int launch_mode(const stes_distill_args& a, hipStream_t s) {
     if (a.V <= 8 * 64) {
-        // As few lanes a row as hold its list and, 16 classes a lane, its logits: a wave's instructions then serve the most rows
-        // (131,072 x 300 bf16, 30 listed: loss 52 us with 16 classes a lane, 80 us with 8; 131,072 x 40 fp32: 13.0 and 13.9 us).
-        const int g = a.k > (a.V + 15) / 16 ? a.k : (a.V + 15) / 16;
-        if (g <= 4) return launch_group<TS, TG, 4, MODE>(a, s);
-        if (g <= 8) return launch_group<TS, TG, 8, MODE>(a, s);
-        if (g <= 16) return launch_group<TS, TG, 16, MODE>(a, s);
-        if (g <= 32) return launch_group<TS, TG, 32, MODE>(a, s);
+        const int g = lanes_of(a.V, a.k);
+        if (g == 4) return launch_group<TS, TG, 4, MODE>(a, s);
+        if (g == 8) return launch_group<TS, TG, 8, MODE>(a, s);
+        if (g == 16) return launch_group<TS, TG, 16, MODE>(a, s);
+        if (g == 32) return launch_group<TS, TG, 32, MODE>(a, s);
         return launch_short<TS, TG, 64, 8, MODE>(a, s);
     }
     if constexpr (sizeof(TS) == sizeof(TG)) {
@@ -582,9 +592,8 @@ int launch(const stes_distill_args& a, bool bwd, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int64_t stes_distill_ws_floats(int M, int V) {
-    (void)V;
-    return M > 0 ? M : 1;
+extern "C" int64_t stes_distill_ws_floats(int M, int V, int k) {
+    return M <= 0 || (V <= 8 * 64 && M <= rows_at_once(lanes_of(V, k))) ? 0 : M;
 }
 
 extern "C" int stes_distill(const stes_distill_args* a, void* stream) {

@@ -8,7 +8,6 @@ student's class distribution from the teacher's distribution over its k best cla
 """
 from __future__ import annotations
 
-import ctypes as C
 import functools
 import math
 
@@ -32,27 +31,28 @@ def _flat(t, n):
     return t
 
 
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 @functools.lru_cache(maxsize=256)
-def _ws_floats(M, V):
-    return lib.lib().stes_distill_ws_floats(M, V)
+def _ws_floats(M, V, k):
+    return lib.lib().stes_distill_ws_floats(M, V, k)
 
 
 def _call(entry, logits, idx, val, weight, temperature, denom, grad_scale=1.0, upstream=None, loss=None, stats=None, d=None, accumulate=False):
     """One call of the library; every tensor [M, ...] with contiguous rows."""
     M, V = logits.shape
-    ws = None if loss is None else torch.empty(_ws_floats(M, V), dtype=torch.float32, device=logits.device)   # (of this call's own)
-    a = lib.DistillArgs(
+    n = 0 if loss is None else _ws_floats(M, V, idx.shape[1])
+    ws = torch.empty(n, dtype=torch.float32, device=logits.device) if n else None          # (of this call's own)
+    lib.call(entry, lib.pack_distill(
         logits.data_ptr(), _ld(logits), _ELEMENT[logits.dtype], idx.data_ptr(), _ld(idx), idx.dtype == torch.int64,
-        val.data_ptr(), _ld(val), _ELEMENT[val.dtype], None if weight is None else weight.data_ptr(), M, V, idx.shape[1],
-        temperature, denom, grad_scale, None if upstream is None else upstream.data_ptr(),
-        None if loss is None else loss.data_ptr(), None if stats is None else stats.data_ptr(),
-        None if d is None else d.data_ptr(), 0 if d is None else _ld(d), 0 if d is None else _ELEMENT[d.dtype], accumulate,
-        None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-    lib.call(entry, C.byref(a))
+        val.data_ptr(), _ld(val), _ELEMENT[val.dtype], _at(weight), M, V, idx.shape[1], temperature, denom, grad_scale, _at(upstream),
+        _at(loss), _at(stats), _at(d), 0 if d is None else _ld(d), 0 if d is None else _ELEMENT[d.dtype], accumulate, _at(ws), n))
 
 
 class _Distill(torch.autograd.Function):

@@ -8,6 +8,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -26,6 +27,14 @@ _P, _I32, _I64, _F32, _F64, _U32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, 
 
 def _struct(name, fields):
     return type(name, (C.Structure,), {"_fields_": fields})
+
+
+def _packer(args):
+    """pack(value of every field, 0 for a null pointer) -> the bytes of such a struct, to be passed by address (a third of the time that it
+    takes to make the object, where a call takes 10 us)."""
+    s = struct.Struct("@" + "".join({_P: "P", _I64: "q", _I32: "i", _F32: "f", _F64: "d"}[t] for _, t in args._fields_) + "0q")
+    assert s.size == C.sizeof(args)
+    return s.pack
 
 
 GemmArgs = _struct("GemmArgs", [
@@ -107,6 +116,7 @@ GatedScanArgs = _struct("GatedScanArgs", [
     ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
     ("ws", _P), ("ws_bytes", _I64), ("ws_zero", _I32), ("scrub", _P), ("scrub_bytes", _I64),
     ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
+pack_scan = _packer(GatedScanArgs)
 SCAN_BLOCK = 256            # STES_SCAN_BLOCK in include/stes.h
 
 DistillArgs = _struct("DistillArgs", [
@@ -120,6 +130,7 @@ DistillArgs = _struct("DistillArgs", [
     ("loss", _P), ("stats", _P),
     ("dlogits", _P), ("ld_d", _I64), ("d_f32", _I32), ("accumulate", _I32),
     ("ws", _P), ("ws_floats", _I64)])
+pack_distill = _packer(DistillArgs)
 DISTILL_MAX_K = 64          # STES_DISTILL_MAX_K
 
 _SIGS = {
@@ -203,7 +214,7 @@ def lib():
         L.stes_augment_ws_floats.restype = C.c_int64
         L.stes_gated_scan_ws_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
         L.stes_gated_scan_ws_bytes.restype = C.c_int64
-        L.stes_distill_ws_floats.argtypes = [C.c_int, C.c_int]
+        L.stes_distill_ws_floats.argtypes = [C.c_int, C.c_int, C.c_int]
         L.stes_distill_ws_floats.restype = C.c_int64
         L.stes_gru_set_spin_limit.argtypes = [C.c_int]
         L.stes_gru_set_spin_limit.restype = C.c_int

@@ -7,7 +7,6 @@ videos, frame streams and ragged batches, differentiable (stes_gated_scan_fwd / 
 """
 from __future__ import annotations
 
-import ctypes as C
 import functools
 import threading
 
@@ -39,18 +38,16 @@ _KEPT_BYTES = 16 << 20              # larger workspaces are not kept: clearing t
 _kept = {}                          # (device, stream) -> _Workspaces
 
 
-def _call(entry, a, dev):
-    """One call of the library with the workspace that it needs.  A captured call gets one of its own, cleared in the graph: a
-    graph may be replayed on any stream, next to others."""
-    n = _ws_bytes(a.B, a.T, a.H)
+def _call(entry, fields, dims, dev):
+    """One call of the library with the workspace that it needs: `fields` are the arguments in front of it, `dims` those behind.  A
+    captured call gets a workspace of its own, cleared in the graph: a graph may be replayed on any stream, next to others."""
+    n = 0 if dims[1] <= lib.SCAN_BLOCK else _ws_bytes(*dims[:3])
     if not n:
-        lib.call(entry, C.byref(a))
+        lib.call(entry, lib.pack_scan(*fields, 0, 0, 0, 0, 0, *dims))
         return
-    a.ws_bytes = n
     if n > _KEPT_BYTES or torch.cuda.is_current_stream_capturing():
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        a.ws = ws.data_ptr()
-        lib.call(entry, C.byref(a))
+        lib.call(entry, lib.pack_scan(*fields, ws.data_ptr(), n, 0, 0, 0, *dims))
         return
     key = (dev.index, lib.stream())
     k = _kept.get(key)
@@ -60,15 +57,16 @@ def _call(entry, a, dev):
         if k.pair is None or k.pair[0].numel() < n:
             k.pair, k.turn, k.dirty = [torch.zeros(n, dtype=torch.uint8, device=dev) for _ in range(2)], 0, [0, 0]
         i, j = k.turn, 1 - k.turn
-        a.ws, a.ws_zero = k.pair[i].data_ptr(), 1
-        if k.dirty[j]:
-            a.scrub, a.scrub_bytes = k.pair[j].data_ptr(), k.dirty[j]
         try:
-            lib.call(entry, C.byref(a))
+            lib.call(entry, lib.pack_scan(*fields, k.pair[i].data_ptr(), n, 1, k.pair[j].data_ptr() if k.dirty[j] else 0, k.dirty[j], *dims))
         except Exception:
             k.pair = None
             raise
         k.dirty[i], k.dirty[j], k.turn = n, 0, j
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _row_stride(t, B, H, name):
@@ -105,15 +103,10 @@ def _forward(pre, h0, lengths, reverse, out, state_out, keep_states):
     states = torch.empty(B, -(-T // lib.SCAN_BLOCK), H, dtype=torch.float32, device=dev) if keep_states else None
     if B and H:
         ld, bs = _strides(pre, T, W)
-        ld_h, bs_h = _strides(h, T, H)
-        a = lib.GatedScanArgs(
-            pre.data_ptr(), ld, bs,
-            None if h0 is None else h0.data_ptr(), 0 if h0 is None or h0.dim() == 1 else _row_stride(h0, B, H, "h0"),
-            None if lengths is None else lengths.data_ptr(),
-            h.data_ptr(), ld_h, bs_h, last.data_ptr(), bs_hl, None if states is None else states.data_ptr(),
-            None, 0, 0, None, 0, None, 0, 0, None, None,
-            None, 0, 0, None, 0, B, T, H, _ELEMENT[pre.dtype], reverse)
-        _call("stes_gated_scan_fwd", a, dev)
+        ld_h, bs_h = (H, T * H) if out is None else _strides(h, T, H)
+        _call("stes_gated_scan_fwd", (
+            pre.data_ptr(), ld, bs, _at(h0), 0 if h0 is None or h0.dim() == 1 else _row_stride(h0, B, H, "h0"), _at(lengths),
+            h.data_ptr(), ld_h, bs_h, last.data_ptr(), bs_hl, _at(states), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), (B, T, H, _ELEMENT[pre.dtype], reverse), dev)
     return h, last, states
 
 
@@ -151,12 +144,9 @@ def _backward(pre, lengths, states, reverse, h0_dim, dh, dlast):
             ld_dh, bs_dh = _strides(dh, T, H)
         if dlast is not None:
             dlast = dlast.contiguous()
-        a = lib.GatedScanArgs(
-            pre.data_ptr(), ld, bs, None, 0, None if lengths is None else lengths.data_ptr(), None, 0, 0, None, 0, states.data_ptr(),
-            None if dh is None else dh.data_ptr(), ld_dh, bs_dh, None if dlast is None else dlast.data_ptr(), H,
-            dpre.data_ptr(), W, T * W, None if dh0 is None else dh0.data_ptr(), None if total is None else total.data_ptr(),
-            None, 0, 0, None, 0, B, T, H, _ELEMENT[pre.dtype], reverse)
-        _call("stes_gated_scan_bwd", a, dev)
+        _call("stes_gated_scan_bwd", (
+            pre.data_ptr(), ld, bs, 0, 0, _at(lengths), 0, 0, 0, 0, 0, states.data_ptr(), _at(dh), ld_dh, bs_dh, _at(dlast), H,
+            dpre.data_ptr(), W, T * W, _at(dh0), _at(total)), (B, T, H, _ELEMENT[pre.dtype], reverse), dev)
     return dpre, (total if h0_dim == 1 else dh0), None, None
 
 
@@ -179,7 +169,7 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
     H, dev = W // 2, pre.device
     if W % 2:
         _refuse(f"the last dimension of pre holds gates and candidates and is even, got {W}")
-    if (W > 1 and pre.stride(2) != 1) or (T > 1 and pre.stride(1) < W):
+    if not pre.is_contiguous() and ((W > 1 and pre.stride(2) != 1) or (T > 1 and pre.stride(1) < W)):
         _refuse("frames of pre must be contiguous and not overlap")
     if h0 is not None:
         if h0.device != dev or h0.dtype != torch.float32 or h0.shape not in ((B, H), (H,)):
