@@ -35,6 +35,7 @@ class _Workspaces:
 
 
 _KEPT_BYTES = 16 << 20              # larger workspaces are not kept: clearing them is a small part of such calls (2 % of the data)
+_KEPT_STREAMS = 64
 _kept = {}                          # (device, stream) -> _Workspaces
 
 
@@ -52,6 +53,8 @@ def _call(entry, fields, dims, dev):
     key = (dev.index, lib.stream())
     k = _kept.get(key)
     if k is None:
+        if len(_kept) >= _KEPT_STREAMS:
+            _kept.pop(next(iter(_kept)), None)                 # (its memory goes back in its stream's order)
         k = _kept.setdefault(key, _Workspaces())
     with k.lock:
         if k.pair is None or k.pair[0].numel() < n:
