@@ -5,17 +5,15 @@ raises, it never falls back to another implementation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
-import struct
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libstes_hip.so")
 
-_lib = None
+_lib = _native = None
 
 
 class StesError(RuntimeError):
@@ -27,14 +25,6 @@ _P, _I32, _I64, _F32, _F64, _U32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, 
 
 def _struct(name, fields):
     return type(name, (C.Structure,), {"_fields_": fields})
-
-
-def _packer(args):
-    """pack(value of every field, 0 for a null pointer) -> the bytes of such a struct, to be passed by address (a third of the time that it
-    takes to make the object, where a call takes 10 us)."""
-    s = struct.Struct("@" + "".join({_P: "P", _I64: "q", _I32: "i", _F32: "f", _F64: "d"}[t] for _, t in args._fields_) + "0q")
-    assert s.size == C.sizeof(args)
-    return s.pack
 
 
 GemmArgs = _struct("GemmArgs", [
@@ -116,7 +106,6 @@ GatedScanArgs = _struct("GatedScanArgs", [
     ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
     ("ws", _P), ("ws_bytes", _I64), ("ws_zero", _I32), ("scrub", _P), ("scrub_bytes", _I64),
     ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
-pack_scan = _packer(GatedScanArgs)
 SCAN_BLOCK = 256            # STES_SCAN_BLOCK in include/stes.h
 
 DistillArgs = _struct("DistillArgs", [
@@ -130,7 +119,6 @@ DistillArgs = _struct("DistillArgs", [
     ("loss", _P), ("stats", _P),
     ("dlogits", _P), ("ld_d", _I64), ("d_f32", _I32), ("accumulate", _I32),
     ("ws", _P), ("ws_floats", _I64)])
-pack_distill = _packer(DistillArgs)
 DISTILL_MAX_K = 64          # STES_DISTILL_MAX_K
 
 _SIGS = {
@@ -235,6 +223,29 @@ ERR_UNSUPPORTED = -3        # STES_ERR_UNSUPPORTED in include/stes.h
 _det_ticket = None
 
 
+def native():
+    """The compiled host side of the sequence operators (csrc/stes_torch.cpp): checks, workspaces, streams, autograd."""
+    global _native
+    if _native is None:
+        lib()
+        try:
+            from . import _stes_torch
+        except ImportError as e:
+            raise StesError("_stes_torch.so cannot be loaded: build it with `python -m spot_amd.build`; there is no fallback path") from e
+        _stes_torch.set_error(StesError)
+        _native = _stes_torch
+    return _native
+
+
+def native_call(kernel, fn, *args):
+    """A call of native(), timed as `kernel` where launches are."""
+    if TIMING is None:
+        return fn(*args)
+    out = []
+    _timed(kernel, None, 0, lambda: out.append(fn(*args)))
+    return out[0]
+
+
 def set_deterministic(on: bool):
     """The library's deterministic mode (stes_set_deterministic in include/stes.h): every cross-workgroup float sum is
     committed in a fixed order, so two runs of the same work give the same bits.  A test mode: slower, one stream."""
@@ -265,39 +276,6 @@ def check(rc: int, what: str):
 def stream():
     """The current stream of the current device, as the hipStream_t the library takes."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())       # (torch.cuda.current_stream() builds an object first: 2.6 us more)
-
-
-_HERE_ALREADY = contextlib.nullcontext()
-
-
-def on_device(dev):
-    """Makes `dev` the current device for a call on its tensors (nothing where it is: the usual case)."""
-    return _HERE_ALREADY if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
-
-
-def written(*tensors):
-    """Tells autograd of caller's tensors that a kernel has changed in place, as torch's own in-place functions do: a graph that
-    saved one of them refuses its backward pass."""
-    for t in tensors:
-        if t is not None and not t.is_inference():
-            torch.autograd.graph.increment_version(t)
-
-
-def guard_leaves(node):
-    """For the outputs' `grad_fn` of autograd functions that may be captured into a graph.  The node that accumulates a leaf's gradient
-    keeps the stream on which it was made for as long as some autograd graph holds it; a backward pass that is captured while an
-    eager graph of the same leaf lives would pull that stream into the capture, which ends the process.  Eager calls mark
-    their leaves' nodes, captured ones refuse marked nodes."""
-    for n, _ in node.next_functions:
-        for _ in range(4):                           # (through the views and copies that a call makes of a leaf)
-            if n is not None and len(n.next_functions) == 1:
-                n = n.next_functions[0][0]
-        if n is not None and not n.next_functions:
-            mark = n.metadata
-            if not torch.cuda.is_current_stream_capturing():
-                mark["stes_eager"] = True
-            elif "stes_eager" in mark:
-                raise StesError("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first")
 
 
 def ptr(t):

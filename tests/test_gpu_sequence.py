@@ -507,21 +507,24 @@ def test_gated_scan_calls_of_changing_sizes_share_a_stream():
     assert not bad
 
 
-def test_gated_scan_keeps_workspaces_of_few_streams(monkeypatch):
-    from spot_amd import recurrence
-    monkeypatch.setattr(recurrence, "_KEPT_STREAMS", 3)
-    monkeypatch.setattr(recurrence, "_kept", {})
+def test_gated_scan_keeps_workspaces_of_few_streams():
+    from spot_amd import lib
+    from spot_amd.recurrence import gated_scan
     pre, start, _, _, _ = _scan_inputs(2, 900, 96, BF, False, "rows", seed=8)
     p, s = pre.cuda(), start.cuda()
-    want = recurrence.gated_scan(p, s)
+    want = gated_scan(p, s)
     torch.cuda.synchronize()
     got = []
     streams = [torch.cuda.Stream() for _ in range(6)]
-    for _ in range(3):
-        for st in streams:
-            with torch.cuda.stream(st):
-                got.append(recurrence.gated_scan(p, s))
-    assert len(recurrence._kept) == 3
+    most = lib.native().keep_streams(3)
+    try:
+        for _ in range(12):
+            for st in streams:
+                with torch.cuda.stream(st):
+                    got.append(gated_scan(p, s))
+            assert lib.native().kept_streams() <= max(3, most)
+    finally:
+        lib.native().keep_streams(most)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
 
