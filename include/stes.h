@@ -511,8 +511,12 @@ int stes_loss(const float* logits, int64_t ldl, const float* loc, int64_t ldloc,
  * stes_distill: loss [1] and, when dlogits is given, the gradient in the same pass over the logits; stats [M][2] (optional):
  * the row's maximum and 1 / sum exp((logits - max) / tau), from which stes_distill_bwd computes the gradient later.
  * dlogits: fp32 (d_f32) or bf16, written, or added to when accumulate != 0; it must not overlap logits.  Columns from V up are
- * not touched.  ws: stes_distill_ws_floats(M, V, k) floats (0 for a few rows).  M = 0 is a call (loss 0).  Sums are taken in a fixed order. */
+ * not touched.  ws: stes_distill_ws_floats(M, V, k, zeros != NULL) floats.  zeros (optional): STES_DISTILL_WORDS
+ * zero words, which the call may use and leaves zero; it then needs one launch instead of two where its workgroups are few enough.  Calls that
+ * may overlap need other zeros each.  M = 0 is a call (loss 0).  Sums are taken in a fixed order (which
+ * may be another with dlogits than without). */
 #define STES_DISTILL_MAX_K 64
+#define STES_DISTILL_WORDS 8192
 typedef struct {
     const void* logits; int64_t ld; int32_t f32;
     const void* idx; int64_t ld_idx; int32_t idx_i64;
@@ -524,8 +528,9 @@ typedef struct {
     float* loss; float* stats;
     void* dlogits; int64_t ld_d; int32_t d_f32; int32_t accumulate;
     float* ws; int64_t ws_floats;
+    uint64_t* zeros;
 } stes_distill_args;
-int64_t stes_distill_ws_floats(int M, int V, int k);
+int64_t stes_distill_ws_floats(int M, int V, int k, int with_zeros);
 int stes_distill(const stes_distill_args* a, void* stream);
 int stes_distill_bwd(const stes_distill_args* a, void* stream);
 /* torch.optim.AdamW update over a flat fp32 range (model/common.py:40, step() :61-75). */

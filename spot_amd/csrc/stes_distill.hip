@@ -6,9 +6,9 @@
 // classes, k of V, are written over by the lanes that hold them.  Rows too long for a workgroup's registers are read twice (the
 // second time mostly from the cache).
 //
-// Measured (a copy of 1 GiB runs at 4,980 GB/s): loss and gradient in one pass of 8,192 x 32,003 bf16 206 us (5.1 TB/s); of
-// 2,048 x 50,001 fp32 loss 73 to 110 us and gradient 148 us (5.6 TB/s and, behind the gradient's writes, 3.7; 5.5 TB/s); 16,384 x 1,000
-// bf16 15 and 16 us (bound by the teacher's part of a row, some 200 instructions a wave, and its chain of loads: index, then logit);
+// Measured (a copy of 1 GiB runs at 4,980 GB/s): loss and gradient in one pass of 8,192 x 32,003 bf16 203 us (5.2 TB/s); of
+// 2,048 x 50,001 fp32 loss 72 to 110 us and gradient 148 us (5.6 TB/s and, behind the gradient's writes, 3.7; 5.5 TB/s); 16,384 x 1,000
+// bf16 15 and 15 us (bound by the teacher's part of a row, some 200 instructions a wave, and its chain of loads: index, then logit);
 // short rows are bound by instructions too: 131,072 x 300 bf16 loss 52 us, gradient 65 us.
 #include "stes_common.h"
 
@@ -178,10 +178,59 @@ __device__ __forceinline__ float row_factor(const stes_distill_args& p, float sc
 // A lane's part of KL / ln 2 = sum P (log2 P - log2 q), for a class of probability P and logit s; ls = log2(sum)
 __device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, float ct) { return P * (log2_(P) - ((s - mx) * ct - ls)); }
 
-// A workgroup's part of the loss; the only one of a launch is the loss.
-__device__ __forceinline__ void leave(const stes_distill_args& p, float* part, double sum, double factor) {
-    if (gridDim.x == 1) *p.loss = (float)(sum * factor);
-    else part[blockIdx.x] = (float)sum;
+constexpr int MAX_ROUNDS = 1 << 22;                  // (an exit for broken zeros: the loss becomes NaN)
+
+// A workgroup's part of the loss (`sum` is thread 0's); the only one of a launch is the loss.  With `p.zeros` the workgroups hand their
+// parts to the last one, which adds them up in an order of its own: words that are valid when they are not zero, in relaxed atomics of
+// agent scope, and it leaves them zero.  One workgroup waits and the others wait for nothing: every wait ends.  Without them, and from
+// 16 parts a thread on, where reading them one after the other takes longer than a launch, distill_sum_kernel adds up.  Loss and
+// gradient of 1,024 x 7 4.4 us (two launches 6.3, one workgroup in one launch 9.7), of 16,384 x 1,000 20.4 (21.1); loss of 30,000 x 600,
+// 7,500 parts for 256 threads, 23.8 (22.6).
+__host__ __device__ inline bool in_one_launch(const stes_distill_args& p, int blocks, int threads) {
+    return blocks == 1 || (p.zeros && blocks <= STES_DISTILL_WORDS && blocks <= 16 * threads);
+}
+
+template <int BLOCK>
+__device__ __forceinline__ void hand_over(const stes_distill_args& p, double sum, double factor, double* red) {
+    if (gridDim.x == 1 || !in_one_launch(p, gridDim.x, BLOCK)) {
+        if (threadIdx.x == 0) {
+            if (gridDim.x == 1) *p.loss = (float)(sum * factor);
+            else p.ws[blockIdx.x] = (float)sum;
+        }
+        return;
+    }
+    const int n = gridDim.x - 1;
+    if (blockIdx.x != n) {
+        if (threadIdx.x == 0) __hip_atomic_store(p.zeros + blockIdx.x, ((uint64_t)__float_as_uint((float)sum) << 32) | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return;
+    }
+    double s = threadIdx.x == 0 ? (double)(float)sum : 0.0;
+    for (int i = threadIdx.x; i < n; i += 4 * BLOCK) {
+        uint64_t w[4];
+        bool all = false;
+        for (int round = 0; !all && round < MAX_ROUNDS; ++round) {
+            if (round) __builtin_amdgcn_s_sleep(4);
+            all = true;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = i + u * BLOCK < n ? __hip_atomic_load(p.zeros + i + u * BLOCK, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 1u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) all = all && w[u] != 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            s += all ? (double)__uint_as_float((uint32_t)(w[u] >> 32)) : __builtin_nan("");
+            if (i + u * BLOCK < n) __hip_atomic_store(p.zeros + i + u * BLOCK, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int w = 0; w < BLOCK / 64; ++w) t += red[w];
+        *p.loss = (float)(t * factor);
+    }
 }
 
 enum { LOSS = 1, GRAD = 2, STATS_IN = 4 };           // what a launch does
@@ -205,7 +254,7 @@ template <typename TS, int G, int E> struct ShortRow {
 };
 
 template <typename TS, typename TG, int G, int E, int BLOCK, int MODE>
-__global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill_args p, int rounds, float* __restrict__ part, double factor, float scale) {
+__global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill_args p, int rounds, double factor, float scale) {
     constexpr int RPB = BLOCK / G;
     __shared__ double red[BLOCK / 64];
     __shared__ float target[MODE & GRAD ? BLOCK * E : 1];    // P of the rows at work, zero but for the listed classes
@@ -284,15 +333,15 @@ __global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill
         if (threadIdx.x == 0) {
             total = 0.0;
             for (int w = 0; w < BLOCK / 64; ++w) total += red[w];
-            leave(p, part, total, factor);
         }
+        hand_over<BLOCK>(p, total, factor, red);
     }
 }
 
 // ---------------------------------------------------------------- rows in registers
 // A team of TEAM threads holds a row: N vectors of 16 bytes a thread (W elements each), a few elements in front of the first 16-byte
 // boundary and behind the last one as single elements.  TEAM = 64: a wave per row, four rows a workgroup, no barrier.
-// STREAM: rows of any length, read again instead of held.
+// STREAM: rows of any length, read again instead of held.  Seven waves a SIMD for TEAM = 64: loss of 16,384 x 1,000 15.2 us, 16.4 with six.
 template <int TEAM> struct Team {
     static constexpr int WAVES = TEAM / 64;
     static __device__ __forceinline__ float max_(float v, float* red) {
@@ -338,17 +387,20 @@ __device__ __forceinline__ void walk(const VT* row, int i0, int n, F f) {
 }
 
 template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MODE>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(const stes_distill_args p, float* __restrict__ part, double factor, float scale) {
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM, TEAM == 64 ? 7 : 1) void distill_row_kernel(const stes_distill_args p, double factor, float scale) {
     typedef typename Vec<TS, W>::type VS;
     typedef typename Vec<TG, W>::type VG;
     typedef Team<TEAM> Tm;
-    __shared__ float red[TEAM / 64 > 4 ? TEAM / 64 : 4];
-    constexpr int RPB = TEAM == 64 ? 4 : 1;
+    constexpr int RPB = TEAM == 64 ? 4 : 1, BLOCK = TEAM * RPB;
+    __shared__ float red[BLOCK / 64];
+    __shared__ double parts[BLOCK / 64];
     const int lane = threadIdx.x & 63, i0 = threadIdx.x % TEAM;
     const long m = (long)blockIdx.x * RPB + threadIdx.x / TEAM;
     const bool row = m < p.M;
     float out = 0.f;
     if (row) {
+        // (the list first: 8,192 x 32,003 bf16, 32 listed: loss 108 to 105 us, gradient 207 to 201, both 207 to 203.5)
+        const Listed listed = load_listed(p, m, true, lane);
         const TS* s = (const TS*)p.logits + m * p.ld;
         const float ct = LOG2E / p.temperature;
         const float w = p.weight ? p.weight[m] : 1.f;
@@ -366,8 +418,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
             for (int i = 0; i < N; ++i)
                 if (i * TEAM + i0 < nv) x[i] = sv[i * TEAM + i0];
         }
-        const Entry t = teacher_row<64>(p, load_listed(p, m, true, lane), lane, lane, ct, threadIdx.x % TEAM < 64);
-        const float st = t.at >= 0 ? (float)s[t.at] : 0.f;
+        float st = 0.f;                                      // (asked for ahead of the work on the list)
+        if (threadIdx.x % TEAM < 64 && listed.at >= 0 && listed.at < p.V) st = (float)s[listed.at];
+        const Entry t = teacher_row<64>(p, listed, lane, lane, ct, threadIdx.x % TEAM < 64);
         const bool counts = t.some && w != 0.f;
         float mx = 0.f, sum = 1.f;
         if (MODE & STATS_IN) { mx = p.stats[2 * m]; sum = p.stats[2 * m + 1]; }
@@ -461,8 +514,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void distill_row_kernel(co
         if (TEAM == 64) {
             if (lane == 0) red[threadIdx.x >> 6] = out;
             __syncthreads();
-            if (threadIdx.x == 0) leave(p, part, (red[0] + red[1]) + (red[2] + red[3]), factor);
-        } else if (threadIdx.x == 0) leave(p, part, out, factor);
+            out = (red[0] + red[1]) + (red[2] + red[3]);
+        }
+        hand_over<BLOCK>(p, out, factor, parts);
     }
 }
 
@@ -491,8 +545,12 @@ int lanes_of(int V, int k) {
     while (g < need) g *= 2;
     return g;
 }
-// rows of up to 512 classes whose loss one workgroup computes in one launch
-int rows_at_once(int g) { return 4 * (1024 / g); }
+// workgroups of a launch over rows of up to 512 classes, and the rounds of each
+int short_rounds(int M, int rows) { return (int)((((long)M + rows - 1) / rows + 2047) / 2048); }
+int short_blocks(int M, int rows) {
+    const long teams = ((long)M + rows - 1) / rows, rounds = short_rounds(M, rows);
+    return (int)((teams + rounds - 1) / rounds);
+}
 
 int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a, STES_ERR_ARG, "stes_distill: null pointer");
@@ -508,7 +566,8 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(a->ld >= a->V && a->ld_idx >= a->k && a->ld_val >= a->k, STES_ERR_ARG, "stes_distill: rows overlap");
     STES_CHECK(!a->dlogits || a->ld_d >= a->V, STES_ERR_ARG, "stes_distill: rows of dlogits overlap");
     STES_CHECK(!bwd || (a->stats && a->dlogits), STES_ERR_ARG, "stes_distill_bwd: stats and dlogits are needed");
-    const int64_t need = bwd ? 0 : stes_distill_ws_floats(a->M, a->V, a->k);
+    STES_CHECK((uintptr_t)a->zeros % 8 == 0, STES_ERR_ARG, "stes_distill: zeros is aligned to 8 bytes");
+    const int64_t need = bwd ? 0 : stes_distill_ws_floats(a->M, a->V, a->k, a->zeros != nullptr);
     STES_CHECK(!need || (a->ws && a->ws_floats >= need), STES_ERR_ARG, "stes_distill: workspace too small");
     const int64_t M = a->M;
     const StesRows d{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, ins[4] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V},
@@ -522,17 +581,9 @@ float grad_factor(const stes_distill_args& a) { return (float)((double)a.grad_sc
 
 template <typename TS, typename TG, int G, int E, int MODE>
 int launch_short(const stes_distill_args& a, hipStream_t s) {
-    // A loss of a few rounds of one large workgroup is done in one launch.  1,024 frames of 7 classes: 12 us on the GPU and 16 us a call
-    // from Python; many workgroups and the launch that adds up what they leave: 5 + 4 us and 19 us a call.
-    if ((MODE & LOSS) && a.M <= rows_at_once(G)) {
-        hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 1024, MODE>), dim3(1), dim3(1024), 0, s, a, (a.M + 1024 / G - 1) / (1024 / G), a.ws, loss_factor(a), grad_factor(a));
-        return 1;
-    }
-    constexpr int RPB = 256 / G;
-    const long teams = ((long)a.M + RPB - 1) / RPB;
-    const int rounds = (int)((teams + 2047) / 2048), blocks = (int)((teams + rounds - 1) / rounds);
-    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 256, MODE>), dim3(blocks), dim3(256), 0, s, a, rounds, a.ws, loss_factor(a), grad_factor(a));
-    return blocks;
+    const int blocks = short_blocks(a.M, 256 / G);
+    hipLaunchKernelGGL((distill_short_kernel<TS, TG, G, E, 256, MODE>), dim3(blocks), dim3(256), 0, s, a, short_rounds(a.M, 256 / G), loss_factor(a), grad_factor(a));
+    return in_one_launch(a, blocks, 256) ? 0 : blocks;
 }
 
 template <typename TS, typename TG, int G, int MODE>
@@ -544,11 +595,11 @@ template <typename TS, typename TG, int W, int TEAM, int N, bool STREAM, int MOD
 int launch_row(const stes_distill_args& a, hipStream_t s) {
     constexpr int RPB = TEAM == 64 ? 4 : 1;
     const int blocks = (int)(((long)a.M + RPB - 1) / RPB);
-    hipLaunchKernelGGL((distill_row_kernel<TS, TG, W, TEAM, N, STREAM, MODE>), dim3(blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, s, a, a.ws, loss_factor(a), grad_factor(a));
-    return blocks;
+    hipLaunchKernelGGL((distill_row_kernel<TS, TG, W, TEAM, N, STREAM, MODE>), dim3(blocks), dim3(TEAM * RPB), 0, s, a, loss_factor(a), grad_factor(a));
+    return in_one_launch(a, blocks, TEAM * RPB) ? 0 : blocks;
 }
 
-// -> how many partial sums the launch leaves
+// -> how many partial sums the launch leaves in the workspace
 template <typename TS, typename TG, int W, int MODE>
 int launch_rows(const stes_distill_args& a, hipStream_t s) {
     if constexpr (W == 1) {
@@ -592,8 +643,10 @@ int launch(const stes_distill_args& a, bool bwd, hipStream_t s) {
 
 }  // namespace
 
-extern "C" int64_t stes_distill_ws_floats(int M, int V, int k) {
-    return M <= 0 || (V <= 8 * 64 && M <= rows_at_once(lanes_of(V, k))) ? 0 : M;
+extern "C" int64_t stes_distill_ws_floats(int M, int V, int k, int with_zeros) {
+    if (M <= 1) return 0;
+    const int blocks = V <= 8 * 64 ? short_blocks(M, 256 / lanes_of(V, k)) : M;          // (or fewer)
+    return blocks == 1 || (with_zeros && blocks <= 16 * 256) ? 0 : blocks;
 }
 
 extern "C" int stes_distill(const stes_distill_args* a, void* stream) {
@@ -604,7 +657,7 @@ extern "C" int stes_distill(const stes_distill_args* a, void* stream) {
         parts = a->f32 ? launch<float>(*a, false, (hipStream_t)stream) : launch<bf16>(*a, false, (hipStream_t)stream);
         STES_LAUNCH_CHECK();
     }
-    if (parts != 1) {                                        // (no rows: a sum of nothing)
+    if (parts || !a->M) {                                    // (no rows: a sum of nothing)
         hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a->ws, parts, loss_factor(*a), a->loss);
         STES_LAUNCH_CHECK();
     }

@@ -121,14 +121,15 @@ variable_list once(variable_list&& grads, const char* what) {
     return std::move(grads);
 }
 
-// ---------------------------------------------------------------- the scan's workspaces
-// The two workspaces that the calls on one stream take in turn: a call finds its own zero and leaves the one of the call before zero,
+// ---------------------------------------------------------------- kept workspaces
+// The two workspaces that the scan's calls on one stream take in turn: a call finds its own zero and leaves the one of the call before zero,
 // so none needs a launch that clears.  A call's launch happens under the lock: what is clean follows the stream's order.
 struct Kept {
     std::mutex lock;
     Tensor pair[2];
     int turn = 0;
     int64_t dirty[2] = {0, 0};
+    Tensor zeros;                           // of the distillation's calls, which leave it zero
 };
 constexpr int64_t KEPT_BYTES = 16 << 20;    // larger workspaces are not kept: clearing them is a small part of such calls (2 % of the data)
 struct Streams {
@@ -376,12 +377,20 @@ void into(stes_distill_args& a, const Tensor& d) { a.dlogits = d.data_ptr(), a.l
 // loss, and whatever else `a` asks for
 Tensor distill_call(stes_distill_args& a, const Tensor& logits) {
     const Tensor loss = fresh({}, logits, at::kFloat);
-    const int64_t n = stes_distill_ws_floats(a.M, a.V, a.k);
+    void* s = stream_of(logits.device());
+    a.loss = static_cast<float*>(loss.data_ptr());
+    std::shared_ptr<Kept> k;
+    if (a.M > 1 && !capturing()) {          // (a graph may be replayed on any stream, next to others)
+        k = kept(logits.device().index(), s);
+        std::lock_guard<std::mutex> g(k->lock);
+        if (!k->zeros.defined()) k->zeros = at::zeros({STES_DISTILL_WORDS}, logits.options().dtype(at::kLong));
+        a.zeros = static_cast<uint64_t*>(k->zeros.data_ptr());
+    }
+    const int64_t n = stes_distill_ws_floats(a.M, a.V, a.k, a.zeros != nullptr);
     Tensor ws;                              // (of this call's own)
     if (n) ws = fresh({n}, logits, at::kFloat);
-    a.loss = static_cast<float*>(loss.data_ptr());
     a.ws = at_<float>(ws), a.ws_floats = n;
-    check(stes_distill(&a, stream_of(logits.device())), "stes_distill");
+    check(stes_distill(&a, s), "stes_distill");
     return loss;
 }
 

@@ -118,7 +118,7 @@ DistillArgs = _struct("DistillArgs", [
     ("grad_scale", _F32), ("upstream", _P),
     ("loss", _P), ("stats", _P),
     ("dlogits", _P), ("ld_d", _I64), ("d_f32", _I32), ("accumulate", _I32),
-    ("ws", _P), ("ws_floats", _I64)])
+    ("ws", _P), ("ws_floats", _I64), ("zeros", _P)])
 DISTILL_MAX_K = 64          # STES_DISTILL_MAX_K
 
 _SIGS = {
@@ -202,7 +202,7 @@ def lib():
         L.stes_augment_ws_floats.restype = C.c_int64
         L.stes_gated_scan_ws_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
         L.stes_gated_scan_ws_bytes.restype = C.c_int64
-        L.stes_distill_ws_floats.argtypes = [C.c_int, C.c_int, C.c_int]
+        L.stes_distill_ws_floats.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
         L.stes_distill_ws_floats.restype = C.c_int64
         L.stes_gru_set_spin_limit.argtypes = [C.c_int]
         L.stes_gru_set_spin_limit.restype = C.c_int

@@ -819,6 +819,29 @@ def test_distill_one_row_and_views(V):
     _check(g, total, ref["dlogits_err"].sum(0, keepdims=True) + 4 * SO.U * np.abs(ref["dlogits"]).sum(0, keepdims=True), "expanded")
 
 
+def test_distill_calls_of_changing_sizes_share_a_stream():
+    """Calls with few and many workgroups one after the other, on two streams at once: each finds the words clean through which
+    workgroups hand over their sums."""
+    from spot_amd.distill import topk_distill_grad, topk_distill_loss
+    cases = []
+    for M, V, k in ((1024, 7, 4), (1, 7, 4), (3, 20000, 5), (5000, 600, 3), (20000, 530, 2), (70, 300, 64), (1024, 7, 4), (300, 4000, 16), (2000, 2, 1)):
+        s, idx, val, _ = _kl_inputs(M, V, k, BF, M + V)
+        ref = SO.topk_distill(_np(s), _np(idx), _np(val), 2.0)
+        cases.append((s.cuda(), idx.cuda(), val.cuda(), ref))
+    got, order = [], np.random.default_rng(0).integers(0, len(cases), 60)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in order:
+        s, idx, val, _ = cases[i]
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append((i, topk_distill_loss(s, idx, val, 2.0), topk_distill_grad(s, idx, val, 2.0)[0]))
+    torch.cuda.synchronize()
+    for i, a, b in got:
+        _check(a, cases[i][3]["loss"], cases[i][3]["loss_err"], "loss")
+        assert torch.equal(a, b)
+
+
 def test_distill_gradient_against_differences():
     from spot_amd.distill import topk_distill_loss
     s, idx, val, w = _kl_inputs(64, 40, 6, F32, 3, True, True)

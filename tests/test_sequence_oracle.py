@@ -144,7 +144,8 @@ def _distill_args(**kw):
                                 dict(logits=None), dict(idx=None), dict(val=None), dict(loss=None), dict(ld=6), dict(ld_idx=3), dict(ld_val=3),
                                 dict(dlogits=512, ld_d=6), dict(dlogits=1 << 20, ld_d=7), dict(dlogits=(1 << 20) + 40, ld_d=7), dict(dlogits=(1 << 20) - 2, ld_d=9), dict(dlogits=(2 << 20) + 47, ld_d=7),
                                 dict(dlogits=3 << 20, ld_d=7), dict(weight=(4 << 20) + 20, dlogits=4 << 20, ld_d=7), dict(ld=13, dlogits=(1 << 20) + 14, ld_d=13), dict(M=1 << 22, V=1000, ld=1000),
-                                dict(M=1000, V=1000, ld=1000, ws_floats=999), dict(M=100, V=1000, ld=1000, ws=None), dict(M=3000, k=4, ws_floats=2999)])
+                                dict(M=1000, V=1000, ld=1000, ws_floats=999), dict(M=100, V=1000, ld=1000, ws=None), dict(M=3000, ws_floats=46), dict(M=100, V=1000, ld=1000, zeros=1 << 25, ws=None, stats=None, loss=None), dict(zeros=(1 << 25) + 4),
+                                dict(M=4097, V=1000, ld=1000, zeros=1 << 25, ws_floats=4096)])
 def test_distill_refuses(kw):
     _refused("stes_distill", _distill_args(**kw))
 
