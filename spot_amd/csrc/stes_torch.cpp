@@ -71,6 +71,8 @@ int f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 void written(const Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// (forward-mode tangents would be lost without a word)
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
 bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---------------------------------------------------------------- leaves
@@ -110,13 +112,16 @@ torch::autograd::edge_list guarded(torch::autograd::edge_list edges) {
     return edges;
 }
 
-// Gradients that cannot be differentiated again: they say so where somebody tries.
-variable_list once(variable_list&& grads, const char* what) {
+// Gradients that cannot be differentiated again: they depend on what `node` depends on and on the gradients that came in, through a node
+// that says so where somebody tries.
+variable_list once(variable_list&& grads, const Node& node, const variable_list& came, const char* what) {
     if (!at::GradMode::is_enabled()) return std::move(grads);
     for (Tensor& g : grads)
         if (g.defined()) {
-            auto end = std::make_shared<torch::autograd::DelayedError>(c10::str(what, " is differentiable once"), 1);
-            g = (*end)({g.detach().set_requires_grad(true)})[0];
+            torch::autograd::edge_list edges = torch::autograd::collect_next_edges(came);
+            edges.insert(edges.end(), node.next_edges().begin(), node.next_edges().end());
+            std::shared_ptr<Node> end(new torch::autograd::Error(c10::str(what, " is differentiable once"), std::move(edges)), torch::autograd::deleteNode);
+            torch::autograd::set_history(g, end);
         }
     return std::move(grads);
 }
@@ -272,7 +277,7 @@ struct GatedScanBackward : public Node {
                 scan_call(stes_gated_scan_bwd, "stes_gated_scan_bwd", a, p.device());
             }
         }
-        return once({dpre, h0_dim == 1 ? total : dh0}, "gated_scan");
+        return once({dpre, h0_dim == 1 ? total : dh0}, *this, grads, "gated_scan");
     }
 };
 
@@ -305,6 +310,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
     }
     if (lengths.defined() && (lengths.device() != dev || lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B || !lengths.is_contiguous()))
         refuse(SCAN, "lengths must be contiguous int32 [", B, "] on ", dev, ", got ", lengths.scalar_type(), " ", lengths.sizes(), " on ", lengths.device());
+    if (has_tangent(pre) || (h0.defined() && has_tangent(h0))) refuse(SCAN, "no forward-mode derivatives");
     const bool grad = asks_for_gradients(pre) || (h0.defined() && asks_for_gradients(h0));
     if (grad && (out.defined() || state_out.defined())) refuse(SCAN, "out and state_out are for calls without gradients");
     if (out.defined()) {
@@ -408,6 +414,7 @@ Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, d
     Tensor weight = weight_.value_or(Tensor());
     if (weight.defined() && (weight.device() != dev || weight.scalar_type() != at::kFloat || weight.sizes() != lead)) refuse(KL, "weight must be float32 ", lead, " on ", dev);
     if (asks_for_gradients(val) || (weight.defined() && asks_for_gradients(weight))) refuse(KL, "the teacher's logits and the weights are constants: detach them");
+    if (has_tangent(logits) || has_tangent(val) || (weight.defined() && has_tangent(weight))) refuse(KL, "no forward-mode derivatives");
     if (!(temperature >= 1e-6 && temperature <= 1e6)) refuse(KL, "the temperature lies between 1e-6 and 1e6, got ", temperature);
     Rows r{flat(logits, V), flat(idx, k), flat(val, k), Tensor(), temperature, 0.0};
     if (std::max(r.logits.size(0), V) > INT32_MAX) refuse(KL, "sizes beyond 32 bits: ", logits.sizes());
@@ -442,7 +449,7 @@ struct DistillBackward : public Node {
                 check(stes_distill_bwd(&a, stream_of(r.logits.device())), "stes_distill_bwd");
             }
         }
-        return once({d}, "topk_distill_loss");
+        return once({d}, *this, grads, "topk_distill_loss");
     }
 };
 

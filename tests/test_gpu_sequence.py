@@ -3,6 +3,7 @@ the running error bounds that the oracle derives from the inputs, plus half a st
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import sequence_oracle as SO
 
@@ -563,6 +564,101 @@ def test_gated_scan_in_graphs(T):
             torch.cuda.synchronize()
             for a, b in zip(out, want):
                 assert torch.equal(a, b)
+
+
+def _differentiable_calls():
+    """(leaf, call of it) for both operators, with kept statistics and, for the scan, joined blocks."""
+    from spot_amd.distill import topk_distill_loss
+    from spot_amd.recurrence import gated_scan
+    p = torch.randn(2, 300, 16, device="cuda", requires_grad=True)
+    x = torch.randn(9, 50, device="cuda", requires_grad=True)
+    val, idx = torch.randn(9, 50, device="cuda").topk(3)
+    n = torch.tensor([300, 17], dtype=torch.int32, device="cuda")
+    return [(p, lambda t: gated_scan(t, lengths=n)[0].square().sum()), (x, lambda t: topk_distill_loss(t, idx, val, 2.0))]
+
+
+def test_gradients_behave_as_torchs_own_functions_do():
+    """Kept graphs, graphs used up, inputs changed in between, tensors saved elsewhere, recomputation, gradients that accumulate, hooks,
+    anomaly mode, no second derivative and no tangents, and no memory that stays."""
+    from spot_amd import lib
+    for leaf, f in _differentiable_calls():
+        want, = torch.autograd.grad(f(leaf), leaf)
+        y = f(leaf)
+        a, = torch.autograd.grad(y, leaf, retain_graph=True)
+        b, = torch.autograd.grad(y, leaf)
+        assert torch.equal(a, want) and torch.equal(b, want)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf)
+        c = leaf.detach().clone().requires_grad_()
+        d = c * 1.0
+        y = f(d)
+        d.data.add_(0)                                      # (not seen by autograd, and it changes nothing)
+        torch.autograd.grad(y, c, retain_graph=True)
+        with torch.no_grad():
+            d.add_(1.0)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, c)
+        with torch.autograd.graph.save_on_cpu():
+            y = f(leaf)
+        assert torch.equal(torch.autograd.grad(y, leaf)[0], want)
+        again = torch.utils.checkpoint.checkpoint(f, leaf, use_reentrant=False)
+        assert torch.equal(torch.autograd.grad(again, leaf)[0], want)
+        seen = []
+        with torch.autograd.set_detect_anomaly(True):
+            y = f(leaf)
+            y.register_hook(lambda g: seen.append(g) or 2 * g)
+            y.backward()
+            f(leaf).backward()
+        assert len(seen) == 1
+        _check(leaf.grad, 3 * _np(want), 8 * SO.U * np.abs(_np(want)), "accumulated")
+        g, = torch.autograd.grad(f(leaf), leaf, create_graph=True)
+        _check(g, _np(want), 0 * np.abs(_np(want)), "create_graph")
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad((g * leaf).sum(), leaf)
+        y = f(leaf)
+        up = torch.ones_like(y, requires_grad=True)
+        g, = torch.autograd.grad(y, leaf, up, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad((g * leaf * up).sum(), up)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(lib.StesError):
+                f(torch.autograd.forward_ad.make_dual(leaf.detach(), torch.ones_like(leaf)))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(leaf.detach())
+        with pytest.raises(RuntimeError):
+            torch.vmap(f)(torch.stack([leaf.detach()] * 2))
+        leaf.grad = None
+        torch.cuda.synchronize()
+        del y, again, g, a, b, c, d, seen
+        f(leaf)
+        before = torch.cuda.memory_allocated()
+        for i in range(50):
+            y = f(leaf)
+            if i % 2:
+                torch.autograd.grad(y, leaf)
+            del y
+        assert torch.cuda.memory_allocated() == before
+
+
+def test_backward_passes_from_several_threads():
+    import threading
+    for leaf, f in _differentiable_calls():
+        want, = torch.autograd.grad(f(leaf), leaf)
+        torch.cuda.synchronize()
+        got = []
+
+        def work():
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got.append(torch.autograd.grad(f(leaf), leaf)[0])
+                torch.cuda.current_stream().synchronize()
+        threads = [threading.Thread(target=work) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(60)
+        torch.cuda.synchronize()
+        assert len(got) == 80 and all(torch.equal(g, want) for g in got)
 
 
 def test_capture_refuses_leaves_that_an_eager_graph_holds():
