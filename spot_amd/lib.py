@@ -106,7 +106,6 @@ GatedScanArgs = _struct("GatedScanArgs", [
     ("dpre", _P), ("ld_dpre", _I64), ("bs_dpre", _I64), ("dh0", _P), ("dh0_sum", _P),
     ("ws", _P), ("ws_bytes", _I64), ("ws_zero", _I32), ("scrub", _P), ("scrub_bytes", _I64),
     ("B", _I32), ("T", _I32), ("H", _I32), ("f32", _I32), ("reverse", _I32)])
-SCAN_BLOCK = 256            # STES_SCAN_BLOCK in include/stes.h
 
 DistillArgs = _struct("DistillArgs", [
     ("logits", _P), ("ld", _I64), ("f32", _I32),
@@ -119,7 +118,6 @@ DistillArgs = _struct("DistillArgs", [
     ("loss", _P), ("stats", _P),
     ("dlogits", _P), ("ld_d", _I64), ("d_f32", _I32), ("accumulate", _I32),
     ("ws", _P), ("ws_floats", _I64), ("zeros", _P)])
-DISTILL_MAX_K = 64          # STES_DISTILL_MAX_K
 
 _SIGS = {
     "stes_gated_scan_fwd": [_P, _P],
