@@ -21,7 +21,9 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, dh=None, dlast=None, n
     and a product (u): under (|x| + 8) u relative, z and a alike.  A state is a sum of terms (product of a's) z c; a term from i steps
     back has met i gates with their errors and at most 3 roundings a step, whatever the association of the time axis, and a
     composition in a tree, in blocks and across workgroups adds fewer than 24 more.  With S the sum of the terms' magnitudes that is
-    R_t = a_t (R_{t-1} + (|x| + 12) u S_{t-1}) + (|x| + 12) u z|c|,  S_t = a_t S_{t-1} + z|c|,  bound R_t + 24 u S_t."""
+    R_t = a_t (R_{t-1} + (|x| + 12) u S_{t-1}) + (|x| + 12) u z|c|,  S_t = a_t S_{t-1} + z|c|,  bound R_t + 24 u S_t.
+    |x| counts as 104 at most: sigmoid(-104) is below half of the least fp32 number, and a gate beyond is 0 or 1 however its argument was
+    rounded."""
     pre = np.asarray(pre, np.float64)
     B, T, W = pre.shape
     H = W // 2
@@ -41,7 +43,7 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, dh=None, dlast=None, n
         for t in order:
             g, c = pre[b, t, :H], pre[b, t, H:]
             z, a = _sigmoid(g), _sigmoid(-g)
-            e = (np.abs(g) + 12) * U
+            e = (np.minimum(np.abs(g), 104) + 12) * U
             before[t], before_err[t] = x, R + 24 * U * S
             R = a * (R + e * S) + e * z * np.abs(c)
             S = a * S + z * np.abs(c)
@@ -56,7 +58,7 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, dh=None, dlast=None, n
         for t in reversed(order):
             g, c = pre[b, t, :H], pre[b, t, H:]
             z, a = _sigmoid(g), _sigmoid(-g)
-            e = (np.abs(g) + 12) * U
+            e = (np.minimum(np.abs(g), 104) + 12) * U
             d = 0.0 if dh is None else np.asarray(dh[b, t], np.float64)
             lam, S = carry + d, S + np.abs(d)
             lam_err = R + 24 * U * S

@@ -49,12 +49,12 @@ __device__ __forceinline__ void store_chunk(T* p, typename Chunk<T>::type x, int
     }
 }
 
-// z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open).  Gates
-// below -86 count as -86 (z = 2^-125 there); the minimum hands NaN on.
+// z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open).  A gate below -87
+// closes: z goes to 0 with exp2's overflow (the lowest value of a type as a frame's mask, in its candidate too, adds nothing), and a is 1 there.
 __device__ __forceinline__ void gate_pair(float x, float& z, float& a) {
-    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(x * -1.4426950408889634f, 125.f));
+    const float m = x * -1.4426950408889634f, e = __builtin_amdgcn_exp2f(m);
     z = __builtin_amdgcn_rcpf(1.f + e);
-    a = e * z;
+    a = m > 125.f ? 1.f : e * z;
 }
 
 __device__ __forceinline__ int seq_len(const stes_gated_scan_args& p, int b) {
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
                 gate_pair((float)g[j][v], z, w);
                 const float lam = (float)d[j][v] + k[v];
                 oc[v] = (T)(lam * z);
-                og[v] = (T)(lam * ((float)cand[j][v] - x[j][v]) * z * w);
+                og[v] = (T)(lam * z * ((float)cand[j][v] - x[j][v]) * w);       // (in this order: the difference may be of the type's lowest value, z then 0)
                 k[v] = w * lam;
             }
         } else {
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(64) void scan_short_kernel(const stes_gated_scan_ar
                 gate_pair((float)g[s][v], z, a);
                 const float lam = (dh ? (float)d[BWD ? s : 0][v] : 0.f) + k[v];
                 oc[v] = (T)(lam * z);
-                og[v] = (T)(lam * ((float)cand[s][v] - before[BWD ? s : 0][v]) * z * a);
+                og[v] = (T)(lam * z * ((float)cand[s][v] - before[BWD ? s : 0][v]) * a);
                 k[v] = a * lam;
             }
         }

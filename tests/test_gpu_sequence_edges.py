@@ -1,0 +1,59 @@
+"""The gated scan and the distillation loss at the ends of their types and of their interfaces, on the GPU, against the 64-bit
+restatements (oracle/sequence_oracle.py): tolerances are the oracle's bounds plus half a step of the type that a result is stored in."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import sequence_oracle as SO
+from test_gpu_sequence import _check, _differentiable_calls, _kl_compare, _kl_inputs, _np, _run_scan, _scan_inputs
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def _against_the_oracle(pre, start, lengths, dh, dlast, reverse):
+    with np.errstate(all="ignore"):
+        ref = SO.gated_scan(_np(pre), _np(start), _np(lengths), reverse, _np(dh), _np(dlast), need_grad=True)
+        got = _run_scan_any(pre, start, lengths, dh, dlast, reverse)
+        for name, t in zip(("h", "last", "dpre", "dh0"), got):
+            _check(t, ref[name], ref[name + "_err"], name)
+    return ref, got
+
+
+def _run_scan_any(pre, start, lengths, dh, dlast, reverse):
+    """_run_scan without its comparison of two calls by torch.equal, which NaN fails."""
+    from spot_amd.recurrence import gated_scan
+    p, s = pre.cuda().requires_grad_(), start.cuda().requires_grad_()
+    h, last = gated_scan(p, h0=s, lengths=None if lengths is None else lengths.cuda(), reverse=reverse)
+    return (h, last) + torch.autograd.grad((h, last), (p, s), (dh.cuda(), dlast.cuda()))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,T,H", [(F32, 1, 5), (F32, 5, 8), (BF, 8, 16), (BF, 64, 72), (F32, 300, 24), (BF, 1000, 40)])
+def test_gated_scan_frames_masked_with_the_lowest_value(dtype, T, H, reverse):
+    """Frames whose gates and candidates hold the type's lowest value leave the state as it is: sigmoid is 0 there, and 0 times the
+    lowest value is 0.  Their gates' and candidates' gradients are exactly zero."""
+    pre, start, lengths, dh, dlast = _scan_inputs(3, T, H, dtype, True, "rows", seed=T + H)
+    masked = torch.rand(3, T, generator=torch.Generator().manual_seed(T)) < 0.6
+    masked[2] |= T == 1
+    pre[masked] = torch.finfo(dtype).min
+    _, got = _against_the_oracle(pre, start, lengths, dh, dlast, reverse)
+    assert not bool(got[2].cpu()[masked].any())
+    pre[:] = torch.finfo(dtype).min
+    h, last, dpre, _ = _run_scan(pre, start, None, dh, dlast, reverse)
+    assert torch.equal(last.cpu(), start) and torch.equal(h.cpu(), start.to(dtype)[:, None].expand(3, T, H)) and not bool(dpre.any())
+
+
+@pytest.mark.parametrize("dtype,T,H", [(F32, 4, 6), (BF, 8, 16), (BF, 200, 16), (F32, 200, 9), (F32, 700, 12)])
+def test_gated_scan_gradients_of_saturated_gates(dtype, T, H):
+    """Gates at and beyond the end of the type's range, the gradients to the oracle's bound: exactly zero at the gates, and at the
+    candidates of closed ones."""
+    pre, start, _, dh, dlast = _scan_inputs(2, T, H, dtype, False, "rows", seed=8)
+    v = torch.tensor([INF, -INF, torch.finfo(dtype).max, torch.finfo(dtype).min, 0.0, 30.0, -30.0, 1.0])
+    pick = torch.randint(0, 8, (2, T, H), generator=torch.Generator().manual_seed(1))
+    pre[..., :H] = v[pick].to(dtype)
+    _, got = _against_the_oracle(pre, start, None, dh, dlast, False)
+    dgate, dcand = got[2].cpu()[..., :H], got[2].cpu()[..., H:]
+    assert float(dgate[pick < 4].abs().max()) <= 1e-37 and not bool(dcand[(pick == 1) | (pick == 3)].any())
+    assert float(dgate[pick == 7].abs().max()) > 0.01 and float(dcand[pick == 0].abs().max()) > 0.5
