@@ -459,7 +459,8 @@ int stes_mingru_scan_bwd(const uint16_t* pre, const float* h0, const uint16_t* h
  * streams and ragged batches; stes_mingru_scan_* is its form for short clips with a fixed initial state).  Per sequence b and
  * channel c, in scan order s = 0 .. len-1 (reverse == 0: frame t = s; reverse != 0: t = len-1-s):
  *   z = sigmoid(pre[t][c]),  a = 1 - z = sigmoid(-pre[t][c]),  x_s = a x_{s-1} + z pre[t][H+c],  x_{-1} = h0,  h[t][c] = x_s
- * (below a gate of -87, where sigmoid leaves fp32's normal numbers, z may count as 0)
+ * (below a gate of -87, where sigmoid leaves fp32's normal numbers, z may count as 0; a is never 0: an infinite state or gradient stays
+ * infinite, or becomes NaN where it meets one of the other sign, for any T)
  * and h_last = x_{len-1} (h0 where len = 0).  lengths (int32 [B], values clamped to [0, T]; NULL: T each): rows t >= len of h
  * (and, in backward, of dpre) are written as zeros, whatever pre and dh hold there.
  * pre, h, dh, dpre: bf16 (f32 == 0) or fp32 (f32 == 1); ld_*: elements between frames, bs_*: between sequences; the last dimension is

@@ -49,10 +49,15 @@ __device__ __forceinline__ void store_chunk(T* p, typename Chunk<T>::type x, int
     }
 }
 
+// The least fp32 number.  Added to products that could vanish (and lost in the rounding of all that are normal numbers), it keeps a product
+// of a's above 0: infinity times it stays infinite, as it does step by step, and the largest finite state times it is 5e-7.
+constexpr float LEAST = 0x1p-149f;
+__device__ __forceinline__ float product(float a, float b) { return __builtin_fmaf(a, b, LEAST); }
+
 // z = sigmoid(x) and a = sigmoid(-x), both to full relative precision (1 - z would lose a's digits where the gate is open).  A gate below -87
 // closes: z goes to 0 with exp2's overflow (the lowest value of a type as a frame's mask, in its candidate too, adds nothing), and a is 1 there.
 __device__ __forceinline__ void gate_pair(float x, float& z, float& a) {
-    const float m = x * -1.4426950408889634f, e = __builtin_amdgcn_exp2f(m);
+    const float m = x * -1.4426950408889634f, e = __builtin_amdgcn_exp2f(m) + LEAST;
     z = __builtin_amdgcn_rcpf(1.f + e);
     a = m > 125.f ? 1.f : e * z;
 }
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
         }
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v]; sB[seg][cl * V + v] = B[v]; }
+    for (int v = 0; v < V; ++v) { sA[seg][cl * V + v] = A[v] + LEAST; sB[seg][cl * V + v] = B[v]; }        // (product() above: 130 registers, one workgroup a CU)
     wave_lds_fence();
     {
         float fa = 1.f, fb = 0.f;                            // lane = channel
@@ -217,7 +222,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
             sA[wave * SW + i][lane] = fa;
             sB[wave * SW + i][lane] = fb;
             fb = ia * fb + ib;
-            fa = ia * fa;
+            fa = product(ia, fa);
         }
         tA[wave][lane] = fa;
         tB[wave][lane] = fb;
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(G::NT) void scan_fwd_kernel(const stes_gated_scan_a
         const int ch = at.c0 + lane;
         float x = 0.f, fa[NW], fb[NW], mA = 1.f, mB = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][lane]; fb[w] = tB[w][lane]; mB = fa[w] * mB + fb[w]; mA = fa[w] * mA; }
+        for (int w = 0; w < NW; ++w) { fa[w] = tA[w][lane]; fb[w] = tB[w][lane]; mB = fa[w] * mB + fb[w]; mA = product(fa[w], mA); }
         const long word = at.chain * CT + lane, words = chains * CT;
         if (ch < p.H) {
             if (!JOIN || at.blk == 0) x = p.h0 ? p.h0[at.b * p.bs_h0 + ch] : 0.f;
@@ -309,7 +314,7 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
             k = live ? k : 1.f;
             const float u = live ? z * (float)cand[j][v] : 0.f;
             B[v] = k * B[v] + u;
-            A[v] *= k;
+            A[v] = product(A[v], k);
             R[v] += A[v] * (float)d[j][v];               // d_j reaches the segment's front through a_0 .. a_j
         }
     }
@@ -325,14 +330,14 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
             sA[wave * SW + i][lane] = fa;
             sB[wave * SW + i][lane] = fb;
             fb = ia[i] * fb + ib[i];
-            fa = ia[i] * fa;
+            fa = product(ia[i], fa);
         }
 #pragma unroll
         for (int i = SW - 1; i >= 0; --i) {
             sS[wave * SW + i][lane] = ra;
             sR[wave * SW + i][lane] = rr;
             rr = ia[i] * rr + ir[i];
-            ra = ia[i] * ra;
+            ra = product(ia[i], ra);
         }
         tA[wave][lane] = fa;
         tB[wave][lane] = fb;
@@ -346,7 +351,7 @@ __global__ __launch_bounds__(G::NT) void scan_bwd_kernel(const stes_gated_scan_a
 #pragma unroll
         for (int w = 0; w < NW; ++w) { fa[w] = tA[w][lane]; fb[w] = tB[w][lane]; fr[w] = tR[w][lane]; }
 #pragma unroll
-        for (int w = NW - 1; w >= 0; --w) { mR = fa[w] * mR + fr[w]; mA = fa[w] * mA; }
+        for (int w = NW - 1; w >= 0; --w) { mR = fa[w] * mR + fr[w]; mA = product(fa[w], mA); }
         const long word = at.chain * CT + lane, words = chains * CT;
         if (ch < p.H) {
             x = p.states[((long)at.b * blocks + blk) * H + ch];

@@ -57,3 +57,25 @@ def test_gated_scan_gradients_of_saturated_gates(dtype, T, H):
     dgate, dcand = got[2].cpu()[..., :H], got[2].cpu()[..., H:]
     assert float(dgate[pick < 4].abs().max()) <= 1e-37 and not bool(dcand[(pick == 1) | (pick == 3)].any())
     assert float(dgate[pick == 7].abs().max()) > 0.01 and float(dcand[pick == 0].abs().max()) > 0.5
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,T,H", [(F32, 6, 16), (BF, 64, 64), (F32, 250, 20), (BF, 600, 64), (F32, 3000, 12)])
+def test_gated_scan_infinite_states_stay_infinite(dtype, T, H, reverse):
+    """Infinite initial states, candidates and gradients: what comes behind one is infinite, NaN only where two of other signs meet,
+    whatever the length and however the time axis is cut."""
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, dh, dlast = _scan_inputs(3, T, H, dtype, False, "rows", seed=T, gate=(0.0, 1.5))
+    start[0, 0], start[1, 1], start[2, 2] = INF, -INF, NAN
+    pre[0, T // 2, H + 3], pre[1, T // 3, H + 4], pre[2, T - 1, H + 5] = INF, -INF, INF
+    pre[0, T // 3, H + 6], pre[0, T // 2, H + 6] = INF, -INF
+    dh[1, T // 2, 7], dh[2, T // 2, 8], dlast[0, 9] = INF, -INF, INF
+    ref, got = _against_the_oracle(pre, start, None, dh, dlast, reverse)
+    assert np.isinf(ref["last"][0, 0]) and np.isinf(ref["dh0"][1, 7]) and np.isinf(ref["dh0"][0, 9])
+    state, parts, p = start.cuda(), [], pre.cuda()
+    for lo, hi in ((0, T // 2), (T // 2, T)) if not reverse else ((T // 2, T), (0, T // 2)):
+        h, state = gated_scan(p[:, lo:hi], state, reverse=reverse)
+        parts.append(h)
+    both = torch.cat(parts[::-1] if reverse else parts, 1)
+    for a, b in ((both, got[0]), (state, got[1])):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf()) and torch.equal(a[a.isinf()], b[b.isinf()])
