@@ -72,7 +72,10 @@ void written(const Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 // (forward-mode tangents would be lost without a word)
-bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+template <typename... Tensors>
+void no_tangents(const char* op, const Tensors&... t) {
+    if ((... || (t.defined() && t._fw_grad(0).defined()))) refuse(op, "no forward-mode derivatives");
+}
 bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---------------------------------------------------------------- leaves
@@ -247,6 +250,7 @@ struct GatedScanBackward : public Node {
         std::lock_guard<std::mutex> g(mutex_);
         const Tensor p = pre.unpack(), n = lengths.unpack(), st = states.unpack();
         Tensor dpre, dh0, total;
+        no_tangents(SCAN, grads[0], grads[1]);
         if (grads[0].defined() || grads[1].defined()) {
             const Call call(p.device());
             const int64_t B = p.size(0), T = p.size(1), W = p.size(2), H = W / 2;
@@ -310,7 +314,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
     }
     if (lengths.defined() && (lengths.device() != dev || lengths.scalar_type() != at::kInt || lengths.dim() != 1 || lengths.size(0) != B || !lengths.is_contiguous()))
         refuse(SCAN, "lengths must be contiguous int32 [", B, "] on ", dev, ", got ", lengths.scalar_type(), " ", lengths.sizes(), " on ", lengths.device());
-    if (has_tangent(pre) || (h0.defined() && has_tangent(h0))) refuse(SCAN, "no forward-mode derivatives");
+    no_tangents(SCAN, pre, h0, out, state_out);
     const bool grad = asks_for_gradients(pre) || (h0.defined() && asks_for_gradients(h0));
     if (grad && (out.defined() || state_out.defined())) refuse(SCAN, "out and state_out are for calls without gradients");
     if (out.defined()) {
@@ -414,7 +418,7 @@ Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, d
     Tensor weight = weight_.value_or(Tensor());
     if (weight.defined() && (weight.device() != dev || weight.scalar_type() != at::kFloat || weight.sizes() != lead)) refuse(KL, "weight must be float32 ", lead, " on ", dev);
     if (asks_for_gradients(val) || (weight.defined() && asks_for_gradients(weight))) refuse(KL, "the teacher's logits and the weights are constants: detach them");
-    if (has_tangent(logits) || has_tangent(val) || (weight.defined() && has_tangent(weight))) refuse(KL, "no forward-mode derivatives");
+    no_tangents(KL, logits, val, weight);
     if (!(temperature >= 1e-6 && temperature <= 1e6)) refuse(KL, "the temperature lies between 1e-6 and 1e6, got ", temperature);
     Rows r{flat(logits, V), flat(idx, k), flat(val, k), Tensor(), temperature, 0.0};
     if (std::max(r.logits.size(0), V) > INT32_MAX) refuse(KL, "sizes beyond 32 bits: ", logits.sizes());
@@ -438,6 +442,7 @@ struct DistillBackward : public Node {
         const Rows r{logits.unpack(), idx.unpack(), val.unpack(), weight.unpack(), temperature, denom};
         const Tensor st = stats.unpack();
         Tensor d;
+        no_tangents(KL, grads[0]);
         if (grads[0].defined()) {
             const Call call(r.logits.device());
             d = fresh(r.logits.sizes(), r.logits);
@@ -483,6 +488,7 @@ std::tuple<Tensor, Tensor> topk_distill_grad(const Tensor& logits, const Tensor&
                                              std::optional<double> denom, double grad_scale, const Maybe& out_, bool accumulate) {
     const Rows r = distill_check(logits, idx, val, temperature, weight, denom);
     Tensor out = out_.value_or(Tensor()), d;
+    no_tangents(KL, out);
     const Call call(r.logits.device());
     if (!out.defined()) {
         if (accumulate) refuse(KL, "accumulate adds to out");

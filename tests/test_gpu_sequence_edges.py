@@ -79,3 +79,29 @@ def test_gated_scan_infinite_states_stay_infinite(dtype, T, H, reverse):
     both = torch.cat(parts[::-1] if reverse else parts, 1)
     for a, b in ((both, got[0]), (state, got[1])):
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf()) and torch.equal(a[a.isinf()], b[b.isinf()])
+
+
+def test_tangents_are_refused_in_backward_passes_and_in_results():
+    """A tangent that arrives with the upstream gradient, or that a result to be written carries, would be lost without a word."""
+    from spot_amd import lib
+    from spot_amd.distill import topk_distill_grad
+    from spot_amd.recurrence import gated_scan
+    ad = torch.autograd.forward_ad
+    for leaf, f in _differentiable_calls():
+        y = f(leaf)
+        with ad.dual_level():
+            for up in (ad.make_dual(torch.ones_like(y), torch.ones_like(y)),):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(y, leaf, up, retain_graph=True)
+        torch.autograd.grad(y, leaf)
+    p = torch.randn(2, 3, 8, device="cuda", requires_grad=True)
+    h, last = gated_scan(p)
+    with ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(last, p, ad.make_dual(torch.ones_like(last), torch.ones_like(last)))
+        dual = lambda *s: ad.make_dual(torch.zeros(*s, device="cuda"), torch.ones(*s, device="cuda"))  # noqa: E731
+        for kw in (dict(out=dual(2, 3, 4)), dict(state_out=dual(2, 4))):
+            with pytest.raises(lib.StesError, match="forward-mode"):
+                gated_scan(p.detach(), **kw)
+        with pytest.raises(lib.StesError, match="forward-mode"):
+            topk_distill_grad(torch.zeros(4, 7, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda"), torch.zeros(4, 2, device="cuda"), out=dual(4, 7))
