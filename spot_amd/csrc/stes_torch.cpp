@@ -16,8 +16,10 @@
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -72,6 +74,14 @@ void written(const Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 // (forward-mode tangents would be lost without a word)
+// A trace would record the allocation of a result and not the kernel that writes it.
+void untraced(const char* op) {
+    using c10::impl::TorchDispatchModeKey;
+    typedef c10::impl::TorchDispatchModeTLS Modes;
+    bool traced = at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    if (Modes::any_modes_set()) traced = traced || Modes::get_mode(TorchDispatchModeKey::PROXY) || Modes::get_mode(TorchDispatchModeKey::FAKE) || Modes::get_mode(TorchDispatchModeKey::FUNCTIONAL);
+    if (traced) refuse(op, "cannot be traced (torch.jit.trace, make_fx): call it outside of what is recorded");
+}
 template <typename... Tensors>
 void no_tangents(const char* op, const Tensors&... t) {
     if ((... || (t.defined() && t._fw_grad(0).defined()))) refuse(op, "no forward-mode derivatives");
@@ -250,6 +260,7 @@ struct GatedScanBackward : public Node {
         std::lock_guard<std::mutex> g(mutex_);
         const Tensor p = pre.unpack(), n = lengths.unpack(), st = states.unpack();
         Tensor dpre, dh0, total;
+        untraced(SCAN);
         no_tangents(SCAN, grads[0], grads[1]);
         if (grads[0].defined() || grads[1].defined()) {
             const Call call(p.device());
@@ -297,6 +308,7 @@ bool apart(const Tensor& t, int64_t width) {
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const Maybe& lengths_, bool reverse, const Maybe& out_, const Maybe& state_out_) {
     Tensor h0 = h0_.value_or(Tensor()), lengths = lengths_.value_or(Tensor()), out = out_.value_or(Tensor()), state_out = state_out_.value_or(Tensor());
+    untraced(SCAN);
     if (!pre.is_cuda() || pre.dim() != 3 || !element(pre)) refuse(SCAN, "pre must be a bfloat16 or float32 tensor [B, T, 2H] on the GPU");
     const int64_t B = pre.size(0), T = pre.size(1), W = pre.size(2), H = W / 2;
     const c10::Device dev = pre.device();
@@ -405,6 +417,7 @@ Tensor distill_call(stes_distill_args& a, const Tensor& logits) {
 }
 
 Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, double temperature, const Maybe& weight_, std::optional<double> denom) {
+    untraced(KL);
     if (!logits.is_cuda() || !element(logits) || logits.dim() < 1) refuse(KL, "logits must be a bfloat16 or float32 tensor [..., classes] on the GPU");
     const c10::Device dev = logits.device();
     const int64_t V = logits.size(-1);
@@ -442,6 +455,7 @@ struct DistillBackward : public Node {
         const Rows r{logits.unpack(), idx.unpack(), val.unpack(), weight.unpack(), temperature, denom};
         const Tensor st = stats.unpack();
         Tensor d;
+        untraced(KL);
         no_tangents(KL, grads[0]);
         if (grads[0].defined()) {
             const Call call(r.logits.device());

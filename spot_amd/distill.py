@@ -4,7 +4,8 @@ student's class distribution from the teacher's distribution over its k best cla
     loss = topk_distill_loss(student_logits, idx, val, temperature=2.0)             # for loss.backward()
     loss, dlogits = topk_distill_grad(student_logits, idx, val, temperature=2.0)    # both in one pass over the logits
 
-`idx` and `val` are what `teacher_logits.topk(k)` gives; an index below zero marks an unused place of a frame's list.
+`idx` and `val` are what `teacher_logits.topk(k)` gives; an index below zero marks an unused place of a frame's list.  Neither call can be
+traced (torch.jit.trace, make_fx).
 """
 from __future__ import annotations
 

@@ -105,3 +105,20 @@ def test_tangents_are_refused_in_backward_passes_and_in_results():
                 gated_scan(p.detach(), **kw)
         with pytest.raises(lib.StesError, match="forward-mode"):
             topk_distill_grad(torch.zeros(4, 7, device="cuda"), torch.zeros(4, 2, dtype=torch.int64, device="cuda"), torch.zeros(4, 2, device="cuda"), out=dual(4, 7))
+
+
+def test_tracing_refuses_forward_and_backward_passes():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from spot_amd import lib
+    for leaf, f in _differentiable_calls():
+        want = f(leaf)
+        with pytest.raises(lib.StesError, match="trace"):
+            make_fx(f)(leaf.detach())
+        with pytest.raises(lib.StesError, match="trace"):
+            torch.jit.trace(f, (leaf.detach(),), check_trace=False)
+        with pytest.raises(RuntimeError, match="trace"):
+            make_fx(lambda u: torch.autograd.grad(want, leaf, u, retain_graph=True)[0])(torch.ones_like(want))
+        torch.autograd.grad(want, leaf)
+        from torch.utils.flop_counter import FlopCounterMode
+        with FlopCounterMode(display=False):                # a mode that only looks on
+            assert torch.equal(f(leaf), want)
