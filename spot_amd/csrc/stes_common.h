@@ -2,8 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-#include <algorithm>
 #include "../../include/stes.h"
+#include "stes_share.h"
 
 typedef __bf16 bf16;
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -59,34 +59,6 @@ int stes_set_error(int code, const char* msg);
     do { if (!(cond)) return stes_set_error((code), (msg)); } while (0)
 #define STES_LAUNCH_CHECK() \
     do { hipError_t e_ = hipGetLastError(); if (e_ != hipSuccess) return stes_set_error(STES_ERR_LAUNCH, hipGetErrorString(e_)); } while (0)
-
-// A tensor [B][T][width] as a caller describes it, and whether two of them share memory.
-struct StesRows {
-    const void* p;
-    int es;                 // bytes of an element
-    int64_t ld, bs;         // elements between frames, between sequences
-    int64_t T, B, width;
-};
-
-static inline bool stes_share(const StesRows& a, const StesRows& b) {
-    if (!a.p || !b.p || !a.T || !a.B || !a.width || !b.T || !b.B || !b.width) return false;
-    auto bytes = [](const StesRows& r) { return ((r.T - 1) * r.ld + (r.B - 1) * r.bs + r.width) * r.es; };
-    const int64_t d = (const char*)b.p - (const char*)a.p;
-    if (d >= bytes(a) || -d >= bytes(b)) return false;
-    // Parts of one buffer: with equal strides an element is common where  d + v - u = i * ld + j * bs,  u and v in the rows' widths and
-    // i, j differences of frames and sequences; for other strides crossing ranges count as shared.
-    if (a.es != b.es || d % a.es || (a.T > 1 && b.T > 1 && a.ld != b.ld) || (a.B > 1 && b.B > 1 && a.bs != b.bs)) return true;
-    const int64_t e = d / a.es, ld = a.T > 1 ? a.ld : b.T > 1 ? b.ld : 1, bs = a.B > 1 ? a.bs : b.B > 1 ? b.bs : 1;
-    if (ld <= 0 || bs <= 0) return true;
-    auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
-    const int64_t lo = std::max(1 - b.B, -floor_div(a.width + (a.T - 1) * ld - e, bs)), hi = std::min(a.B - 1, floor_div(e + b.width + (b.T - 1) * ld, bs));
-    if (hi - lo > 64) return true;
-    for (int64_t j = lo; j <= hi; ++j) {
-        const int64_t r = e - j * bs;                               // i * ld in (r - a.width, r + b.width)
-        if (std::max(1 - b.T, floor_div(r - a.width, ld) + 1) <= std::min(a.T - 1, floor_div(r + b.width - 1, ld))) return true;
-    }
-    return false;
-}
 
 static inline int stes_div_up(long a, long b) { return (int)((a + b - 1) / b); }
 

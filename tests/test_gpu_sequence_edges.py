@@ -122,3 +122,22 @@ def test_tracing_refuses_forward_and_backward_passes():
         from torch.utils.flop_counter import FlopCounterMode
         with FlopCounterMode(display=False):                # a mode that only looks on
             assert torch.equal(f(leaf), want)
+
+
+@pytest.mark.parametrize("B", [34, 100, 192])
+@pytest.mark.parametrize("T", [2, 5, 300])
+def test_gated_scan_in_columns_of_a_time_major_buffer(B, T):
+    """[T][B][3H], frames outermost: pre in the first 2H columns, the states written beside them; one column more is refused."""
+    from spot_amd import lib
+    from spot_amd.recurrence import gated_scan
+    H = 8
+    pre, start, _, _, _ = _scan_inputs(B, T, H, F32, False, "rows", seed=B + T)
+    want = gated_scan(pre.cuda(), start.cuda())
+    buf = torch.full((T, B, 3 * H), NAN, device="cuda")
+    view = buf.transpose(0, 1)
+    view[..., :2 * H] = pre.cuda()
+    h, last = gated_scan(view[..., :2 * H], start.cuda(), out=view[..., 2 * H:])
+    assert torch.equal(h, want[0]) and torch.equal(last, want[1]) and torch.equal(view[..., :2 * H], pre.cuda())
+    for out in (view[..., 2 * H - 1:3 * H - 1], view[..., :H]):
+        with pytest.raises(lib.StesError):
+            gated_scan(view[..., :2 * H], start.cuda(), out=out)

@@ -26,3 +26,55 @@ def test_tracing_is_refused():
         with pytest.raises(lib.StesError) as e:            # (and the refusal of a host tensor is another one)
             f(x)
         assert "trace" not in str(e.value)
+
+
+@pytest.fixture(scope="module")
+def share(tmp_path_factory):
+    """stes_share (csrc/stes_share.h) as a function of two layouts (address, element bytes, ld, bs, T, B, width)."""
+    import ctypes as C
+    import os
+    import subprocess
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    d = tmp_path_factory.mktemp("share")
+    (d / "s.cpp").write_text('#include "%s"\nextern "C" int share(const long long* q) {\n'
+                             '    auto r = [](const long long* v) { return StesRows{(const void*)v[0], (int)v[1], v[2], v[3], v[4], v[5], v[6]}; };\n'
+                             '    return stes_share(r(q), r(q + 7));\n}\n' % os.path.join(here, "spot_amd", "csrc", "stes_share.h"))
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", str(d / "s.cpp"), "-o", str(d / "s.so")])
+    fn = C.CDLL(str(d / "s.so")).share
+    return lambda a, b: bool(fn((C.c_longlong * 14)(*a, *b)))
+
+
+def _elements(p, es, ld, bs, T, B, width):
+    return {p // es + t * ld + b * bs + v for t in range(T) for b in range(B) for v in range(width)}
+
+
+@pytest.mark.parametrize("B", [3, 33, 34, 100, 1000])
+@pytest.mark.parametrize("T", [1, 2, 7, 300])
+def test_columns_of_one_buffer_do_not_share_memory(share, B, T):
+    """pre in the first 2H of 3H columns and h in the last, frames or sequences outermost; one column to the left they share."""
+    H, p = 8, 1 << 20
+    for ld, bs in ((3 * H, 3 * H * T), (3 * H * B, 3 * H)):
+        pre = (p, 4, ld, bs, T, B, 2 * H)
+        for off, want in ((2 * H, False), (2 * H - 1, True), (0, True), (H, True)):
+            h = (p + 4 * off, 4, ld, bs, T, B, H)
+            assert share(pre, h) is want and share(h, pre) is want
+        late = (p + 4 * ld * T, 4, ld, bs, T, B, H)                      # the frames behind (frames outermost: behind all)
+        assert share(pre, late) is bool(_elements(*pre) & _elements(*late))
+
+
+def test_shared_memory_against_sets_of_elements(share):
+    """Random layouts of equal strides: never missed, and refused wrongly only where a batch's sequences lie across one another."""
+    import random
+    rng = random.Random(5)
+    wrong = 0
+    for _ in range(20000):
+        T, B, w1, w2 = rng.randint(1, 6), rng.randint(1, 6), rng.randint(1, 5), rng.randint(1, 5)
+        inner = rng.randint(max(w1, w2), 12)
+        outer = inner * max(T, B) + rng.randint(0, 5)
+        ld, bs = (inner, outer) if rng.random() < 0.5 else (outer, inner)
+        a = (4096, 4, ld, bs, T, B, w1)
+        b = (4096 + 4 * rng.randint(-80, 80), 4, ld, bs, rng.choice((1, T)), rng.choice((1, B)), w2)
+        truth = bool(_elements(*a) & _elements(*b))
+        assert not truth or share(a, b), (a, b)
+        wrong += share(a, b) and not truth
+    assert wrong == 0
