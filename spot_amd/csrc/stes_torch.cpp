@@ -12,13 +12,13 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
-#include <unordered_map>
 #include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/StreamGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/function.h>
@@ -89,38 +89,23 @@ void no_tangents(const char* op, const Tensors&... t) {
 bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 // ---------------------------------------------------------------- leaves
-// The node that accumulates a leaf's gradient keeps the stream on which it was made for as long as some autograd graph holds it; a
-// backward pass that is captured while an eager graph of the same leaf lives would pull that stream into the capture, which ends the
-// process.  Eager calls note their leaves' nodes, captured ones refuse nodes that are noted and live.
-struct Leaves {
-    std::mutex lock;
-    std::unordered_map<Node*, std::weak_ptr<Node>> eager;
-    size_t sweep = 64;
-};
-Leaves& leaves() {
-    static Leaves* all = new Leaves;                  // (never destroyed: autograd's threads outlive main)
-    return *all;
-}
-
-// The inputs' edges into the graph, held while they are looked at: leaves' nodes live as long as something holds them.
-torch::autograd::edge_list guarded(torch::autograd::edge_list edges) {
-    const bool now = capturing();
-    Leaves& l = leaves();
-    std::lock_guard<std::mutex> g(l.lock);
+// The node that accumulates a leaf's gradient keeps the stream on which it was made for as long as some autograd graph holds it, whoever made
+// that graph; a captured backward pass makes that stream wait for the capture's, which ends the process where it is not part of the
+// capture (the default stream cannot be).  A captured call refuses such leaves.
+torch::autograd::edge_list guarded(torch::autograd::edge_list edges, c10::Device dev) {
+    if (!capturing()) return edges;
+    const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).unwrap();
     for (const auto& e : edges) {
         std::shared_ptr<Node> n = e.function;
         for (int i = 0; i < 4 && n && n->num_outputs() == 1; ++i) n = n->next_edge(0).function;      // (through the views and copies that a call makes of a leaf)
         if (!n || n->num_outputs() != 0) continue;
-        if (!now) l.eager[n.get()] = n;
-        else {
-            const auto seen = l.eager.find(n.get());
-            if (seen != l.eager.end() && seen->second.lock() == n)
-                refuse("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first");
+        const std::optional<c10::Stream> made = n->stream();
+        if (!made || *made == here) continue;
+        if (made->id() != 0) {
+            const c10::StreamGuard there(*made);
+            if (capturing()) continue;                // (another stream of a capture)
         }
-    }
-    if (l.eager.size() > l.sweep) {
-        for (auto i = l.eager.begin(); i != l.eager.end();) i = i->second.expired() ? l.eager.erase(i) : std::next(i);
-        l.sweep = 64 + 2 * l.eager.size();
+        refuse("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first");
     }
     return edges;
 }
@@ -354,7 +339,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
     std::shared_ptr<GatedScanBackward> node(new GatedScanBackward, torch::autograd::deleteNode);
     {
         const Call call(dev);
-        node->set_next_edges(guarded(torch::autograd::collect_next_edges(pre, h0)));
+        node->set_next_edges(guarded(torch::autograd::collect_next_edges(pre, h0), dev));
         r = scan_forward(pre, h0, lengths, reverse, out, state_out, true);
     }
     node->pre = SavedVariable(pre, false);
@@ -483,7 +468,7 @@ Tensor topk_distill_loss(const Tensor& logits, const Tensor& idx, const Tensor& 
     Tensor loss, stats;
     {
         const Call call(r.logits.device());
-        node->set_next_edges(guarded(torch::autograd::collect_next_edges(r.logits)));
+        node->set_next_edges(guarded(torch::autograd::collect_next_edges(r.logits), r.logits.device()));
         stats = fresh({r.logits.size(0), 2}, r.logits, at::kFloat);
         a.stats = at_<float>(stats);
         loss = distill_call(a, r.logits);

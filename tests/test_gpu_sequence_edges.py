@@ -141,3 +141,34 @@ def test_gated_scan_in_columns_of_a_time_major_buffer(B, T):
     for out in (view[..., 2 * H - 1:3 * H - 1], view[..., :H]):
         with pytest.raises(lib.StesError):
             gated_scan(view[..., :2 * H], start.cuda(), out=out)
+
+
+def test_capture_accepts_leaves_of_its_own_stream_and_refuses_others():
+    """A leaf that an eager graph holds is refused in a capture for the stream that graph ran on, whoever made the graph: one that ran on the
+    capture's own stream does no harm, one that torch's own functions made does."""
+    from spot_amd import lib
+    from spot_amd.recurrence import gated_scan
+    for leaf, f in _differentiable_calls():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            alive = f(leaf)
+            want, = torch.autograd.grad(alive, leaf, retain_graph=True)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            g, = torch.autograd.grad(f(leaf), leaf)
+        for _ in range(3):
+            g.zero_()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(g, want)
+        del alive
+    p = torch.randn(2, 4, 16, device="cuda", requires_grad=True)
+    alive = (p * 2).sum()                                   # on the default stream
+    torch.cuda.synchronize()
+    with pytest.raises(lib.StesError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.ones(4, device="cuda").mul_(2)
+            gated_scan(p)
+    del alive
