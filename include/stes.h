@@ -511,7 +511,8 @@ int stes_loss(const float* logits, int64_t ldl, const float* loc, int64_t ldloc,
  * -inf) add nothing to the loss and have a gradient of zero whatever their logits hold.  An idx >= V makes its row's KL and gradient
  * NaN.  Softmax statistics and sums are fp32.
  * stes_distill: loss [1] and, when dlogits is given, the gradient in the same pass over the logits; stats [M][2] (optional):
- * the row's maximum and 1 / sum exp((logits - max) / tau), from which stes_distill_bwd computes the gradient later.
+ * the row's maximum and its sum of exp((logits - max) / tau), from which stes_distill_bwd computes the gradient later (what a row
+ * that adds nothing to the loss holds there is not specified).
  * dlogits: fp32 (d_f32) or bf16, written, or added to when accumulate != 0; it must not overlap logits.  Columns from V up are
  * not touched.  ws: stes_distill_ws_floats(M, V, k, zeros != NULL) floats.  zeros (optional): STES_DISTILL_WORDS
  * zero words, which the call may use and leaves zero; it then needs one launch instead of two where its workgroups are few enough.  Calls that

@@ -172,3 +172,38 @@ def test_capture_accepts_leaves_of_its_own_stream_and_refuses_others():
             torch.ones(4, device="cuda").mul_(2)
             gated_scan(p)
     del alive
+
+
+@pytest.mark.parametrize("V", [7, 300, 1000, 20000, 70000])
+def test_distill_statistics_are_the_maximum_and_the_sum(V):
+    """The contract of the C interface: stats hold a row's maximum and sum exp((logits - max) / tau), and the backward pass takes what the
+    caller gives."""
+    import ctypes as C
+    from spot_amd import lib
+    M, k, tau = 6, 3, 2.0
+    s, idx, val, _ = _kl_inputs(M, V, k, F32, V)
+    x, i, v = s.cuda(), idx.cuda(), val.cuda()
+    stats, loss, d = torch.full((M, 2), NAN, device="cuda"), torch.zeros(1, device="cuda"), torch.full((M, V), NAN, device="cuda")
+    n = lib.lib().stes_distill_ws_floats(M, V, k, 0)
+    ws = torch.zeros(max(n, 1), device="cuda")
+    base = dict(logits=lib.ptr(x), ld=V, f32=1, idx=lib.ptr(i), ld_idx=k, idx_i64=1, val=lib.ptr(v), ld_val=k, val_f32=1, M=M, V=V, k=k, temperature=tau, denom=3.0,
+                grad_scale=1.0)
+
+    def args(**kw):
+        a = lib.DistillArgs()
+        for name, value in {**base, **kw}.items():
+            setattr(a, name, value)
+        return a
+    a = args(loss=lib.ptr(loss), stats=lib.ptr(stats), ws=lib.ptr(ws), ws_floats=n)
+    lib.check(lib.lib().stes_distill(C.byref(a), lib.stream()), "stes_distill")
+    top = _np(s).max(1)
+    y = (_np(s) - top[:, None]) / tau
+    total = np.exp(y).sum(1)
+    _check(stats[:, 0], top, 0 * top, "maximum")
+    # exp2 of a rounded argument (3 u |y|) good to 2 u, and fewer than V / 4 + 16 roundings of the sum
+    _check(stats[:, 1], total, SO.U * ((np.exp(y) * (4 * np.abs(y) + 2)).sum(1) + (V / 4 + 16) * total), "sum")
+    given = torch.tensor(np.stack([top, total], 1), dtype=F32, device="cuda")
+    a = args(stats=lib.ptr(given), dlogits=lib.ptr(d), ld_d=V, d_f32=1)
+    lib.check(lib.lib().stes_distill_bwd(C.byref(a), lib.stream()), "stes_distill_bwd")
+    ref = SO.topk_distill(_np(s), _np(idx), _np(val), tau, None, 3.0)
+    _check(d, ref["dlogits"], ref["dlogits_err"], "dlogits")
