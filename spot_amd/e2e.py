@@ -281,6 +281,21 @@ class E2EModel(BaseRGBModel):
             raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
         return [h.detach().to(self.device, torch.float32).expand(n, -1).clone() for h in self._model._pred_fine.h0]
 
+    def _check_state(self, seq, state):
+        """A state that does not fit the model and `seq` is refused before a layer's state moves on."""
+        layers, dev = self._model._pred_fine, next(self._model.parameters()).device
+        state = list(state) if isinstance(state, (list, tuple, torch.Tensor)) else []
+        fit = len(state) == layers.n_layers and all(isinstance(s, torch.Tensor) and s.dim() == 2 and s.device == dev and s.dtype == torch.float32
+                                                    and s.is_contiguous() and s.shape == (state[0].shape[0], layers.hidden_size) for s in state)
+        n = state[0].shape[0] if fit else 0
+        if fit and n:
+            at = sorted(s.data_ptr() for s in state)             # (layers' states lie apart)
+            fit = all(q - p >= 4 * n * layers.hidden_size for p, q in zip(at, at[1:]))
+        if not fit or n < 1 or seq.shape[0] < 1 or seq.shape[0] % n:
+            raise lib.StesError(f"predict_stream: {seq.shape[0]} clips and a state of {[tuple(s.shape) if isinstance(s, torch.Tensor) else type(s).__name__ for s in state]} "
+                                f"do not fit: clips are a multiple of the streams of new_stream(), states one float32 tensor [n, {layers.hidden_size}] on {dev} for each "
+                                f"of {layers.n_layers} layers")
+
     def predict_stream(self, seq, state):
         """predict_async() for the next frames of n streams (`state` of new_stream(n), updated in place): seq [n * W, T, C, H, W] holds W
         clips of every stream, one after the other in time.  Clips are independent in the backbone (T = clip_len where it
@@ -292,13 +307,7 @@ class E2EModel(BaseRGBModel):
             raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
         if seq.dim() == 4:
             seq = seq.unsqueeze(0)
-        n, hidden = (state[0].shape if len(state) else (0, 0))
-        layers = self._model._pred_fine
-        if (len(state) != layers.n_layers or hidden != layers.hidden_size or n < 1 or seq.shape[0] < 1 or seq.shape[0] % n
-                or any(s.shape != state[0].shape or s.dtype != torch.float32 or not s.is_contiguous() for s in state)
-                or len({s.data_ptr() for s in state}) != len(state)):
-            raise lib.StesError(f"predict_stream: {seq.shape[0]} clips and a state of {len(state)} layers {[tuple(s.shape) for s in state]} "
-                                "do not fit: clips are a multiple of the streams of new_stream(), states one float32 tensor a layer")
+        self._check_state(seq, state)
         if seq.device != torch.device(self.device) and str(seq.device) != str(self.device):
             seq = seq.to(self.device, non_blocking=True)
         if self._model.training:
