@@ -50,7 +50,14 @@ void check(int rc, const char* entry) {
     if (rc) throw Refused(c10::str(entry, " failed (", rc, "): ", stes_last_error()), rc);
 }
 
-void* stream_of(c10::Device dev) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream(); }
+auto current(c10::Device dev) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()); }
+void* stream_of(c10::Device dev) { return current(dev).stream(); }
+// The device's default stream and torch's own streams last as long as the process.  A stream from outside, whose number is its handle, may be
+// destroyed and its handle given out again (and one handle stands for a default stream of each thread): nothing is kept for it.
+bool lasts(c10::Device dev) {
+    const auto s = current(dev);
+    return !s.stream() || s.id() != reinterpret_cast<c10::StreamId>(s.stream());
+}
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // Makes `dev` the current device for a call on its tensors, and allocations skip the layers that record gradients.
@@ -94,7 +101,7 @@ bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradM
 // capture (the default stream cannot be).  A captured call refuses such leaves.
 torch::autograd::edge_list guarded(torch::autograd::edge_list edges, c10::Device dev) {
     if (!capturing()) return edges;
-    const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).unwrap();
+    const c10::Stream here = current(dev).unwrap();
     for (const auto& e : edges) {
         std::shared_ptr<Node> n = e.function;
         for (int i = 0; i < 4 && n && n->num_outputs() == 1; ++i) n = n->next_edge(0).function;      // (through the views and copies that a call makes of a leaf)
@@ -167,7 +174,7 @@ void scan_call(int (*entry)(const stes_gated_scan_args*, void*), const char* nam
     if (!n) return check(entry(&a, s), name);
     const auto bytes = at::TensorOptions().device(dev).dtype(at::kByte);
     a.ws_bytes = n;
-    if (n > KEPT_BYTES || capturing()) {
+    if (n > KEPT_BYTES || capturing() || !lasts(dev)) {
         const Tensor ws = at::empty({n}, bytes);
         a.ws = ws.data_ptr();
         return check(entry(&a, s), name);
@@ -387,7 +394,7 @@ Tensor distill_call(stes_distill_args& a, const Tensor& logits) {
     void* s = stream_of(logits.device());
     a.loss = static_cast<float*>(loss.data_ptr());
     std::shared_ptr<Kept> k;
-    if (a.M > 1 && !capturing()) {          // (a graph may be replayed on any stream, next to others)
+    if (a.M > 1 && !capturing() && lasts(logits.device())) {          // (a graph may be replayed on any stream, next to others)
         k = kept(logits.device().index(), s);
         std::lock_guard<std::mutex> g(k->lock);
         if (!k->zeros.defined()) k->zeros = at::zeros({STES_DISTILL_WORDS}, logits.options().dtype(at::kLong));

@@ -207,3 +207,28 @@ def test_distill_statistics_are_the_maximum_and_the_sum(V):
     lib.check(lib.lib().stes_distill_bwd(C.byref(a), lib.stream()), "stes_distill_bwd")
     ref = SO.topk_distill(_np(s), _np(idx), _np(val), tau, None, 3.0)
     _check(d, ref["dlogits"], ref["dlogits_err"], "dlogits")
+
+
+def test_streams_from_outside_keep_no_workspaces():
+    """A stream that torch did not make may be destroyed and its handle given out again: nothing is kept for it."""
+    from spot_amd import lib
+    from spot_amd.distill import topk_distill_grad
+    from spot_amd.recurrence import gated_scan
+    pre, start, _, _, _ = _scan_inputs(2, 900, 96, BF, False, "rows", seed=8)
+    s, idx, val, _ = _kl_inputs(5000, 40, 4, F32, 1)
+    p, h0, c = pre.cuda().requires_grad_(), start.cuda(), (s.cuda(), idx.cuda(), val.cuda())
+
+    def work():
+        h, last = gated_scan(p, h0)
+        return (h.detach(), last.detach(), torch.autograd.grad(h, p, torch.ones_like(h))[0]) + topk_distill_grad(*c)
+    want = work()
+    mine = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    before = lib.native().kept_streams()
+    got = []
+    with torch.cuda.stream(torch.cuda.ExternalStream(mine.cuda_stream)):
+        for _ in range(3):
+            got.append(work())
+    torch.cuda.synchronize()
+    assert lib.native().kept_streams() == before
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
