@@ -275,10 +275,14 @@ class E2EModel(BaseRGBModel):
         return scores, loc
 
     # ------------------------------------------------------------------ frame streams (minGRU heads)
+    def _check_causal(self):
+        """(channel attention gates a clip's frames by their mean over the whole clip, later frames among them)"""
+        if self._temporal_arch != "mingru" or self._model.time_backward or self._model._use_channel_attention:
+            raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward and without use_channel_attention")
+
     def new_stream(self, n=1):
         """The head's state at the start of n frame streams, for predict_stream: fp32 [n, hidden] per layer."""
-        if self._temporal_arch != "mingru" or self._model.time_backward:
-            raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
+        self._check_causal()
         return [h.detach().to(self.device, torch.float32).expand(n, -1).clone() for h in self._model._pred_fine.h0]
 
     def _check_state(self, seq, state):
@@ -303,8 +307,7 @@ class E2EModel(BaseRGBModel):
         the leading dimension will do), while the
         minGRU head runs over a stream's W * T frames as one sequence that starts where the last call's ended: a video's scores
         do not depend on how it is cut into calls."""
-        if self._temporal_arch != "mingru" or self._model.time_backward:
-            raise NotImplementedError("frame streams need a causal head: temporal_arch mingru without time_backward")
+        self._check_causal()
         if seq.dim() == 4:
             seq = seq.unsqueeze(0)
         self._check_state(seq, state)
