@@ -10,6 +10,7 @@ gradients in `.grad` (views of the engine's flat gradient buffer), so the refere
 """
 from __future__ import annotations
 
+import math
 from contextlib import nullcontext
 
 import numpy as np
@@ -334,6 +335,15 @@ class E2EModel(BaseRGBModel):
         eng = m.engine
         if frame.shape[1] != m._clip_len and m._require_clip_len > 0:
             raise lib.StesError("train_step expects clips of exactly clip_len frames")
+        if m.time_backward:                                      # as Impl.forward turns its clips round; what belongs to their frames goes along
+            B, T = frame.shape[:2]
+
+            def turned(t, *tail):
+                return t if t is None or t.numel() != B * T * math.prod(tail) else t.reshape(B, T, *tail).flip(1)
+            frame, label, xy = frame.flip(1), turned(label), turned(xy, 2)
+            if distill is not None:
+                distill = {**distill, "idx": turned(distill["idx"], *distill["idx"].shape[-1:]), "val": turned(distill["val"], *distill["val"].shape[-1:]),
+                           "frame_weight": turned(distill.get("frame_weight"))}
         eng.forward(frame, train=True)
         eng.attach_grads(zero=True)
         out = eng.loss_backward(label.reshape(-1), xy.reshape(-1, 2) if xy is not None else None, self._num_classes,
