@@ -518,7 +518,7 @@ __global__ __launch_bounds__(1024) void scan_dh0_sum_kernel(const float* __restr
 // ---------------------------------------------------------------- host
 constexpr int CT = 64;                       // channels of a tile, of either type
 
-int blocks_of(int T) { return (T + STES_SCAN_BLOCK - 1) / STES_SCAN_BLOCK; }
+int blocks_of(int T) { return T / STES_SCAN_BLOCK + (T % STES_SCAN_BLOCK != 0); }
 // words of one kind in the workspace
 long words_of(int B, int T, int H) { return (long)blocks_of(T) * B * ((H + CT - 1) / CT * CT); }
 

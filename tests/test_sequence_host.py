@@ -78,3 +78,17 @@ def test_shared_memory_against_sets_of_elements(share):
         assert not truth or share(a, b), (a, b)
         wrong += share(a, b) and not truth
     assert wrong == 0
+
+
+@pytest.mark.parametrize("T", [2**31 - 1, 2**31 - 200, 2**31 - 255, 2**31 - 511])
+def test_scan_refuses_lengths_next_to_the_end_of_32_bits(T):
+    import ctypes as C
+    from spot_amd import lib
+    L = lib.lib()
+    assert L.stes_gated_scan_ws_bytes(1, T, 1) == 256 + 16 * 64 * (-(-T // 256))
+    a = lib.GatedScanArgs()
+    for n, v in dict(pre=1 << 40, ld_pre=2, bs_pre=2 * T, h=2 << 40, ld_h=1, bs_h=T, h_last=3 << 40, bs_hl=1, states=4 << 40, dpre=5 << 40, ld_dpre=2, bs_dpre=2 * T,
+                     ws=6 << 40, ws_bytes=1 << 38, B=1, T=T, H=1).items():
+        setattr(a, n, v)
+    for e in (L.stes_gated_scan_fwd, L.stes_gated_scan_bwd):
+        assert e(C.byref(a), None) == lib.ERR_UNSUPPORTED
