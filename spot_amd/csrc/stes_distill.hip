@@ -175,14 +175,15 @@ __device__ __forceinline__ float row_factor(const stes_distill_args& p, float sc
     return bad ? __builtin_nanf("") : f;
 }
 
-// A lane's part of KL / ln 2 = sum P (log2 P - log2 q), for a class of probability P and logit s; ls = log2(sum)
-__device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, float ct) { return P * (log2_(P) - ((s - mx) * ct - ls)); }
+// A lane's part of KL tau / 4 = sum P (log P - log q) tau / 4, for a class of probability P and logit s; ls = log2(sum), tl = tau ln 2 / 4.
+// Logits of the type's lowest value stay finite in it: nothing multiplies their distance from the maximum by more than 1.
+__device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, float tl) { return P * (tl * (log2_(P) + ls) - (0.25f * s - 0.25f * mx)); }
 
 constexpr int MAX_ROUNDS = 1 << 22;                  // (an exit for broken zeros: the loss becomes NaN)
 
-// A workgroup's part of the loss (`sum` is thread 0's); the only one of a launch is the loss.  With `p.zeros` the workgroups hand their
-// parts to the last one, which adds them up in an order of its own: words that are valid when they are not zero, in relaxed atomics of
-// agent scope, and it leaves them zero.  One workgroup waits and the others wait for nothing: every wait ends.  Without them, and from
+// A workgroup's part of the loss (`sum` is thread 0's, in 64 bits: rows near 3e38 may pass fp32's range together, before `factor` divides them);
+// the only one of a launch is the loss.  With `p.zeros` the workgroups hand their parts to the last one, which adds them up in an order of its own: words that are valid when they are not zero (a part of 0 is 5e-324 instead), in relaxed
+// atomics of agent scope, and it leaves them zero.  One workgroup waits and the others wait for nothing: every wait ends.  Without them, and from
 // 16 parts a thread on, where reading them one after the other takes longer than a launch, distill_sum_kernel adds up.  Loss and
 // gradient of 1,024 x 7 4.4 us (two launches 6.3, one workgroup in one launch 9.7), of 16,384 x 1,000 20.4 (21.1); loss of 30,000 x 600,
 // 7,500 parts for 256 threads, 23.8 (22.6).
@@ -190,21 +191,23 @@ __host__ __device__ inline bool in_one_launch(const stes_distill_args& p, int bl
     return blocks == 1 || (p.zeros && blocks <= STES_DISTILL_WORDS && blocks <= 16 * threads);
 }
 
+__device__ __forceinline__ uint64_t part_word(double sum) { const uint64_t w = (uint64_t)__double_as_longlong(sum); return w ? w : 1u; }
+
 template <int BLOCK>
 __device__ __forceinline__ void hand_over(const stes_distill_args& p, double sum, double factor, double* red) {
     if (gridDim.x == 1 || !in_one_launch(p, gridDim.x, BLOCK)) {
         if (threadIdx.x == 0) {
             if (gridDim.x == 1) *p.loss = (float)(sum * factor);
-            else p.ws[blockIdx.x] = (float)sum;
+            else ((double*)p.ws)[blockIdx.x] = sum;
         }
         return;
     }
     const int n = gridDim.x - 1;
     if (blockIdx.x != n) {
-        if (threadIdx.x == 0) __hip_atomic_store(p.zeros + blockIdx.x, ((uint64_t)__float_as_uint((float)sum) << 32) | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) __hip_atomic_store(p.zeros + blockIdx.x, part_word(sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return;
     }
-    double s = threadIdx.x == 0 ? (double)(float)sum : 0.0;
+    double s = threadIdx.x == 0 ? sum : 0.0;
     for (int i = threadIdx.x; i < n; i += 4 * BLOCK) {
         uint64_t w[4];
         bool all = false;
@@ -218,7 +221,7 @@ __device__ __forceinline__ void hand_over(const stes_distill_args& p, double sum
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            s += all ? (double)__uint_as_float((uint32_t)(w[u] >> 32)) : __builtin_nan("");
+            s += all ? __longlong_as_double((long long)w[u]) : __builtin_nan("");
             if (i + u * BLOCK < n) __hip_atomic_store(p.zeros + i + u * BLOCK, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill
 #pragma unroll
         for (int e = 0; e < E; ++e) mine[e * G + l] = 0.f;
     }
-    const float ct = LOG2E / p.temperature;
+    const float ct = LOG2E / p.temperature, tl = p.temperature * (0.25f * LN2);
     const long first = (long)blockIdx.x * rounds * RPB + threadIdx.x / G;
     double total = 0.0;
     ShortRow<TS, G, E> next;
@@ -300,9 +303,9 @@ __global__ __launch_bounds__(BLOCK) void distill_short_kernel(const stes_distill
         }
         if (MODE & LOSS) {
             const float st = t.at >= 0 ? (float)((const TS*)p.logits)[m * p.ld + t.at] : 0.f;
-            float kl = LN2 * group_sum<G>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), ct) : 0.f);
+            float kl = group_sum<G>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), tl) : 0.f);
             if (t.bad) kl = __builtin_nanf("");
-            if (counts && l == 0) total += (double)(w * kl);
+            if (counts && l == 0) total += (double)w * kl;
         }
         if (MODE & GRAD) {
             if (t.at >= 0) mine[t.at] = t.p;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM, TEAM == 64 ? 7 : 1) void d
     const int lane = threadIdx.x & 63, i0 = threadIdx.x % TEAM;
     const long m = (long)blockIdx.x * RPB + threadIdx.x / TEAM;
     const bool row = m < p.M;
-    float out = 0.f;
+    double out = 0.0;
     if (row) {
         // (the list first: 8,192 x 32,003 bf16, 32 listed: loss 108 to 105 us, gradient 207 to 201, both 207 to 203.5)
         const Listed listed = load_listed(p, m, true, lane);
@@ -471,9 +474,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM, TEAM == 64 ? 7 : 1) void d
         }
         if (!(MODE & STATS_IN) && p.stats && i0 == 0) { p.stats[2 * m] = mx; p.stats[2 * m + 1] = sum; }
         if ((MODE & LOSS) && threadIdx.x % TEAM < 64) {
-            float kl = LN2 * group_sum<64>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), ct) : 0.f);
+            float kl = group_sum<64>(t.at >= 0 ? kl_part(t.p, st, mx, log2_(sum), p.temperature * (0.25f * LN2)) : 0.f);
             if (t.bad) kl = __builtin_nanf("");
-            out = counts ? w * kl : 0.f;
+            out = counts ? (double)w * kl : 0.0;
         }
         if (MODE & GRAD) {
             TG* d = (TG*)p.dlogits + m * p.ld_d;
@@ -512,16 +515,16 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM, TEAM == 64 ? 7 : 1) void d
     }
     if (MODE & LOSS) {
         if (TEAM == 64) {
-            if (lane == 0) red[threadIdx.x >> 6] = out;
+            if (lane == 0) parts[threadIdx.x >> 6] = out;
             __syncthreads();
-            out = (red[0] + red[1]) + (red[2] + red[3]);
+            out = (parts[0] + parts[1]) + (parts[2] + parts[3]);
         }
         hand_over<BLOCK>(p, out, factor, parts);
     }
 }
 
 // loss = factor * (part[0] + part[1] + ...), in a fixed order
-__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restrict__ part, int n, double factor, float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void distill_sum_kernel(const double* __restrict__ part, int n, double factor, float* __restrict__ loss) {
     __shared__ double red[16];
     double s = 0.0;
 #pragma unroll 4
@@ -568,7 +571,7 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     STES_CHECK(!bwd || (a->stats && a->dlogits), STES_ERR_ARG, "stes_distill_bwd: stats and dlogits are needed");
     STES_CHECK((uintptr_t)a->zeros % 8 == 0, STES_ERR_ARG, "stes_distill: zeros is aligned to 8 bytes");
     const int64_t need = bwd ? 0 : stes_distill_ws_floats(a->M, a->V, a->k, a->zeros != nullptr);
-    STES_CHECK(!need || (a->ws && a->ws_floats >= need), STES_ERR_ARG, "stes_distill: workspace too small");
+    STES_CHECK(!need || (a->ws && a->ws_floats >= need && (uintptr_t)a->ws % 8 == 0), STES_ERR_ARG, "stes_distill: workspace too small or not aligned to 8 bytes");
     const int64_t M = a->M;
     const StesRows d{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, ins[4] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V},
         {a->idx, a->idx_i64 ? 8 : 4, a->ld_idx, 0, M, 1, a->k}, {a->val, a->val_f32 ? 4 : 2, a->ld_val, 0, M, 1, a->k}, {a->weight, 4, M, 0, 1, 1, M}};
@@ -576,7 +579,7 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     return STES_OK;
 }
 
-double loss_factor(const stes_distill_args& a) { return (double)a.temperature * a.temperature / a.denom; }
+double loss_factor(const stes_distill_args& a) { return 4.0 * a.temperature / a.denom; }          // (the rows' parts are KL tau / 4)
 float grad_factor(const stes_distill_args& a) { return (float)((double)a.grad_scale * a.temperature / a.denom); }
 
 template <typename TS, typename TG, int G, int E, int MODE>
@@ -646,7 +649,7 @@ int launch(const stes_distill_args& a, bool bwd, hipStream_t s) {
 extern "C" int64_t stes_distill_ws_floats(int M, int V, int k, int with_zeros) {
     if (M <= 1) return 0;
     const int blocks = V <= 8 * 64 ? short_blocks(M, 256 / lanes_of(V, k)) : M;          // (or fewer)
-    return blocks == 1 || (with_zeros && blocks <= 16 * 256) ? 0 : blocks;
+    return blocks == 1 || (with_zeros && blocks <= 16 * 256) ? 0 : 2 * (int64_t)blocks;          // (of 64 bits each)
 }
 
 extern "C" int stes_distill(const stes_distill_args* a, void* stream) {
@@ -658,7 +661,7 @@ extern "C" int stes_distill(const stes_distill_args* a, void* stream) {
         STES_LAUNCH_CHECK();
     }
     if (parts || !a->M) {                                    // (no rows: a sum of nothing)
-        hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a->ws, parts, loss_factor(*a), a->loss);
+        hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const double*)a->ws, parts, loss_factor(*a), a->loss);
         STES_LAUNCH_CHECK();
     }
     return STES_OK;

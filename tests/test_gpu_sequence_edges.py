@@ -232,3 +232,17 @@ def test_streams_from_outside_keep_no_workspaces():
     torch.cuda.synchronize()
     assert lib.native().kept_streams() == before
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+@pytest.mark.parametrize("V", [6, 300, 700, 9000, 80000])
+@pytest.mark.parametrize("dtype,tau", [(F32, 1.0), (BF, 1.0), (F32, 0.5), (BF, 4.0)])
+def test_distill_listed_classes_at_the_lowest_value(V, dtype, tau):
+    """A class that the teacher lists and the student masks with the type's lowest value: the divergence is of the order of 3e38 and finite, in
+    one row and where several rows' sum alone passes the range of fp32."""
+    M = 9
+    s, idx, val, w = _kl_inputs(M, V, 2, dtype, V + 1, False, True)
+    for m in (1, 2, 3, 4, 8):
+        s[m, idx[m, m % 2]] = torch.finfo(dtype).min
+    ref = _kl_compare(s, idx, val, None, tau, denom=100.0)
+    assert np.isfinite(ref["loss"]) and 1e36 < ref["loss"] < 1e38
+    _kl_compare(s, idx, val, 4 * w, tau, denom=1000.0)
