@@ -513,9 +513,10 @@ int stes_loss(const float* logits, int64_t ldl, const float* loc, int64_t ldloc,
  * stes_distill: loss [1] and, when dlogits is given, the gradient in the same pass over the logits; stats [M][2] (optional):
  * the row's maximum and its sum of exp((logits - max) / tau), from which stes_distill_bwd computes the gradient later (what a row
  * that adds nothing to the loss holds there is not specified).
- * dlogits: fp32 (d_f32) or bf16, written, or added to when accumulate != 0; it must not overlap logits.  Columns from V up are
- * not touched.  ws: stes_distill_ws_floats(M, V, k, zeros != NULL) floats, aligned to 8 bytes.  zeros (optional): STES_DISTILL_WORDS
- * zero words, which the call may use and leaves zero; it then needs one launch instead of two where its workgroups are few enough.  Calls that
+ * dlogits: fp32 (d_f32) or bf16, written, or added to when accumulate != 0.  Nothing that a call writes may overlap anything else that it is
+ * given.  Columns from V up are not touched.  ws: stes_distill_ws_floats(M, V, k, zeros != NULL) floats, aligned to 8 bytes.  zeros
+ * (optional): STES_DISTILL_WORDS zero words, which the call may use and leaves zero; it then needs one launch instead of two where its
+ * workgroups are few enough.  Calls that
  * may overlap need other zeros each.  M = 0 is a call (loss 0).  Sums over rows are taken in 64 bits, in
  * a fixed order (which may be another with dlogits than without, and with zeros than without). */
 #define STES_DISTILL_MAX_K 64

@@ -573,9 +573,12 @@ int distill_check(const stes_distill_args* a, bool bwd) {
     const int64_t need = bwd ? 0 : stes_distill_ws_floats(a->M, a->V, a->k, a->zeros != nullptr);
     STES_CHECK(!need || (a->ws && a->ws_floats >= need && (uintptr_t)a->ws % 8 == 0), STES_ERR_ARG, "stes_distill: workspace too small or not aligned to 8 bytes");
     const int64_t M = a->M;
-    const StesRows d{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, ins[4] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V},
-        {a->idx, a->idx_i64 ? 8 : 4, a->ld_idx, 0, M, 1, a->k}, {a->val, a->val_f32 ? 4 : 2, a->ld_val, 0, M, 1, a->k}, {a->weight, 4, M, 0, 1, 1, M}};
-    for (const StesRows& r : ins) STES_CHECK(!stes_share(d, r), STES_ERR_ARG, "stes_distill: dlogits shares memory with what the call reads");
+    const StesRows stats = stes_flat(a->stats, 4, 2 * M), none{};
+    const StesRows outs[5] = {{a->dlogits, a->d_f32 ? 4 : 2, a->ld_d, 0, M, 1, a->V}, stes_flat(bwd ? nullptr : a->loss, 4, 1), bwd ? none : stats, stes_flat(a->ws, 4, need),
+                              stes_flat(bwd || M == 1 ? nullptr : a->zeros, 4, 2 * STES_DISTILL_WORDS)};
+    const StesRows ins[6] = {{a->logits, a->f32 ? 4 : 2, a->ld, 0, M, 1, a->V}, {a->idx, a->idx_i64 ? 8 : 4, a->ld_idx, 0, M, 1, a->k}, {a->val, a->val_f32 ? 4 : 2, a->ld_val, 0, M, 1, a->k},
+                             stes_flat(a->weight, 4, M), stes_flat(a->upstream, 4, 1), bwd ? stats : none};
+    STES_CHECK(!stes_any_shared(outs, ins), STES_ERR_ARG, "stes_distill: what a call writes shares memory with what else it writes or reads");
     return STES_OK;
 }
 

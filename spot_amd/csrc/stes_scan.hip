@@ -561,12 +561,10 @@ int scan_check(const stes_gated_scan_args* a, bool bwd) {
         dh{a->dh, es, a->ld_dh, a->bs_dh, T, B, H}, dlast{a->dh_last, 4, 0, a->bs_dhl, 1, a->bs_dhl ? B : 1, H},
         dpre{a->dpre, es, a->ld_dpre, a->bs_dpre, T, B, 2 * H}, dh0{a->dh0, 4, 0, H, 1, B, H}, total{a->dh0_sum, 4, 0, H, 1, 1, H};
     const StesRows none{};
-    const StesRows outs[3] = {bwd ? dpre : h, bwd ? dh0 : last, bwd ? total : states}, ins[5] = {pre, len, bwd ? states : h0, bwd ? dh : none, bwd ? dlast : none};
-    for (int i = 0; i < 3; ++i) {
-        for (int j = 0; j < 5; ++j)
-            STES_CHECK((i == 1 && j == 2 && !bwd && a->h_last == a->h0) || !stes_share(outs[i], ins[j]), STES_ERR_ARG, "stes_gated_scan: what a call writes shares memory with what it reads");
-        for (int j = 0; j < i; ++j) STES_CHECK(!stes_share(outs[i], outs[j]), STES_ERR_ARG, "stes_gated_scan: two results share memory");
-    }
+    const StesRows outs[5] = {bwd ? dpre : h, bwd ? dh0 : last, bwd ? total : states, stes_flat(a->ws, 1, stes_gated_scan_ws_bytes(a->B, a->T, a->H)),
+                              stes_flat(a->scrub, 1, a->scrub_bytes)}, ins[5] = {pre, len, bwd ? states : h0, bwd ? dh : none, bwd ? dlast : none};
+    const bool in_place = !bwd && a->h_last == a->h0;                       // (checked above)
+    STES_CHECK(!stes_any_shared(outs, ins, in_place ? 1 : -1, 2), STES_ERR_ARG, "stes_gated_scan: what a call writes shares memory with what else it writes or reads");
     return STES_OK;
 }
 

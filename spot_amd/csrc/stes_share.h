@@ -39,3 +39,17 @@ static inline bool stes_share(StesRows a, StesRows b) {
     }
     return false;
 }
+
+static inline StesRows stes_flat(const void* p, int es, int64_t n) { return StesRows{p, es, n, n, 1, 1, n}; }
+
+// Whether anything that a call writes shares memory with something else that it writes or reads, but for the pair (fine_out, fine_in).
+template <int N, int M>
+static inline bool stes_any_shared(const StesRows (&outs)[N], const StesRows (&ins)[M], int fine_out = -1, int fine_in = -1) {
+    for (int i = 0; i < N; ++i) {
+        for (int j = 0; j < M; ++j)
+            if (!(i == fine_out && j == fine_in) && stes_share(outs[i], ins[j])) return true;
+        for (int j = 0; j < i; ++j)
+            if (stes_share(outs[i], outs[j])) return true;
+    }
+    return false;
+}

@@ -92,3 +92,54 @@ def test_scan_refuses_lengths_next_to_the_end_of_32_bits(T):
         setattr(a, n, v)
     for e in (L.stes_gated_scan_fwd, L.stes_gated_scan_bwd):
         assert e(C.byref(a), None) == lib.ERR_UNSUPPORTED
+
+
+def _refused(entry, cls, base, kw):
+    import ctypes as C
+    from spot_amd import lib
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses: only where nothing can be launched")
+    a = getattr(lib, cls)()
+    for n, v in {**base, **kw}.items():
+        setattr(a, n, v)
+    return getattr(lib.lib(), entry)(C.byref(a), None) == -1 and b"share" in lib.lib().stes_last_error()
+
+
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("kw", [dict(loss=MB + 40), dict(loss=2 * MB), dict(loss=3 * MB + 4), dict(weight=4 * MB), dict(loss=8 * MB, weight=8 * MB - 8), dict(loss=5 * MB + 12),
+                                dict(stats=MB + 8), dict(stats=4 * MB), dict(stats=5 * MB + 4), dict(stats=2 * MB - 4), dict(ws=MB + 64), dict(ws=5 * MB), dict(stats=9 * MB, ws=9 * MB),
+                                dict(ws=6 * MB - 8, loss=6 * MB), dict(zeros=MB - 65528), dict(zeros=5 * MB - 8), dict(upstream=5 * MB), dict(upstream=6 * MB), dict(zeros=6 * MB - 16)])
+def test_distill_refuses_results_and_workspaces_that_share_memory(kw):
+    base = dict(logits=MB, ld=600, f32=1, idx=2 * MB, ld_idx=4, val=3 * MB, ld_val=4, val_f32=1, M=30, V=600, k=4, temperature=1.0, denom=3.0, grad_scale=1.0,
+                dlogits=5 * MB, ld_d=600, d_f32=1, loss=6 * MB, ws=7 * MB, ws_floats=1 << 20)
+    if "weight" in kw and "loss" not in kw:
+        kw = {**kw, "dlogits": 4 * MB - 8}
+    if kw.get("stats") == 4 * MB:
+        kw = {**kw, "weight": 4 * MB + 8}
+    assert _refused("stes_distill", "DistillArgs", base, kw)
+
+
+@pytest.mark.parametrize("kw", [dict(stats=5 * MB - 8), dict(stats=8 * MB, dlogits=8 * MB + 16), dict(upstream=5 * MB + 600)])
+def test_distill_backward_refuses_a_gradient_over_what_it_reads(kw):
+    base = dict(logits=MB, ld=600, f32=1, idx=2 * MB, ld_idx=4, val=3 * MB, ld_val=4, val_f32=1, M=30, V=600, k=4, temperature=1.0, denom=3.0, grad_scale=1.0,
+                dlogits=5 * MB, ld_d=600, d_f32=1, stats=9 * MB)
+    assert _refused("stes_distill_bwd", "DistillArgs", base, kw)
+
+
+@pytest.mark.parametrize("bwd", [False, True])
+@pytest.mark.parametrize("kw", [dict(ws=MB), dict(ws=2 * MB), dict(ws=3 * MB), dict(ws=4 * MB), dict(scrub=MB, scrub_bytes=16), dict(scrub=3 * MB + 16, scrub_bytes=16), dict(scrub=6 * MB + 16, scrub_bytes=16),
+                                dict(scrub=4 * MB, scrub_bytes=32)])
+def test_scan_refuses_workspaces_that_share_memory(kw, bwd):
+    if bwd:
+        base = dict(pre=MB, ld_pre=16, bs_pre=16000, dpre=2 * MB, ld_dpre=16, bs_dpre=16000, dh0=3 * MB, states=4 * MB, ws=6 * MB, ws_bytes=1 << 19, B=2, T=1000, H=8)
+    else:
+        base = dict(pre=MB, ld_pre=16, bs_pre=16000, h=2 * MB, ld_h=8, bs_h=8000, h_last=3 * MB, bs_hl=8, states=4 * MB, ws=6 * MB, ws_bytes=1 << 19, B=2, T=1000, H=8)
+    assert _refused("stes_gated_scan_bwd" if bwd else "stes_gated_scan_fwd", "GatedScanArgs", base, kw)
+
+
+def test_small_tensors_between_the_rows_of_a_gradient_do_not_share_memory(share):
+    d = (MB, 4, 700, 0, 30, 1, 600)
+    for at, n, want in ((600, 100, False), (600, 101, True), (599, 1, True), (1300, 1, False), (699, 1, False), (700, 1, True), (29 * 700 + 600, 10000, False)):
+        assert share(d, (MB + 4 * at, 4, n, n, 1, 1, n)) is want
