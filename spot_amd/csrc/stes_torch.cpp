@@ -152,6 +152,18 @@ Streams& streams() {
     return *s;
 }
 
+// The lock of a stream's workspaces.  Its holder allocates, and an allocation that Python watches (torch's memory history, dispatch modes) needs the
+// interpreter: a Python thread that waits for the lock lets go of it.
+std::unique_lock<std::mutex> hold(std::mutex& lock) {
+    std::unique_lock<std::mutex> held(lock, std::try_to_lock);
+    if (!held.owns_lock()) {
+        std::optional<pybind11::gil_scoped_release> others;
+        if (PyGILState_Check()) others.emplace();
+        held.lock();
+    }
+    return held;
+}
+
 std::shared_ptr<Kept> kept(int device, void* stream) {
     Streams& s = streams();
     std::shared_ptr<Kept> oldest;           // (freed after the lock)
@@ -180,7 +192,7 @@ void scan_call(int (*entry)(const stes_gated_scan_args*, void*), const char* nam
         return check(entry(&a, s), name);
     }
     const auto k = kept(dev.index(), s);
-    std::lock_guard<std::mutex> g(k->lock);
+    const auto held = hold(k->lock);
     if (!k->pair[0].defined() || k->pair[0].numel() < n) {
         k->pair[0] = Tensor();
         Tensor one = at::zeros({n}, bytes), two = at::zeros({n}, bytes);
@@ -396,7 +408,7 @@ Tensor distill_call(stes_distill_args& a, const Tensor& logits) {
     std::shared_ptr<Kept> k;
     if (a.M > 1 && !capturing() && lasts(logits.device())) {          // (a graph may be replayed on any stream, next to others)
         k = kept(logits.device().index(), s);
-        std::lock_guard<std::mutex> g(k->lock);
+        const auto held = hold(k->lock);
         if (!k->zeros.defined()) k->zeros = at::zeros({STES_DISTILL_WORDS}, logits.options().dtype(at::kLong));
         a.zeros = static_cast<uint64_t*>(k->zeros.data_ptr());
     }
@@ -530,8 +542,8 @@ PYBIND11_MODULE(_stes_torch, m) {
         }
     });
     m.def("set_error", [](py::object type) { stes_error = type.release().ptr(); });
-    m.def("keep_streams", [](size_t most) { std::swap(streams().most, most); return most; }, "How many streams' workspaces are kept; returns what it was");
-    m.def("kept_streams", []() { return streams().all.size(); });
+    m.def("keep_streams", [](size_t most) { std::lock_guard<std::mutex> g(streams().lock); std::swap(streams().most, most); return most; }, "How many streams' workspaces are kept; returns what it was");
+    m.def("kept_streams", []() { std::lock_guard<std::mutex> g(streams().lock); return streams().all.size(); });
     m.def("gated_scan", &gated_scan);
     m.def("topk_distill_loss", &topk_distill_loss);
     m.def("topk_distill_grad", &topk_distill_grad);

@@ -246,3 +246,29 @@ def test_distill_listed_classes_at_the_lowest_value(V, dtype, tau):
     ref = _kl_compare(s, idx, val, None, tau, denom=100.0)
     assert np.isfinite(ref["loss"]) and 1e36 < ref["loss"] < 1e38
     _kl_compare(s, idx, val, 4 * w, tau, denom=1000.0)
+
+
+def test_threads_on_one_stream_while_allocations_are_recorded():
+    """Recording an allocation takes the interpreter's lock: a thread that waits for the workspaces that another one allocates must not keep it."""
+    import threading
+    from spot_amd.recurrence import gated_scan
+    torch.cuda.synchronize()
+    shared, done = torch.cuda.Stream(), []
+
+    def work(k):
+        with torch.cuda.stream(shared):
+            for i in range(1, 16):                          # (growing: every call allocates its workspaces anew)
+                p = torch.zeros(1, 300, 32 * (16 * k + i), device="cuda", requires_grad=True)
+                h, _ = gated_scan(p)
+                g, = torch.autograd.grad(h, p, torch.ones_like(h))
+                done.append(bool(g.any()))
+    torch.cuda.memory._record_memory_history("all", stacks="python", max_entries=1000)
+    try:
+        threads = [threading.Thread(target=work, args=(k,), daemon=True) for k in range(3)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(30)
+    finally:
+        torch.cuda.memory._record_memory_history(None)
+    assert len(done) == 45
