@@ -272,3 +272,12 @@ def test_threads_on_one_stream_while_allocations_are_recorded():
     finally:
         torch.cuda.memory._record_memory_history(None)
     assert len(done) == 45
+
+
+@pytest.mark.parametrize("T", [0, 5, 300])
+def test_gated_scan_of_no_sequences_has_a_zero_gradient_of_the_shared_state(T):
+    from spot_amd.recurrence import gated_scan
+    p, s = torch.zeros(0, T, 16, device="cuda", requires_grad=True), torch.randn(8, device="cuda", requires_grad=True)
+    h, last = gated_scan(p, s)
+    g = torch.autograd.grad((h, last), (p, s), (torch.ones_like(h), torch.ones_like(last)))
+    assert g[0].shape == p.shape and g[1].shape == (8,) and not bool(g[1].any())

@@ -143,3 +143,60 @@ def test_small_tensors_between_the_rows_of_a_gradient_do_not_share_memory(share)
     d = (MB, 4, 700, 0, 30, 1, 600)
     for at, n, want in ((600, 100, False), (600, 101, True), (599, 1, True), (1300, 1, False), (699, 1, False), (700, 1, True), (29 * 700 + 600, 10000, False)):
         assert share(d, (MB + 4 * at, 4, n, n, 1, 1, n)) is want
+
+
+class _Engine:
+    def __init__(self):
+        self.flat, self.flat_grad, self.weights_dirty = torch.zeros(8), torch.zeros(8), False
+
+
+class _Recorder:
+    """The model side of DataParallelTrainer: keeps what the trainer hands to the step."""
+
+    def __init__(self):
+        self._model = torch.nn.Linear(1, 1)
+        self._model.engine = _Engine()
+        self.seen = []
+
+    def train_step(self, frame, label, xy, lr, **kw):
+        self.seen.append((kw["distill"], kw["ext_denoms"]))
+        for lo, hi in ((4, 8), (0, 4)):
+            kw["on_ready"](lo, hi)
+        kw["after_backward"](self._model.engine)
+        return torch.zeros(8)
+
+
+def _denominator_worker(rank, world, port, q):
+    import os
+    import torch.distributed as dist
+    from spot_amd.dp import DataParallelTrainer
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    m = _Recorder()
+    t = DataParallelTrainer(m, dist)
+    label = torch.zeros(3, 5, dtype=torch.int64)
+    label[rank, 2] = 1
+    given = {"idx": torch.zeros(3, 5, 2), "val": torch.zeros(3, 5, 2), "weight": 0.5}
+    for d in (given, {**given, "denom": None}, {**given, "denom": 7.0}, None):
+        m._model.engine.flat_grad.fill_(rank + 1.0)
+        t.step(None, label, None, distill=d)
+    q.put((rank, [None if d is None else (d["denom"], d["weight"]) for d, _ in m.seen], m.seen[0][1].tolist(), m._model.engine.flat_grad.tolist(), "denom" in given))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_distillation_denominator_counts_the_frames_of_all_ranks_gloo():
+    from test_host_logic import _spawn_gloo
+    for rank, seen, denoms, grad, touched in _spawn_gloo(_denominator_worker):
+        assert seen == [(30.0, 0.5), (30.0, 0.5), (7.0, 0.5), None] and not touched
+        assert denoms == [28 + 2 * 5.0, 2.0] and grad == [3.0] * 8
+
+
+def test_distillation_denominator_of_one_process_is_the_callers():
+    from spot_amd.dp import DataParallelTrainer
+    m = _Recorder()
+    m.train_step = lambda *a, **kw: m.seen.append(kw["distill"])
+    d = {"idx": 0, "val": 0}
+    DataParallelTrainer(m).step(None, torch.zeros(3, 5), None, distill=d)
+    assert m.seen == [d]
