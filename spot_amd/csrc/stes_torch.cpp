@@ -12,6 +12,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_map>
 #include <vector>
 
 #include <ATen/ATen.h>
@@ -97,22 +98,43 @@ bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradM
 
 // ---------------------------------------------------------------- leaves
 // The node that accumulates a leaf's gradient keeps the stream on which it was made for as long as some autograd graph holds it, whoever made
-// that graph; a captured backward pass makes that stream wait for the capture's, which ends the process where it is not part of the
-// capture (the default stream cannot be).  A captured call refuses such leaves.
+// that graph; a captured backward pass makes that stream wait for the capture's, which ends the process where an eager graph made the
+// node (the default stream cannot be part of a capture).  A captured call refuses such leaves, and notes those that it finds in order: a later
+// capture on another stream may meet them while this one's outputs live.
+struct Leaves {
+    std::mutex lock;
+    std::unordered_map<Node*, std::weak_ptr<Node>> captured;
+    size_t sweep = 64;
+};
+Leaves& leaves() {
+    static Leaves* all = new Leaves;                  // (never destroyed: autograd's threads outlive main)
+    return *all;
+}
+
+// The inputs' edges into the graph, held while they are looked at: leaves' nodes live as long as something holds them.
 torch::autograd::edge_list guarded(torch::autograd::edge_list edges, c10::Device dev) {
     if (!capturing()) return edges;
     const c10::Stream here = current(dev).unwrap();
+    Leaves& l = leaves();
+    std::lock_guard<std::mutex> g(l.lock);
     for (const auto& e : edges) {
         std::shared_ptr<Node> n = e.function;
         for (int i = 0; i < 4 && n && n->num_outputs() == 1; ++i) n = n->next_edge(0).function;      // (through the views and copies that a call makes of a leaf)
         if (!n || n->num_outputs() != 0) continue;
         const std::optional<c10::Stream> made = n->stream();
-        if (!made || *made == here) continue;
-        if (made->id() != 0) {
+        bool inside = !made || *made == here;
+        if (!inside && made->id() != 0) {
             const c10::StreamGuard there(*made);
-            if (capturing()) continue;                // (another stream of a capture)
+            inside = capturing();                     // (another stream of a capture)
         }
-        refuse("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first");
+        const auto seen = l.captured.find(n.get());
+        if (!inside && (seen == l.captured.end() || seen->second.lock() != n))
+            refuse("an autograd graph from outside this capture still holds one of its leaves: drop its outputs first");
+        l.captured[n.get()] = n;
+    }
+    if (l.captured.size() > l.sweep) {
+        for (auto i = l.captured.begin(); i != l.captured.end();) i = i->second.expired() ? l.captured.erase(i) : std::next(i);
+        l.sweep = 64 + 2 * l.captured.size();
     }
     return edges;
 }

@@ -281,3 +281,19 @@ def test_gated_scan_of_no_sequences_has_a_zero_gradient_of_the_shared_state(T):
     h, last = gated_scan(p, s)
     g = torch.autograd.grad((h, last), (p, s), (torch.ones_like(h), torch.ones_like(last)))
     assert g[0].shape == p.shape and g[1].shape == (8,) and not bool(g[1].any())
+
+
+def test_captures_on_two_streams_share_a_leaf():
+    """The outputs of one capture hold a leaf whose gradient's node was made on that capture's stream: another capture's forward pass takes it."""
+    for leaf, f in _differentiable_calls():
+        want = f(leaf).detach().clone()
+        torch.cuda.synchronize()
+        kept = []
+        for _ in range(2):
+            gr, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            with torch.cuda.graph(gr, stream=side):
+                kept.append((gr, f(leaf), side))
+        for gr, y, _ in kept:
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
