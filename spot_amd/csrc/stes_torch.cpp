@@ -96,6 +96,28 @@ void no_tangents(const char* op, const Tensors&... t) {
 }
 bool asks_for_gradients(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
+// A tensor saved for the backward pass.  Hooks (torch.autograd.graph.saved_tensors_hooks) may give another one back: of the same sizes, type and
+// device, or it is refused, but of any strides.
+struct Saved {
+    SavedVariable variable;
+    std::vector<int64_t> sizes;
+    at::ScalarType type = at::kFloat;
+    c10::Device device = c10::kCPU;
+
+    void operator=(const Tensor& t) {
+        variable = SavedVariable(t, false);
+        sizes = t.sizes().vec(), type = t.scalar_type(), device = t.device();
+    }
+    Tensor unpack() const {
+        Tensor t = variable.unpack();
+        if (t.defined() && (t.sizes() != at::IntArrayRef(sizes) || t.scalar_type() != type || t.device() != device))
+            refuse("a saved ", type, " ", at::IntArrayRef(sizes), " on ", device, " came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+        return t;
+    }
+    Tensor whole() const { const Tensor t = unpack(); return t.defined() ? t.contiguous() : t; }
+    void reset() { variable.reset_data(); }
+};
+
 // ---------------------------------------------------------------- leaves
 // The node that accumulates a leaf's gradient keeps the stream on which it was made for as long as some autograd graph holds it, whoever made
 // that graph; a captured backward pass makes that stream wait for the capture's, which ends the process where an eager graph made the
@@ -237,6 +259,9 @@ constexpr const char* SCAN = "gated_scan: ";
 // (frame stride, sequence stride) of a [B, T, width] tensor; the frame stride of a single frame is immaterial.
 std::pair<int64_t, int64_t> strides(const Tensor& t, int64_t width) { return {t.size(1) > 1 ? t.stride(1) : width, t.stride(0)}; }
 
+// Whether the frames of a [B, T, width] tensor are contiguous and do not overlap.
+bool frames(const Tensor& t) { return t.is_contiguous() || ((t.size(2) <= 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) >= t.size(2))); }
+
 // Stride between the rows of a float32 [B, H] tensor whose rows are contiguous and apart.
 int64_t row_stride(const Tensor& t, int64_t B, int64_t H, const char* name) {
     if (t.scalar_type() != at::kFloat || t.dim() != 2 || t.size(0) != B || t.size(1) != H)
@@ -271,25 +296,26 @@ Scanned scan_forward(const Tensor& pre, const Tensor& h0, const Tensor& lengths,
 }
 
 struct GatedScanBackward : public Node {
-    SavedVariable pre, lengths, states;
+    Saved pre, lengths, states;
     bool reverse = false;
     int h0_dim = 0;                         // of an initial state that asks for a gradient
 
     std::string name() const override { return "GatedScanBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> g(mutex_);
-        pre.reset_data();
-        lengths.reset_data();
-        states.reset_data();
+        pre.reset();
+        lengths.reset();
+        states.reset();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> g(mutex_);
-        const Tensor p = pre.unpack(), n = lengths.unpack(), st = states.unpack();
-        Tensor dpre, dh0, total;
+        Tensor p = pre.unpack(), dpre, dh0, total;
         untraced(SCAN);
         no_tangents(SCAN, grads[0], grads[1]);
         if (grads[0].defined() || grads[1].defined()) {
             const Call call(p.device());
+            const Tensor n = lengths.whole(), st = states.whole();
+            if (!frames(p)) p = p.contiguous();
             const int64_t B = p.size(0), T = p.size(1), W = p.size(2), H = W / 2;
             dpre = fresh({B, T, W}, p);
             if (h0_dim) dh0 = fresh({B, H}, p, at::kFloat);
@@ -299,7 +325,7 @@ struct GatedScanBackward : public Node {
                 stes_gated_scan_args a{};
                 if (dh.defined()) {
                     // (a gradient that was expanded or transposed)
-                    if (!dh.is_contiguous() && ((H > 1 && dh.stride(2) != 1) || (T > 1 && dh.stride(1) < H))) dh = dh.contiguous();
+                    if (!frames(dh)) dh = dh.contiguous();
                     std::tie(a.ld_dh, a.bs_dh) = strides(dh, H);
                 }
                 if (dlast.defined()) dlast = dlast.contiguous();
@@ -340,7 +366,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
     const c10::Device dev = pre.device();
     if (W % 2) refuse(SCAN, "the last dimension of pre holds gates and candidates and is even, got ", W);
     if (std::max({B, T, W}) > INT32_MAX) refuse(SCAN, "sizes beyond 32 bits: ", pre.sizes());
-    if (!pre.is_contiguous() && ((W > 1 && pre.stride(2) != 1) || (T > 1 && pre.stride(1) < W))) refuse(SCAN, "frames of pre must be contiguous and not overlap");
+    if (!frames(pre)) refuse(SCAN, "frames of pre must be contiguous and not overlap");
     if (h0.defined()) {
         const bool rows = h0.dim() == 2 && h0.size(0) == B && h0.size(1) == H;
         if (h0.device() != dev || h0.scalar_type() != at::kFloat || !(rows || (h0.dim() == 1 && h0.size(0) == H)))
@@ -383,9 +409,9 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
         node->set_next_edges(guarded(torch::autograd::collect_next_edges(pre, h0), dev));
         r = scan_forward(pre, h0, lengths, reverse, out, state_out, true);
     }
-    node->pre = SavedVariable(pre, false);
-    if (lengths.defined()) node->lengths = SavedVariable(lengths, false);
-    node->states = SavedVariable(r.states, false);
+    node->pre = pre;
+    if (lengths.defined()) node->lengths = lengths;
+    node->states = r.states;
     node->reverse = reverse;
     node->h0_dim = h0.defined() && h0.requires_grad() ? h0.dim() : 0;
     torch::autograd::set_history(r.h, node);
@@ -468,23 +494,24 @@ Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, d
 }
 
 struct DistillBackward : public Node {
-    SavedVariable logits, idx, val, weight, stats;
+    Saved logits, idx, val, weight, stats;
     double temperature = 1.0, denom = 1.0;
 
     std::string name() const override { return "DistillBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> g(mutex_);
-        for (SavedVariable* v : {&logits, &idx, &val, &weight, &stats}) v->reset_data();
+        for (Saved* v : {&logits, &idx, &val, &weight, &stats}) v->reset();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> g(mutex_);
-        const Rows r{logits.unpack(), idx.unpack(), val.unpack(), weight.unpack(), temperature, denom};
-        const Tensor st = stats.unpack();
+        Rows r{logits.unpack(), Tensor(), Tensor(), Tensor(), temperature, denom};
         Tensor d;
         untraced(KL);
         no_tangents(KL, grads[0]);
         if (grads[0].defined()) {
             const Call call(r.logits.device());
+            const Tensor i = idx.unpack(), v = val.unpack(), st = stats.whole();
+            r.logits = flat(r.logits, r.logits.size(1)), r.idx = flat(i, i.size(1)), r.val = flat(v, v.size(1)), r.weight = weight.whole();
             d = fresh(r.logits.sizes(), r.logits);
             if (r.logits.size(0)) {
                 stes_distill_args a = distill_args(r);
@@ -514,11 +541,11 @@ Tensor topk_distill_loss(const Tensor& logits, const Tensor& idx, const Tensor& 
         a.stats = at_<float>(stats);
         loss = distill_call(a, r.logits);
     }
-    node->logits = SavedVariable(r.logits, false);
-    node->idx = SavedVariable(r.idx, false);
-    node->val = SavedVariable(r.val, false);
-    if (r.weight.defined()) node->weight = SavedVariable(r.weight, false);
-    node->stats = SavedVariable(stats, false);
+    node->logits = r.logits;
+    node->idx = r.idx;
+    node->val = r.val;
+    if (r.weight.defined()) node->weight = r.weight;
+    node->stats = stats;
     node->temperature = r.temperature, node->denom = r.denom;
     torch::autograd::set_history(loss, node);
     return loss;

@@ -297,3 +297,23 @@ def test_captures_on_two_streams_share_a_leaf():
             gr.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, want)
+
+
+def test_saved_tensors_may_come_back_with_other_strides_and_are_refused_as_others():
+    """What hooks give back for a saved tensor: the same values in another layout do, another size or type is refused."""
+    hooks = torch.autograd.graph.saved_tensors_hooks
+
+    def apart(t):                                           # every element on its own, the last dimension outermost
+        if t.dim() < 2 or not t.numel():
+            return torch.stack([t, t], -1)[..., 0]
+        return t.movedim(-1, 0).contiguous().movedim(0, -1)
+    for leaf, f in _differentiable_calls():
+        want, = torch.autograd.grad(f(leaf), leaf)
+        with hooks(lambda t: t.clone(), apart):
+            y = f(leaf)
+        assert torch.equal(torch.autograd.grad(y, leaf)[0], want)
+        for change in (lambda t: t[..., :-1], lambda t: t.double(), lambda t: t.cpu(), lambda t: t[None]):
+            with hooks(lambda t: t, lambda t, change=change: change(t) if t.shape == leaf.shape and t.data_ptr() == leaf.data_ptr() else t):
+                y = f(leaf)
+            with pytest.raises(RuntimeError, match="came back as"):
+                torch.autograd.grad(y, leaf)
