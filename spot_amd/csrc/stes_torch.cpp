@@ -71,6 +71,10 @@ struct Call {
 Tensor fresh(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type)); }
 Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options()); }
 
+// torch only notes some values down: a negative view's memory holds the opposite, a zero tensor has no memory.
+bool noted(const Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+Tensor plain(const Tensor& t) { return !t.defined() || !noted(t) ? t : t._is_zerotensor() ? t.clone() : t.resolve_neg(); }
+
 template <typename T = void> T* at_(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
 bool element(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
@@ -112,7 +116,7 @@ struct Saved {
         Tensor t = variable.unpack();
         if (t.defined() && (t.sizes() != at::IntArrayRef(sizes) || t.scalar_type() != type || t.device() != device))
             refuse("a saved ", type, " ", at::IntArrayRef(sizes), " on ", device, " came back as ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
-        return t;
+        return plain(t);
     }
     Tensor whole() const { const Tensor t = unpack(); return t.defined() ? t.contiguous() : t; }
     void reset() { variable.reset_data(); }
@@ -321,7 +325,7 @@ struct GatedScanBackward : public Node {
             if (h0_dim) dh0 = fresh({B, H}, p, at::kFloat);
             if (h0_dim == 1) total = fresh({H}, p, at::kFloat);
             if (H && (B || total.defined())) {
-                Tensor dh = grads[0], dlast = grads[1];
+                Tensor dh = plain(grads[0]), dlast = plain(grads[1]);
                 stes_gated_scan_args a{};
                 if (dh.defined()) {
                     // (a gradient that was expanded or transposed)
@@ -358,9 +362,10 @@ bool apart(const Tensor& t, int64_t width) {
     return out.second == 1 || out.first >= in.first * (in.second - 1) + width;
 }
 
-std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const Maybe& lengths_, bool reverse, const Maybe& out_, const Maybe& state_out_) {
-    Tensor h0 = h0_.value_or(Tensor()), lengths = lengths_.value_or(Tensor()), out = out_.value_or(Tensor()), state_out = state_out_.value_or(Tensor());
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre_, const Maybe& h0_, const Maybe& lengths_, bool reverse, const Maybe& out_, const Maybe& state_out_) {
     untraced(SCAN);
+    const Tensor pre = plain(pre_), lengths = plain(lengths_.value_or(Tensor())), out = out_.value_or(Tensor()), state_out = state_out_.value_or(Tensor());
+    Tensor h0 = plain(h0_.value_or(Tensor()));
     if (!pre.is_cuda() || pre.dim() != 3 || !element(pre)) refuse(SCAN, "pre must be a bfloat16 or float32 tensor [B, T, 2H] on the GPU");
     const int64_t B = pre.size(0), T = pre.size(1), W = pre.size(2), H = W / 2;
     const c10::Device dev = pre.device();
@@ -382,12 +387,12 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& pre, const Maybe& h0_, const
     const bool grad = asks_for_gradients(pre) || (h0.defined() && asks_for_gradients(h0));
     if (grad && (out.defined() || state_out.defined())) refuse(SCAN, "out and state_out are for calls without gradients");
     if (out.defined()) {
-        if (out.device() != dev || out.scalar_type() != pre.scalar_type() || out.dim() != 3 || out.size(0) != B || out.size(1) != T || out.size(2) != H || asks_for_gradients(out))
-            refuse(SCAN, "out must be ", pre.scalar_type(), " [", B, ", ", T, ", ", H, "] on ", dev, ", without gradients");
+        if (out.device() != dev || out.scalar_type() != pre.scalar_type() || out.dim() != 3 || out.size(0) != B || out.size(1) != T || out.size(2) != H || asks_for_gradients(out) || noted(out))
+            refuse(SCAN, "out must be ", pre.scalar_type(), " [", B, ", ", T, ", ", H, "] on ", dev, ", without gradients, with memory of its values");
         if ((H > 1 && out.stride(2) != 1) || !apart(out, H)) refuse(SCAN, "frames of out must be contiguous and not overlap");
     }
     if (state_out.defined()) {
-        if (state_out.device() != dev || asks_for_gradients(state_out)) refuse(SCAN, "state_out must be on ", dev, ", without gradients");
+        if (state_out.device() != dev || asks_for_gradients(state_out) || noted(state_out)) refuse(SCAN, "state_out must be on ", dev, ", without gradients, with memory of its values");
         const int64_t stride = row_stride(state_out, B, H, "state_out");
         if (h0.defined() && state_out.data_ptr() == h0.data_ptr() && B > 1 && (h0.dim() == 1 || h0.stride(0) != stride))
             refuse(SCAN, "a state in place is h0 itself, one row per sequence");
@@ -468,8 +473,9 @@ Tensor distill_call(stes_distill_args& a, const Tensor& logits) {
     return loss;
 }
 
-Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, double temperature, const Maybe& weight_, std::optional<double> denom) {
+Rows distill_check(const Tensor& logits_, const Tensor& idx_, const Tensor& val_, double temperature, const Maybe& weight_, std::optional<double> denom) {
     untraced(KL);
+    const Tensor logits = plain(logits_), idx = plain(idx_), val = plain(val_), weight = plain(weight_.value_or(Tensor()));
     if (!logits.is_cuda() || !element(logits) || logits.dim() < 1) refuse(KL, "logits must be a bfloat16 or float32 tensor [..., classes] on the GPU");
     const c10::Device dev = logits.device();
     const int64_t V = logits.size(-1);
@@ -480,7 +486,6 @@ Rows distill_check(const Tensor& logits, const Tensor& idx, const Tensor& val, d
     const int64_t k = idx.size(-1);
     if (k < 1 || k > STES_DISTILL_MAX_K) refuse(KL, "1 to ", STES_DISTILL_MAX_K, " teacher classes a row, got ", k);
     if (val.device() != dev || !element(val) || val.sizes() != idx.sizes()) refuse(KL, "val must be float32 or bfloat16 ", idx.sizes(), " on ", dev);
-    Tensor weight = weight_.value_or(Tensor());
     if (weight.defined() && (weight.device() != dev || weight.scalar_type() != at::kFloat || weight.sizes() != lead)) refuse(KL, "weight must be float32 ", lead, " on ", dev);
     if (asks_for_gradients(val) || (weight.defined() && asks_for_gradients(weight))) refuse(KL, "the teacher's logits and the weights are constants: detach them");
     no_tangents(KL, logits, val, weight);
@@ -515,7 +520,8 @@ struct DistillBackward : public Node {
             d = fresh(r.logits.sizes(), r.logits);
             if (r.logits.size(0)) {
                 stes_distill_args a = distill_args(r);
-                a.upstream = at_<float>(grads[0]);
+                const Tensor up = plain(grads[0]);
+                a.upstream = at_<float>(up);
                 a.stats = at_<float>(st);
                 into(a, d);
                 check(stes_distill_bwd(&a, stream_of(r.logits.device())), "stes_distill_bwd");
@@ -560,8 +566,8 @@ std::tuple<Tensor, Tensor> topk_distill_grad(const Tensor& logits, const Tensor&
     if (!out.defined()) {
         if (accumulate) refuse(KL, "accumulate adds to out");
         out = fresh(logits.sizes(), logits);
-    } else if (out.device() != logits.device() || !element(out) || out.sizes() != logits.sizes() || asks_for_gradients(out))
-        refuse(KL, "out must be float32 or bfloat16 ", logits.sizes(), " on ", logits.device(), ", without gradients");
+    } else if (out.device() != logits.device() || !element(out) || out.sizes() != logits.sizes() || asks_for_gradients(out) || noted(out))
+        refuse(KL, "out must be float32 or bfloat16 ", logits.sizes(), " on ", logits.device(), ", without gradients, with memory of its values");
     const int64_t V = out.size(-1);
     d = out.dim() == 2 ? out : out.reshape({-1, V});
     if (d.data_ptr() != out.data_ptr()) refuse(KL, "rows of out must be one stride apart");

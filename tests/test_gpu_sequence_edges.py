@@ -317,3 +317,44 @@ def test_saved_tensors_may_come_back_with_other_strides_and_are_refused_as_other
                 y = f(leaf)
             with pytest.raises(RuntimeError, match="came back as"):
                 torch.autograd.grad(y, leaf)
+
+
+def test_lazily_negated_and_lazily_zero_tensors():
+    """Tensors whose memory does not hold their values (torch's negative views, its zero tensors without memory) are read as their values;
+    results are not written through them."""
+    from spot_amd import lib
+    from spot_amd.distill import topk_distill_grad, topk_distill_loss
+    from spot_amd.recurrence import gated_scan
+    neg = torch._neg_view
+    pre, start, _, dh, dlast = _scan_inputs(2, 40, 8, F32, False, "rows", seed=3)
+    p, s, d, dl = pre.cuda().requires_grad_(), start.cuda().requires_grad_(), dh.cuda(), dlast.cuda()
+    zero = torch._efficientzerotensor(2, 8, device="cuda")
+
+    def scan(a, b, u, v):
+        y = gated_scan(a, b)
+        return y + torch.autograd.grad(y, (p, s), (u, v))
+    want = scan(p, s, d, dl)
+    for got in (scan(neg(-p), s, d, dl), scan(p, neg(-s), d, dl), scan(p, s, neg(-d), neg(-dl))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    z = torch.zeros(2, 8, device="cuda")
+    for a, b in zip(scan(p, s, d, zero), scan(p, s, d, z)):
+        assert torch.equal(a, b)
+    assert torch.equal(gated_scan(p.detach(), zero)[0], gated_scan(p.detach(), z)[0])
+    for kw in (dict(out=neg(torch.zeros(2, 40, 8, device="cuda"))), dict(state_out=neg(z.clone())), dict(state_out=torch._efficientzerotensor(2, 8, device="cuda"))):
+        with pytest.raises(lib.StesError):
+            gated_scan(p.detach(), **kw)
+    x, idx, val, w = _kl_inputs(9, 30, 4, F32, 2, False, True)
+    x, idx, val, w, up = x.cuda().requires_grad_(), idx.cuda(), val.cuda(), w.cuda(), torch.tensor(0.5, device="cuda")
+
+    def kl(a, v, wt, u):
+        y = topk_distill_loss(a, idx, v, 2.0, wt)
+        return (y, torch.autograd.grad(y, x, u)[0]) + topk_distill_grad(a, idx, v, 2.0, wt)
+    want = kl(x, val, w, up)
+    for got in (kl(neg(-x), val, w, up), kl(x, neg(-val), w, up), kl(x, val, neg(-w), up), kl(x, val, w, neg(-up))):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    none = kl(x, val, torch._efficientzerotensor(9, device="cuda"), torch._efficientzerotensor((), device="cuda"))
+    assert float(none[0]) == 0 and not bool(none[1].any()) and float(none[2]) == 0 and not bool(none[3].any())
+    g, = torch.autograd.grad(topk_distill_loss(x, idx, val), x, torch._efficientzerotensor((), device="cuda"))
+    assert not bool(g.any())
+    with pytest.raises(lib.StesError):
+        topk_distill_grad(x.detach(), idx, val, out=neg(torch.zeros(9, 30, device="cuda")))
