@@ -6,10 +6,10 @@
 // classes, k of V, are written over by the lanes that hold them.  Rows too long for a workgroup's registers are read twice (the
 // second time mostly from the cache).
 //
-// Measured (a copy of 1 GiB runs at 4,980 GB/s): loss and gradient in one pass of 8,192 x 32,003 bf16 203 us (5.2 TB/s); of
-// 2,048 x 50,001 fp32 loss 72 to 110 us and gradient 148 us (5.6 TB/s and, behind the gradient's writes, 3.7; 5.5 TB/s); 16,384 x 1,000
-// bf16 15 and 15 us (bound by the teacher's part of a row, some 200 instructions a wave, and its chain of loads: index, then logit);
-// short rows are bound by instructions too: 131,072 x 300 bf16 loss 52 us, gradient 65 us.
+// Measured (a copy of 1 GiB runs at 4,980 GB/s): loss and gradient in one pass of 8,192 x 32,003 bf16 205 us (5.1 TB/s); of
+// 2,048 x 50,001 fp32 loss 83 to 110 us and gradient 148 us (4.9 TB/s and, behind the gradient's writes, 3.7; 5.5 TB/s); 16,384 x 1,000
+// bf16 17 and 15 us (bound by the teacher's part of a row, some 200 instructions a wave, and its chain of loads: index, then logit);
+// short rows are bound by instructions too: 131,072 x 300 bf16 loss 55 us, gradient 57 us.
 #include "stes_common.h"
 
 namespace {
@@ -182,11 +182,11 @@ __device__ __forceinline__ float kl_part(float P, float s, float mx, float ls, f
 constexpr int MAX_ROUNDS = 1 << 22;                  // (an exit for broken zeros: the loss becomes NaN)
 
 // A workgroup's part of the loss (`sum` is thread 0's, in 64 bits: rows near 3e38 may pass fp32's range together, before `factor` divides them);
-// the only one of a launch is the loss.  With `p.zeros` the workgroups hand their parts to the last one, which adds them up in an order of its own: words that are valid when they are not zero (a part of 0 is 5e-324 instead), in relaxed
-// atomics of agent scope, and it leaves them zero.  One workgroup waits and the others wait for nothing: every wait ends.  Without them, and from
-// 16 parts a thread on, where reading them one after the other takes longer than a launch, distill_sum_kernel adds up.  Loss and
-// gradient of 1,024 x 7 4.4 us (two launches 6.3, one workgroup in one launch 9.7), of 16,384 x 1,000 20.4 (21.1); loss of 30,000 x 600,
-// 7,500 parts for 256 threads, 23.8 (22.6).
+// the only one of a launch is the loss.  With `p.zeros` the workgroups hand their parts to the last one, which adds them up in an order of its
+// own: words that are valid when they are not zero (a part of 0 is 5e-324 instead), in relaxed atomics of agent scope, and it leaves them
+// zero.  One workgroup waits and the others wait for nothing: every wait ends.  Without them, and from 16 parts a thread on, where reading
+// them one after the other takes longer than a launch, distill_sum_kernel adds up.  Loss and gradient of 1,024 x 7 4.4 us (two launches
+// 6.3, one workgroup in one launch 9.7), of 16,384 x 1,000 20.4 (21.1); loss of 30,000 x 600, 7,500 parts for 256 threads, 23.8 (22.6).
 __host__ __device__ inline bool in_one_launch(const stes_distill_args& p, int blocks, int threads) {
     return blocks == 1 || (p.zeros && blocks <= STES_DISTILL_WORDS && blocks <= 16 * threads);
 }

@@ -14,8 +14,9 @@
 // one beside it), so relaxed atomics of agent scope carry them and no fence or cache write-back is needed.
 //
 // Bound: memory, one read of the inputs and one write of the outputs.  Measured (bf16, 768 channels, a copy of 1 GiB runs at 4,980 GB/s):
-// one sequence of 65,536 frames forward 72 us (4.2 TB/s; 61 us without the joining, the rest is the walk back: 12 chains of 256
-// blocks), 8 x 4,096 frames forward 40 us (3.8 TB/s) and backward 65 us (3.9 TB/s), 16 x 64 frames 5.3 and 8.4 us.
+// one sequence of 65,536 frames forward 75 us (4.0 TB/s; 61 us without the joining, the rest is the walk back: 12 chains of 256
+// blocks), 8 x 4,096 frames forward 41.5 us (3.6 TB/s) and backward 67 us (3.8 TB/s), 16 x 64 frames 5.4 and 7.5 us.
+// (Comparisons here and below were made when the one sequence took 73 us: products that keep off 0 and gates that close cost the rest.)
 // Why 256 steps x 64 channels (512 threads): halving the steps doubles the walk (86 us instead of 73 on the one long sequence); 128
 // channels a row gain nothing over 64 (the lines of a row are whole either way); 32 would split them.  Why 4 steps a thread in bf16: with 8
 // (tiles of 128 steps x 128 channels) a thread needs 197 registers forward and 256 backward: 86 us instead of 73 and 152 instead of 122.

@@ -5,7 +5,6 @@
 // runs on autograd's device thread, where Python code finds another core's caches: clips of 16 x 64 x 768 forward and backward took 52 us
 // where the two threads shared a cache and 121 where they did not.
 #include <algorithm>
-#include <map>
 #include <memory>
 #include <mutex>
 #include <optional>
@@ -85,7 +84,6 @@ int f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 void written(const Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
-// (forward-mode tangents would be lost without a word)
 // A trace would record the allocation of a result and not the kernel that writes it.
 void untraced(const char* op) {
     using c10::impl::TorchDispatchModeKey;
@@ -94,6 +92,7 @@ void untraced(const char* op) {
     if (Modes::any_modes_set()) traced = traced || Modes::get_mode(TorchDispatchModeKey::PROXY) || Modes::get_mode(TorchDispatchModeKey::FAKE) || Modes::get_mode(TorchDispatchModeKey::FUNCTIONAL);
     if (traced) refuse(op, "cannot be traced (torch.jit.trace, make_fx): call it outside of what is recorded");
 }
+// (forward-mode tangents would be lost without a word)
 template <typename... Tensors>
 void no_tangents(const char* op, const Tensors&... t) {
     if ((... || (t.defined() && t._fw_grad(0).defined()))) refuse(op, "no forward-mode derivatives");

@@ -24,6 +24,8 @@ def gated_scan(pre, h0=None, lengths=None, reverse=False, out=None, state_out=No
              from that they share no memory with one another or with what the call reads (columns of one buffer do not)
     -> h [B, T, H] in pre's type and the states after the last step, float32 [B, H] (h0 where a sequence is empty)
 
+    A frame whose gates and candidates hold the type's lowest value leaves the states as they are; an infinite state stays infinite.
+
     Differentiable (once) in pre and h0, from h and from the final states; not to be traced.  T = 0 and T = 1 are calls like any other."""
     if not isinstance(pre, torch.Tensor):
         raise lib.StesError(f"gated_scan: pre must be a tensor, got {type(pre).__name__}")
