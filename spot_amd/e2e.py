@@ -307,7 +307,7 @@ class E2EModel(BaseRGBModel):
         shifts channels in time, a shorter T is zero-padded there; T = 1 is a frame at a time for the plain backbone; one clip without
         the leading dimension will do), while the
         minGRU head runs over a stream's W * T frames as one sequence that starts where the last call's ended: a video's scores
-        do not depend on how it is cut into calls."""
+        do not depend on which calls its clips come in (nor, for the plain backbone, on how it is cut into clips)."""
         self._check_causal()
         if seq.dim() == 4:
             seq = seq.unsqueeze(0)
@@ -326,6 +326,7 @@ class E2EModel(BaseRGBModel):
     def train_step(self, frame, label, xy, lr, fg_weight=5.0, grad_scale=1.0, ext_denoms=None, optimizer_step=True,
                    after_backward=None, grad_mul=1.0, on_ready=None, distill=None):
         """One optimisation step entirely on the device.  frame [B,T,C,H,W] f32 (normalised) or uint8 (decoded), label [B,T] int64, xy [B,T,2] f32.
+        All in the order of the video; a time_backward model turns them round itself.
         distill: {"idx", "val" [B,T,k], "temperature" 1.0, "weight" 1.0, "frame_weight" [B,T] or None, "denom" or None (all frames)}:
         `weight` times the distillation loss from a teacher's top logits (spot_amd.distill) joins the loss.
         Returns the device tensor {sum, cls, loc, sum of class weights, number of event frames, distillation loss (with distill), ...}
